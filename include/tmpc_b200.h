@@ -422,6 +422,121 @@ int32_t tmpc_riccati_solve_il_f32(const TmpcDims* dims, const float* factor, con
 int32_t tmpc_riccati_solve_il_f64(const TmpcDims* dims, const double* factor, const double* rhs, double* x_out,
                                   tmpc_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Sequence operators of a learned policy around the solve: the encoder that
+ * reads an environment's history and emits cost parameters.  No counterpart
+ * in the reference.  _f32: float elements, _bf16: bfloat16 elements; sums,
+ * states and statistics are float in both, and rounded once when stored.
+ * ------------------------------------------------------------------------- */
+
+/* A [batch][token][head][dim] tensor: element strides of the first three
+ * axes, the last axis contiguous. */
+typedef struct TmpcSeqView {
+  void* ptr;
+  int64_t batch;
+  int64_t token;
+  int64_t head;
+} TmpcSeqView;
+
+typedef struct TmpcLinAttnDims {
+  int32_t B;  /* sequences */
+  int32_t T;  /* tokens per sequence */
+  int32_t H;  /* query heads; a state and a decay each */
+  int32_t G;  /* key / value heads, G divides H; query head h reads key head h / (H / G) */
+  int32_t dk; /* query / key size, 1 .. 128 */
+  int32_t dv; /* value size, 1 .. 128 */
+} TmpcLinAttnDims;
+
+/* Linear attention with a decay per head, d_h = exp(log_decay[h]):
+ *     S_t = d_h S_{t-1} + k_t v_t^T      (dk x dv, float)
+ *     o_t = scale S_t^T q_t
+ * log_decay [H] float; lengths [B] int32 or NULL: tokens t >= lengths[b]
+ * (clamped to 0 .. T) give o_t = 0 and leave the state alone.  state_in,
+ * state_out [B][H][dk][dv] float: the state before the first and after the
+ * last token; state_in NULL is zero, state_out NULL is not written; they may
+ * be the same buffer. */
+size_t tmpc_linear_attention_workspace_bytes(const TmpcLinAttnDims* dims);
+int32_t tmpc_linear_attention_f32(const TmpcLinAttnDims* dims, const TmpcSeqView* q, const TmpcSeqView* k,
+                                  const TmpcSeqView* v, const TmpcSeqView* o, const float* log_decay,
+                                  const int32_t* lengths, const float* state_in, float* state_out, double scale,
+                                  void* workspace, size_t workspace_bytes, tmpc_stream_t stream);
+int32_t tmpc_linear_attention_bf16(const TmpcLinAttnDims* dims, const TmpcSeqView* q, const TmpcSeqView* k,
+                                   const TmpcSeqView* v, const TmpcSeqView* o, const float* log_decay,
+                                   const int32_t* lengths, const float* state_in, float* state_out, double scale,
+                                   void* workspace, size_t workspace_bytes, tmpc_stream_t stream);
+/* Its gradient: dout the gradient of o, dstate_out that of the final state
+ * (NULL: zero).  dq, dk, dv as q, k, v (gradients of shared key / value heads
+ * summed over their query heads); dlog_decay [H] and dstate_in may be NULL. */
+size_t tmpc_linear_attention_backward_workspace_bytes(const TmpcLinAttnDims* dims);
+int32_t tmpc_linear_attention_backward_f32(const TmpcLinAttnDims* dims, const TmpcSeqView* q, const TmpcSeqView* k,
+                                           const TmpcSeqView* v, const TmpcSeqView* dout, const TmpcSeqView* dq,
+                                           const TmpcSeqView* dk, const TmpcSeqView* dv, const float* log_decay,
+                                           const int32_t* lengths, const float* state_in, const float* dstate_out,
+                                           float* dlog_decay, float* dstate_in, double scale, void* workspace,
+                                           size_t workspace_bytes, tmpc_stream_t stream);
+int32_t tmpc_linear_attention_backward_bf16(const TmpcLinAttnDims* dims, const TmpcSeqView* q, const TmpcSeqView* k,
+                                            const TmpcSeqView* v, const TmpcSeqView* dout, const TmpcSeqView* dq,
+                                            const TmpcSeqView* dk, const TmpcSeqView* dv, const float* log_decay,
+                                            const int32_t* lengths, const float* state_in, const float* dstate_out,
+                                            float* dlog_decay, float* dstate_in, double scale, void* workspace,
+                                            size_t workspace_bytes, tmpc_stream_t stream);
+/* One token per sequence (dims->T is not read; the token strides of the views
+ * neither): state_out = d_h state_in + k v^T, o = scale state_out^T q.
+ * state_in and state_out [B][H][dk][dv] may be the same buffer. */
+int32_t tmpc_linear_attention_step_f32(const TmpcLinAttnDims* dims, const TmpcSeqView* q, const TmpcSeqView* k,
+                                       const TmpcSeqView* v, const TmpcSeqView* o, const float* log_decay,
+                                       const float* state_in, float* state_out, double scale, tmpc_stream_t stream);
+int32_t tmpc_linear_attention_step_bf16(const TmpcLinAttnDims* dims, const TmpcSeqView* q, const TmpcSeqView* k,
+                                        const TmpcSeqView* v, const TmpcSeqView* o, const float* log_decay,
+                                        const float* state_in, float* state_out, double scale, tmpc_stream_t stream);
+
+/* Residual addition with its root-mean-square norm, rows of d (1 .. 16384)
+ * elements: t = x + residual, y = t (mean(t^2) + eps)^(-1/2) weight.
+ * x and residual have row strides (elements); y, sum (t) are contiguous.
+ * residual NULL: t = x, and sum may be NULL.  inv_rms [rows] or NULL keeps
+ * (mean(t^2) + eps)^(-1/2) for the backward pass. */
+int32_t tmpc_add_rms_norm_f32(int64_t rows, int32_t d, const void* x, int64_t x_stride, const void* residual,
+                              int64_t residual_stride, const void* weight, double eps, void* y, void* sum,
+                              float* inv_rms, tmpc_stream_t stream);
+int32_t tmpc_add_rms_norm_bf16(int64_t rows, int32_t d, const void* x, int64_t x_stride, const void* residual,
+                               int64_t residual_stride, const void* weight, double eps, void* y, void* sum,
+                               float* inv_rms, tmpc_stream_t stream);
+/* Gradient: dy and dsum (NULL: zero) of y and sum, all contiguous; dx is the
+ * gradient of x and of residual, dweight [d] is overwritten. */
+size_t tmpc_add_rms_norm_workspace_bytes(int64_t rows, int32_t d);
+int32_t tmpc_add_rms_norm_backward_f32(int64_t rows, int32_t d, const void* dy, const void* dsum, const void* sum,
+                                       const void* weight, const float* inv_rms, void* dx, void* dweight,
+                                       void* workspace, size_t workspace_bytes, tmpc_stream_t stream);
+int32_t tmpc_add_rms_norm_backward_bf16(int64_t rows, int32_t d, const void* dy, const void* dsum, const void* sum,
+                                        const void* weight, const float* inv_rms, void* dx, void* dweight,
+                                        void* workspace, size_t workspace_bytes, tmpc_stream_t stream);
+
+/* Gated linear layer: h = act(x w_gate^T) * (x w_up^T), x [rows][d],
+ * w_gate, w_up [f][d], h [rows][f], contiguous; act: TMPC_ACT_*.
+ * gate, up [rows][f] or NULL keep the two products for the backward pass. */
+#define TMPC_ACT_SILU 0 /* g / (1 + exp(-g)) */
+#define TMPC_ACT_GELU 1 /* g (1 + erf(g / sqrt 2)) / 2 */
+size_t tmpc_gated_linear_workspace_bytes(int64_t rows, int32_t d, int32_t f, int32_t elem_size);
+int32_t tmpc_gated_linear_f32(int64_t rows, int32_t d, int32_t f, const void* x, const void* w_gate,
+                              const void* w_up, int32_t act, void* h, void* gate, void* up, void* workspace,
+                              size_t workspace_bytes, tmpc_stream_t stream);
+int32_t tmpc_gated_linear_bf16(int64_t rows, int32_t d, int32_t f, const void* x, const void* w_gate,
+                               const void* w_up, int32_t act, void* h, void* gate, void* up, void* workspace,
+                               size_t workspace_bytes, tmpc_stream_t stream);
+/* Gradient from gate, up (kept by the forward pass) and dh [rows][f]:
+ *     dg = dh up act'(gate), du = dh act(gate)
+ *     dx = dg w_gate + du w_up,  dw_gate = dg^T x,  dw_up = du^T x
+ * dx, or dw_gate and dw_up together, may be NULL. */
+size_t tmpc_gated_linear_backward_workspace_bytes(int64_t rows, int32_t d, int32_t f, int32_t elem_size);
+int32_t tmpc_gated_linear_backward_f32(int64_t rows, int32_t d, int32_t f, const void* x, const void* w_gate,
+                                       const void* w_up, int32_t act, const void* gate, const void* up,
+                                       const void* dh, void* dx, void* dw_gate, void* dw_up, void* workspace,
+                                       size_t workspace_bytes, tmpc_stream_t stream);
+int32_t tmpc_gated_linear_backward_bf16(int64_t rows, int32_t d, int32_t f, const void* x, const void* w_gate,
+                                        const void* w_up, int32_t act, const void* gate, const void* up,
+                                        const void* dh, void* dx, void* dw_gate, void* dw_up, void* workspace,
+                                        size_t workspace_bytes, tmpc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

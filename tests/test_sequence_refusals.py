@@ -1,0 +1,126 @@
+"""The sequence operators' checks of their arguments, on the host: every call
+here is refused before anything is launched."""
+import ctypes as C
+
+import pytest
+import torch
+
+from turbompc_b200 import _ffi, sequence
+
+
+def test_wrappers_refuse_host_tensors_and_wrong_types():
+    q = torch.zeros(2, 3, 4, 16)
+    g = torch.zeros(4)
+    with pytest.raises(ValueError, match="CUDA"):
+        sequence.linear_attention(q, q, q, g)
+    with pytest.raises(ValueError, match="CUDA"):
+        sequence.linear_attention_step(q[:, 0], q[:, 0], q[:, 0], g, torch.zeros(2, 4, 16, 16))
+    with pytest.raises(ValueError, match="CUDA"):
+        sequence.add_rms_norm(q, q, torch.ones(16))
+    with pytest.raises(ValueError, match="CUDA"):
+        sequence.gated_linear(q, torch.zeros(8, 16), torch.zeros(8, 16))
+    for bad in (torch.float64, torch.float16):
+        with pytest.raises(TypeError):
+            sequence.linear_attention(q.to(bad), q.to(bad), q.to(bad), g)
+        with pytest.raises(TypeError):
+            sequence.add_rms_norm(q.to(bad), None, torch.ones(16, dtype=bad))
+        with pytest.raises(TypeError):
+            sequence.gated_linear(q.to(bad), torch.zeros(8, 16, dtype=bad), torch.zeros(8, 16, dtype=bad))
+    with pytest.raises(TypeError):
+        sequence.linear_attention([1.0], q, q, g)
+    with pytest.raises(ValueError, match="activation"):
+        sequence.gated_linear(q, torch.zeros(8, 16), torch.zeros(8, 16), activation="relu")
+
+
+def test_entry_points_report_argument_errors():
+    lib = _ffi.load()
+    view = _ffi.TmpcSeqView(None, 0, 0, 0)
+    v = C.byref(view)
+
+    def attention(dims, fn="tmpc_linear_attention_f32"):
+        return getattr(lib, fn)(C.byref(dims) if dims else None, v, v, v, v, None, None, None, None, 1.0, None, 0, None)
+
+    D = _ffi.TmpcLinAttnDims
+    assert attention(None) == -1
+    for bad in (D(-1, 1, 1, 1, 16, 16), D(1, -1, 1, 1, 16, 16), D(1, 1, 3, 2, 16, 16), D(1, 1, 0, 1, 16, 16),
+                D(1, 1, 1, 0, 16, 16), D(1, 1, 1, 1, 0, 16), D(1, 1, 1, 1, 16, 0)):
+        for fn in ("tmpc_linear_attention_f32", "tmpc_linear_attention_bf16"):
+            assert attention(bad, fn) == -2
+    assert attention(D(1, 1, 1, 1, 129, 16)) == -3
+    assert attention(D(1, 1, 1, 1, 16, 129)) == -3
+    assert attention(D(0, 1, 1, 1, 16, 16)) == 0  # an empty batch launches nothing
+    assert attention(D(1, 1, 1, 1, 16, 16)) == -1  # null tensors
+    for s in ("f32", "bf16"):
+        step = getattr(lib, f"tmpc_linear_attention_step_{s}")
+        assert step(C.byref(D(1, 1, 3, 2, 16, 16)), v, v, v, v, None, None, None, 1.0, None) == -2
+        assert step(C.byref(D(1, 1, 1, 1, 256, 16)), v, v, v, v, None, None, None, 1.0, None) == -3
+        assert step(C.byref(D(1, 1, 1, 1, 16, 16)), v, v, v, v, None, None, None, 1.0, None) == -1
+        back = getattr(lib, f"tmpc_linear_attention_backward_{s}")
+        args = [v] * 7 + [None] * 6 + [1.0, None, 0, None]
+        assert back(C.byref(D(1, 1, 2, 3, 16, 16)), *args) == -2
+        assert back(C.byref(D(1, 1, 1, 1, 16, 16)), *args) == -1
+        norm = getattr(lib, f"tmpc_add_rms_norm_{s}")
+        assert norm(-1, 16, None, 16, None, 0, None, 1e-6, None, None, None, None) == -2
+        assert norm(1, 0, None, 0, None, 0, None, 1e-6, None, None, None, None) == -2
+        assert norm(1, 16385, None, 16385, None, 0, None, 1e-6, None, None, None, None) == -3
+        assert norm(1, 16, None, 16, None, 0, None, 1e-6, None, None, None, None) == -1
+        gated = getattr(lib, f"tmpc_gated_linear_{s}")
+        assert gated(-1, 16, 16, None, None, None, 0, None, None, None, None, 0, None) == -2
+        assert gated(1, 0, 16, None, None, None, 0, None, None, None, None, 0, None) == -2
+        assert gated(1, 16, 16, None, None, None, 7, None, None, None, None, 0, None) == -3
+        assert gated(1, 16, 16, None, None, None, 0, None, None, None, None, 0, None) == -1
+        assert gated(0, 16, 16, None, None, None, 0, None, None, None, None, 0, None) == 0
+
+
+def test_workspace_sizes():
+    lib = _ffi.load()
+    D = _ffi.TmpcLinAttnDims
+    assert lib.tmpc_linear_attention_workspace_bytes(C.byref(D(1, 1, 3, 2, 16, 16))) == 0  # invalid
+    assert lib.tmpc_linear_attention_backward_workspace_bytes(C.byref(D(2, 64, 4, 2, 64, 64))) > 0
+    assert lib.tmpc_add_rms_norm_workspace_bytes(100, 512) >= 512 * 4
+    assert lib.tmpc_gated_linear_backward_workspace_bytes(100, 64, 128, 2) >= 2 * 100 * 128 * 2
+
+
+@pytest.mark.gpu
+def test_wrappers_refuse_shapes_and_devices():
+    z = lambda *s, dtype=torch.float32: torch.zeros(*s, device="cuda", dtype=dtype)
+    q, g = z(2, 3, 4, 16), z(4)
+    bad = [
+        dict(q=z(2, 3, 16)), dict(k=z(2, 3, 3, 16)), dict(k=z(2, 4, 4, 16)), dict(v=z(2, 3, 2, 16)),
+        dict(k=z(2, 3, 4, 8)), dict(log_decay=z(3)), dict(log_decay=z(4, 1)),
+        dict(initial_state=z(2, 4, 16, 8)), dict(lengths=torch.zeros(3, dtype=torch.int32, device="cuda")),
+        dict(v=z(2, 3, 4, 129)), dict(lengths=torch.zeros(2, dtype=torch.int32)), dict(log_decay=torch.zeros(4)),
+        dict(k=z(2, 3, 0, 16), v=z(2, 3, 0, 16)),
+    ]
+    for b in bad:
+        a = dict(dict(q=q, k=q, v=q, log_decay=g), **b)
+        with pytest.raises(ValueError):
+            sequence.linear_attention(a.pop("q"), a.pop("k"), a.pop("v"), a.pop("log_decay"), **a)
+    for b in (dict(k=q.bfloat16()), dict(log_decay=g.double()), dict(initial_state=z(2, 4, 16, 16, dtype=torch.float64)),
+              dict(lengths=torch.zeros(2, dtype=torch.int64, device="cuda"))):
+        a = dict(dict(q=q, k=q, v=q, log_decay=g), **b)
+        with pytest.raises(TypeError):
+            sequence.linear_attention(a.pop("q"), a.pop("k"), a.pop("v"), a.pop("log_decay"), **a)
+    t, S = q[:, 0], z(2, 4, 16, 16)
+    with pytest.raises(ValueError, match="contiguous"):
+        sequence.linear_attention_step(t, t, t, g, S.transpose(2, 3))
+    with pytest.raises(ValueError):
+        sequence.linear_attention_step(t, t, t, g, S, state_out=z(2, 4, 16, 8))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        sequence.linear_attention_step(t.clone().requires_grad_(True), t, t, g, S)
+    with pytest.raises(ValueError):
+        sequence.add_rms_norm(q, q[:1], z(16))
+    with pytest.raises(ValueError):
+        sequence.add_rms_norm(q, q, z(15))
+    with pytest.raises(ValueError):
+        sequence.add_rms_norm(z(2, 16385), None, z(16385))
+    with pytest.raises(TypeError):
+        sequence.add_rms_norm(q, q.bfloat16(), z(16))
+    with pytest.raises(ValueError):
+        sequence.gated_linear(q, z(8, 15), z(8, 15))
+    with pytest.raises(ValueError):
+        sequence.gated_linear(q, z(8, 16), z(9, 16))
+    with pytest.raises(ValueError):
+        sequence.gated_linear(q, z(16), z(16))
+    with pytest.raises(TypeError):
+        sequence.gated_linear(q, z(8, 16, dtype=torch.bfloat16), z(8, 16))

@@ -29,6 +29,14 @@ class TmpcAdmmState(C.Structure):
     _fields_ = [(k, C.c_void_p) for k in ("x", "y_g", "y_f0", "y_fdyn", "z_g", "xi_g", "rho_bar")]
 
 
+class TmpcSeqView(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("batch", C.c_int64), ("token", C.c_int64), ("head", C.c_int64)]
+
+
+class TmpcLinAttnDims(C.Structure):
+    _fields_ = [(k, C.c_int32) for k in ("B", "T", "H", "G", "dk", "dv")]
+
+
 class TmpcAdmmConfig(C.Structure):
     _fields_ = [("max_iter", C.c_int32), ("pcg_max_iter", C.c_int32), ("check_every", C.c_int32),
                 ("adapt_rho_every", C.c_int32), ("eps_abs", C.c_double), ("eps_rel", C.c_double),
@@ -42,6 +50,8 @@ LINSYS_DIRECT = 1
 LINSYS_PCG_PACKED = 2
 LAYOUT_REFERENCE = 0
 LAYOUT_INTERLEAVED = 1
+ACT_SILU = 0
+ACT_GELU = 1
 MODEL_QUADROTOR12 = 1
 MODEL_CLOHESSY_WILTSHIRE = 2
 
@@ -99,6 +109,27 @@ for _s in ("f32", "f64"):
     _SIGS[f"tmpc_admm_solve_{_s}"] = (C.c_int32, [C.POINTER(TmpcDims), C.POINTER(TmpcQP),
                                                   C.POINTER(TmpcAdmmState), C.POINTER(TmpcAdmmState), _P,
                                                   C.POINTER(TmpcAdmmConfig), _P, _P, _P, _P, C.c_size_t, _P])
+# Sequence operators: float and bfloat16 elements.
+_V = C.POINTER(TmpcSeqView)
+_LA = C.POINTER(TmpcLinAttnDims)
+_SIGS["tmpc_linear_attention_workspace_bytes"] = (C.c_size_t, [_LA])
+_SIGS["tmpc_linear_attention_backward_workspace_bytes"] = (C.c_size_t, [_LA])
+_SIGS["tmpc_add_rms_norm_workspace_bytes"] = (C.c_size_t, [C.c_int64, C.c_int32])
+_SIGS["tmpc_gated_linear_workspace_bytes"] = (C.c_size_t, [C.c_int64] + [C.c_int32] * 3)
+_SIGS["tmpc_gated_linear_backward_workspace_bytes"] = (C.c_size_t, [C.c_int64] + [C.c_int32] * 3)
+for _s in ("f32", "bf16"):
+    _SIGS[f"tmpc_linear_attention_{_s}"] = (C.c_int32, [_LA] + [_V] * 4 + [_P] * 4 +
+                                            [C.c_double, _P, C.c_size_t, _P])
+    _SIGS[f"tmpc_linear_attention_backward_{_s}"] = (C.c_int32, [_LA] + [_V] * 7 + [_P] * 6 +
+                                                     [C.c_double, _P, C.c_size_t, _P])
+    _SIGS[f"tmpc_linear_attention_step_{_s}"] = (C.c_int32, [_LA] + [_V] * 4 + [_P] * 3 + [C.c_double, _P])
+    _SIGS[f"tmpc_add_rms_norm_{_s}"] = (C.c_int32, [C.c_int64, C.c_int32, _P, C.c_int64, _P, C.c_int64, _P,
+                                                    C.c_double, _P, _P, _P, _P])
+    _SIGS[f"tmpc_add_rms_norm_backward_{_s}"] = (C.c_int32, [C.c_int64, C.c_int32] + [_P] * 8 + [C.c_size_t, _P])
+    _SIGS[f"tmpc_gated_linear_{_s}"] = (C.c_int32, [C.c_int64, C.c_int32, C.c_int32] + [_P] * 3 + [C.c_int32] +
+                                        [_P] * 4 + [C.c_size_t, _P])
+    _SIGS[f"tmpc_gated_linear_backward_{_s}"] = (C.c_int32, [C.c_int64, C.c_int32, C.c_int32] + [_P] * 3 +
+                                                 [C.c_int32] + [_P] * 7 + [C.c_size_t, _P])
 
 _lib = None
 _lock = threading.Lock()

@@ -1,0 +1,119 @@
+// Linear attention, one token per sequence:
+//     S' = d S + k v^T,   o = s S'^T q
+// Bound by HBM: every state element is read and written once (8 bytes each).
+// A block owns one (sequence, head); its threads are laid out as CG column
+// groups of VEC columns by 128 / CG row lanes, so that consecutive threads
+// read consecutive addresses; a thread requests ROWS rows before it uses the
+// first.  The row lanes' partial read-outs meet in shared memory.
+#include "seq_common.cuh"
+
+namespace tmpc {
+namespace seq {
+
+constexpr int kStepThreads = 128;
+
+struct StepArgs {
+  TmpcSeqView q, k, v, o;
+  const float* log_decay;
+  const float* state_in;
+  float* state_out;
+  int H, G, dk, dv, col_groups, row_lanes;
+  float scale;
+};
+
+template <typename T, int VEC, int ROWS>
+__global__ void __launch_bounds__(kStepThreads) step_kernel(const StepArgs a) {
+  using P = Pack<float, VEC>;
+  __shared__ float sq[128], sk[128], part[kStepThreads * VEC];
+  const int64_t bh = blockIdx.x;
+  const int64_t b = bh / a.H;
+  const int h = (int)(bh % a.H), g = h / (a.H / a.G);
+  const int cg = threadIdx.x % a.col_groups, rl = threadIdx.x / a.col_groups;
+  const bool on = rl < a.row_lanes;
+  const float* in = a.state_in + bh * a.dk * a.dv + cg * VEC;
+  float* out = a.state_out + bh * a.dk * a.dv + cg * VEC;
+  P s[ROWS];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const int i = i0 + r * a.row_lanes;
+      if (on && i < a.dk) s[r] = *reinterpret_cast<const P*>(in + (int64_t)i * a.dv);
+    }
+  };
+  load(rl);
+  if (threadIdx.x < a.dk) {
+    sq[threadIdx.x] = to_f((static_cast<const T*>(a.q.ptr) + b * a.q.batch + h * a.q.head)[threadIdx.x]) * a.scale;
+    sk[threadIdx.x] = to_f((static_cast<const T*>(a.k.ptr) + b * a.k.batch + g * a.k.head)[threadIdx.x]);
+  }
+  float v[VEC], o[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    v[e] = on ? to_f((static_cast<const T*>(a.v.ptr) + b * a.v.batch + g * a.v.head)[cg * VEC + e]) : 0.f;
+    o[e] = 0.f;
+  }
+  const float dec = exp2f(fmaxf(a.log_decay[h] * 1.4426950408889634f, -1e4f));
+  __syncthreads();
+  for (int i0 = rl; i0 < a.dk; i0 += ROWS * a.row_lanes) {
+    if (i0 != rl) load(i0);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const int i = i0 + r * a.row_lanes;
+      if (on && i < a.dk) {
+        const float k = sk[i], q = sq[i];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          s[r].v[e] = fmaf(dec, s[r].v[e], k * v[e]);
+          o[e] = fmaf(q, s[r].v[e], o[e]);
+        }
+        *reinterpret_cast<P*>(out + (int64_t)i * a.dv) = s[r];
+      }
+    }
+  }
+  if (on) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) part[rl * a.dv + cg * VEC + e] = o[e];
+  }
+  __syncthreads();
+  if (threadIdx.x < a.dv) {
+    float t = 0.f;
+    for (int r = 0; r < a.row_lanes; ++r) t += part[r * a.dv + threadIdx.x];
+    (static_cast<T*>(a.o.ptr) + b * a.o.batch + h * a.o.head)[threadIdx.x] = from_f<T>(t);
+  }
+}
+
+template <typename T>
+int step(const TmpcLinAttnDims* d, const TmpcSeqView* q, const TmpcSeqView* k, const TmpcSeqView* v,
+         const TmpcSeqView* o, const float* log_decay, const float* state_in, float* state_out, double scale,
+         cudaStream_t st) {
+  if (!d) return TMPC_ERR_NULL_ARG;
+  if (d->B < 0 || d->H < 1 || d->G < 1 || d->H % d->G || d->dk < 1 || d->dv < 1) return TMPC_ERR_BAD_DIMS;
+  if (d->dk > 128 || d->dv > 128 || (int64_t)d->B * d->H > INT32_MAX) return TMPC_ERR_UNSUPPORTED;
+  if (d->B == 0) return TMPC_OK;
+  if (!q || !k || !v || !o || !log_decay || !state_in || !state_out) return TMPC_ERR_NULL_ARG;
+  if (!q->ptr || !k->ptr || !v->ptr || !o->ptr) return TMPC_ERR_NULL_ARG;
+  StepArgs a{*q, *k, *v, *o, log_decay, state_in, state_out, d->H, d->G, d->dk, d->dv, 0, 0, (float)scale};
+  const bool vec = d->dv % 4 == 0 && aligned(state_in, 16) && aligned(state_out, 16);
+  a.col_groups = vec ? d->dv / 4 : d->dv;
+  a.row_lanes = kStepThreads / a.col_groups;
+  const unsigned grid = (unsigned)(d->B * d->H);
+  if (vec) step_kernel<T, 4, 8><<<grid, kStepThreads, 0, st>>>(a);
+  else step_kernel<T, 1, 16><<<grid, kStepThreads, 0, st>>>(a);
+  return (int)cudaPeekAtLastError();
+}
+
+}  // namespace seq
+}  // namespace tmpc
+
+extern "C" {
+
+#define TMPC_STEP_ENTRY(SUF, T)                                                                                      \
+  int32_t tmpc_linear_attention_step_##SUF(const TmpcLinAttnDims* dims, const TmpcSeqView* q, const TmpcSeqView* k,  \
+                                           const TmpcSeqView* v, const TmpcSeqView* o, const float* log_decay,       \
+                                           const float* state_in, float* state_out, double scale,                    \
+                                           tmpc_stream_t stream) {                                                   \
+    return tmpc::seq::step<T>(dims, q, k, v, o, log_decay, state_in, state_out, scale, (cudaStream_t)stream);        \
+  }
+TMPC_STEP_ENTRY(f32, float)
+TMPC_STEP_ENTRY(bf16, __nv_bfloat16)
+
+}  // extern "C"

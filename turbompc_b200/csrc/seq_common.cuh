@@ -1,0 +1,50 @@
+// Shared pieces of the sequence operators (linear attention, residual norm,
+// gated linear layer): element types, conversions, warp sums.
+//
+// Elements are float or __nv_bfloat16; every sum, state and statistic is held
+// in float and rounded once, to nearest even, when an output is stored.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "tmpc_b200.h"
+
+namespace tmpc {
+namespace seq {
+
+using bf16 = __nv_bfloat16;
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(bf16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f(float x);
+template <>
+__device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ bf16 from_f<bf16>(float x) { return __float2bfloat16_rn(x); }
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// N consecutive elements moved as one access of N * sizeof(T) bytes.
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack {
+  T v[N];
+};
+
+inline int sm_count() {
+  int dev = 0, v = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess) return v;
+  if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) v = 148;
+  return v;
+}
+
+inline bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+}  // namespace seq
+}  // namespace tmpc

@@ -512,30 +512,33 @@ int32_t tmpc_add_rms_norm_backward_bf16(int64_t rows, int32_t d, const void* dy,
                                         void* workspace, size_t workspace_bytes, tmpc_stream_t stream);
 
 /* Gated linear layer: h = act(x w_gate^T) * (x w_up^T), x [rows][d],
- * w_gate, w_up [f][d], h [rows][f], contiguous; act: TMPC_ACT_*.
- * gate, up [rows][f] or NULL keep the two products for the backward pass. */
+ * w_gate, w_up [f][d], h [rows][f], contiguous; x, w_gate and w_up 16-byte
+ * aligned (else TMPC_ERR_UNSUPPORTED); act: TMPC_ACT_*.  Products of float
+ * tensors are formed from three bfloat16 components each, exact to 2^-24; a
+ * row holding an infinity may give NaN where float arithmetic gives infinity.
+ * The kernels' waits are bounded (tmpc_set_transfer_poll_limit): after a
+ * time-out the outputs not computed are NaN. */
 #define TMPC_ACT_SILU 0 /* g / (1 + exp(-g)) */
 #define TMPC_ACT_GELU 1 /* g (1 + erf(g / sqrt 2)) / 2 */
 size_t tmpc_gated_linear_workspace_bytes(int64_t rows, int32_t d, int32_t f, int32_t elem_size);
 int32_t tmpc_gated_linear_f32(int64_t rows, int32_t d, int32_t f, const void* x, const void* w_gate,
-                              const void* w_up, int32_t act, void* h, void* gate, void* up, void* workspace,
-                              size_t workspace_bytes, tmpc_stream_t stream);
+                              const void* w_up, int32_t act, void* h, void* workspace, size_t workspace_bytes,
+                              tmpc_stream_t stream);
 int32_t tmpc_gated_linear_bf16(int64_t rows, int32_t d, int32_t f, const void* x, const void* w_gate,
-                               const void* w_up, int32_t act, void* h, void* gate, void* up, void* workspace,
-                               size_t workspace_bytes, tmpc_stream_t stream);
-/* Gradient from gate, up (kept by the forward pass) and dh [rows][f]:
- *     dg = dh up act'(gate), du = dh act(gate)
+                               const void* w_up, int32_t act, void* h, void* workspace, size_t workspace_bytes,
+                               tmpc_stream_t stream);
+/* Gradient from x, the weights and dh [rows][f] (both projections are
+ * recomputed):
+ *     dg = dh u act'(g), du = dh act(g),  g = x w_gate^T, u = x w_up^T
  *     dx = dg w_gate + du w_up,  dw_gate = dg^T x,  dw_up = du^T x
  * dx, or dw_gate and dw_up together, may be NULL. */
 size_t tmpc_gated_linear_backward_workspace_bytes(int64_t rows, int32_t d, int32_t f, int32_t elem_size);
 int32_t tmpc_gated_linear_backward_f32(int64_t rows, int32_t d, int32_t f, const void* x, const void* w_gate,
-                                       const void* w_up, int32_t act, const void* gate, const void* up,
-                                       const void* dh, void* dx, void* dw_gate, void* dw_up, void* workspace,
-                                       size_t workspace_bytes, tmpc_stream_t stream);
+                                       const void* w_up, int32_t act, const void* dh, void* dx, void* dw_gate,
+                                       void* dw_up, void* workspace, size_t workspace_bytes, tmpc_stream_t stream);
 int32_t tmpc_gated_linear_backward_bf16(int64_t rows, int32_t d, int32_t f, const void* x, const void* w_gate,
-                                        const void* w_up, int32_t act, const void* gate, const void* up,
-                                        const void* dh, void* dx, void* dw_gate, void* dw_up, void* workspace,
-                                        size_t workspace_bytes, tmpc_stream_t stream);
+                                        const void* w_up, int32_t act, const void* dh, void* dx, void* dw_gate,
+                                        void* dw_up, void* workspace, size_t workspace_bytes, tmpc_stream_t stream);
 
 #ifdef __cplusplus
 }

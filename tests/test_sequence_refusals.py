@@ -65,11 +65,11 @@ def test_entry_points_report_argument_errors():
         assert norm(1, 16385, None, 16385, None, 0, None, 1e-6, None, None, None, None) == -3
         assert norm(1, 16, None, 16, None, 0, None, 1e-6, None, None, None, None) == -1
         gated = getattr(lib, f"tmpc_gated_linear_{s}")
-        assert gated(-1, 16, 16, None, None, None, 0, None, None, None, None, 0, None) == -2
-        assert gated(1, 0, 16, None, None, None, 0, None, None, None, None, 0, None) == -2
-        assert gated(1, 16, 16, None, None, None, 7, None, None, None, None, 0, None) == -3
-        assert gated(1, 16, 16, None, None, None, 0, None, None, None, None, 0, None) == -1
-        assert gated(0, 16, 16, None, None, None, 0, None, None, None, None, 0, None) == 0
+        assert gated(-1, 16, 16, None, None, None, 0, None, None, 0, None) == -2
+        assert gated(1, 0, 16, None, None, None, 0, None, None, 0, None) == -2
+        assert gated(1, 16, 16, None, None, None, 7, None, None, 0, None) == -3
+        assert gated(1, 16, 16, None, None, None, 0, None, None, 0, None) == -1
+        assert gated(0, 16, 16, None, None, None, 0, None, None, 0, None) == 0
 
 
 def test_workspace_sizes():

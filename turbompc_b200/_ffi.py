@@ -127,9 +127,9 @@ for _s in ("f32", "bf16"):
                                                     C.c_double, _P, _P, _P, _P])
     _SIGS[f"tmpc_add_rms_norm_backward_{_s}"] = (C.c_int32, [C.c_int64, C.c_int32] + [_P] * 8 + [C.c_size_t, _P])
     _SIGS[f"tmpc_gated_linear_{_s}"] = (C.c_int32, [C.c_int64, C.c_int32, C.c_int32] + [_P] * 3 + [C.c_int32] +
-                                        [_P] * 4 + [C.c_size_t, _P])
+                                        [_P] * 2 + [C.c_size_t, _P])
     _SIGS[f"tmpc_gated_linear_backward_{_s}"] = (C.c_int32, [C.c_int64, C.c_int32, C.c_int32] + [_P] * 3 +
-                                                 [C.c_int32] + [_P] * 7 + [C.c_size_t, _P])
+                                                 [C.c_int32] + [_P] * 5 + [C.c_size_t, _P])
 
 _lib = None
 _lock = threading.Lock()

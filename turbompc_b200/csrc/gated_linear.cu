@@ -2,136 +2,213 @@
 //     h = act(x Wg^T) * (x Wu^T)
 //     dg = dh u act'(g), du = dh act(g)
 //     dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x
-// Tiles of 64 x 64 outputs, float products and sums.
-#include "seq_common.cuh"
+//
+// All products run on the tensor cores (seq_gemm.cuh).  Forward: one kernel, a
+// tile holds the same columns of both projections, so the activation and the
+// product happen in its epilogue and neither projection reaches memory.
+// Backward recomputes both projections in the same kernel with another
+// epilogue, which writes dg | du: that costs 4 d operations per element where
+// keeping the projections would cost 8 bytes written and read, and holds no
+// activations between the passes.  dx and dW are one product each over
+// dg | du; dW splits the tokens over the blocks into float partials that a last
+// kernel adds in order.
+#include <algorithm>
+
+#include "seq_gemm.cuh"
 
 namespace tmpc {
 namespace seq {
 
-// act(g) and act'(g).
-__device__ __forceinline__ void activation(int act, float g, float& a, float& da) {
-  if (act == TMPC_ACT_SILU) {
-    const float s = 1.f / (1.f + expf(-g));
-    a = g * s;
-    da = s * (1.f + g * (1.f - s));
-  } else {
-    const float c = 0.5f * erfcf(-0.70710678118654752f * g);
-    a = g * c;
-    da = c + g * 0.39894228040143268f * expf(-0.5f * g * g);
-  }
-}
+inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
-// C[m][n] (+)= sum_k A[m sam + k sak] B[n sbn + k sbk], tile 64 x 64.
+// src [rows][cols] as NC bfloat16 components [NC][rows][pitch].
 template <typename T>
-struct Tile {
-  float a[16][65], b[16][65];
-};
-
-template <typename T>
-__device__ __forceinline__ void gemm_tile(Tile<T>& s, float (&acc)[4][4], const T* A, int64_t sam, int64_t sak,
-                                          const T* B, int64_t sbn, int64_t sbk, int64_t m0, int64_t M, int n0, int N,
-                                          int64_t K) {
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  for (int64_t k0 = 0; k0 < K; k0 += 16) {
-    __syncthreads();
-    for (int e = threadIdx.x; e < 1024; e += 256) {
-      const int am = sak == 1 ? e / 16 : e % 64, ak = sak == 1 ? e % 16 : e / 64;
-      const int bn = sbk == 1 ? e / 16 : e % 64, bk = sbk == 1 ? e % 16 : e / 64;
-      s.a[ak][am] = (m0 + am < M && k0 + ak < K) ? to_f(A[(m0 + am) * sam + (k0 + ak) * sak]) : 0.f;
-      s.b[bk][bn] = (n0 + bn < N && k0 + bk < K) ? to_f(B[(int64_t)(n0 + bn) * sbn + (k0 + bk) * sbk]) : 0.f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(s.a[k][ty * 4 + i], s.b[k][tx * 4 + j], acc[i][j]);
-  }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) gated_fwd_kernel(const T* x, const T* wg, const T* wu, T* h, T* gate, T* up,
-                                                       int64_t N, int d, int f, int act) {
-  __shared__ Tile<T> s;
-  float g[4][4] = {}, u[4][4] = {};
-  const int64_t m0 = (int64_t)blockIdx.x * 64;
-  const int n0 = blockIdx.y * 64;
-  gemm_tile(s, g, x, d, 1, wg, d, 1, m0, N, n0, f, d);
-  gemm_tile(s, u, x, d, 1, wu, d, 1, m0, N, n0, f, d);
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + (threadIdx.x / 16) * 4 + i;
-      const int n = n0 + (threadIdx.x % 16) * 4 + j;
-      if (m < N && n < f) {
-        float a, da;
-        activation(act, g[i][j], a, da);
-        h[m * f + n] = from_f<T>(a * u[i][j]);
-        if (gate) {
-          gate[m * f + n] = from_f<T>(g[i][j]);
-          up[m * f + n] = from_f<T>(u[i][j]);
-        }
-      }
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) gated_dact_kernel(const T* gate, const T* up, const T* dh, T* dg, T* du,
-                                                        int64_t n, int act) {
+__global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ src, bf16* __restrict__ dst, int64_t rows,
+                                                  int cols, int pitch) {
+  const int64_t n = rows * cols;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    float a, da;
-    activation(act, to_f(gate[i]), a, da);
-    const float y = to_f(dh[i]);
-    dg[i] = from_f<T>(y * to_f(up[i]) * da);
-    du[i] = from_f<T>(y * a);
+    const int64_t r = i / cols;
+    const int64_t o = r * pitch + (i - r * cols);
+    if constexpr (sizeof(T) == 2) {
+      dst[o] = src[i];
+    } else {
+      bf16 c[3];
+      gemm::split3(src[i], c);
+      dst[o] = c[0];
+      dst[o + rows * pitch] = c[1];
+      dst[o + 2 * rows * pitch] = c[2];
+    }
   }
 }
 
-// out = A1 B1 (+ A2 B2)
+// dWg | dWu from the float partials [splits][2 fp][d], in order.
 template <typename T>
-__global__ void __launch_bounds__(256) gemm_kernel(const T* A1, const T* B1, const T* A2, const T* B2, int64_t sam,
-                                                  int64_t sak, int64_t sbn, int64_t sbk, T* out, int64_t M, int N,
-                                                  int64_t K) {
-  __shared__ Tile<T> s;
-  float acc[4][4] = {};
-  const int64_t m0 = (int64_t)blockIdx.x * 64;
-  const int n0 = blockIdx.y * 64;
-  gemm_tile(s, acc, A1, sam, sak, B1, sbn, sbk, m0, M, n0, N, K);
-  if (A2) gemm_tile(s, acc, A2, sam, sak, B2, sbn, sbk, m0, M, n0, N, K);
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + (threadIdx.x / 16) * 4 + i;
-      const int n = n0 + (threadIdx.x % 16) * 4 + j;
-      if (m < M && n < N) out[m * N + n] = from_f<T>(acc[i][j]);
-    }
+__global__ void __launch_bounds__(256) dw_sum_kernel(const float* __restrict__ part, T* __restrict__ dwg,
+                                                    T* __restrict__ dwu, int f, int fp, int d, int splits) {
+  const int64_t n = (int64_t)f * d, slab = (int64_t)2 * fp * d;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < 2 * n; i += (int64_t)gridDim.x * 256) {
+    const bool up = i >= n;
+    const int64_t j = up ? i - n : i;
+    const float* s = part + (up ? (int64_t)fp * d : 0) + j;
+    float a = 0.f;
+    for (int k = 0; k < splits; ++k) a += s[k * slab];
+    (up ? dwu : dwg)[j] = from_f<T>(a);
+  }
 }
 
 inline int check_gated(int64_t rows, int d, int f, int act) {
-  if (rows < 0 || rows > INT32_MAX || d < 1 || f < 1) return TMPC_ERR_BAD_DIMS;
+  if (rows < 0 || rows > INT32_MAX - 256 || d < 1 || f < 1) return TMPC_ERR_BAD_DIMS;
   if ((act != TMPC_ACT_SILU && act != TMPC_ACT_GELU) || d > 65536 || f > 65536) return TMPC_ERR_UNSUPPORTED;
   return TMPC_OK;
 }
 
+// Where the operands of the products live: the caller's tensors when TMA can
+// read them (bfloat16, rows of a multiple of 16 bytes), copies otherwise.
+struct Plan {
+  bool direct;
+  int comps, dp, fp, splits;
+  int64_t x, wg, wu, dgu, part, total;  // byte offsets in the workspace
+};
+
+// Splits of dW's token axis: the fewest that fill the SMs' last wave best, each
+// at least 8 blocks of 64 tokens.
+inline int dw_splits(int64_t rows, int64_t tiles, int sms) {
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(32, (rows + 511) / 512));
+  int best = 1;
+  double eff = 0;
+  for (int s = 1; s <= most; ++s) {
+    const int64_t units = tiles * s, waves = (units + sms - 1) / sms;
+    const double e = (double)units / (double)(waves * sms);
+    if (e > eff + 0.02) best = s, eff = e;
+  }
+  return best;
+}
+
+inline int tile_n(int n) { return n > 128 ? 256 : n > 64 ? 128 : 64; }
+
+inline Plan make_plan(int64_t rows, int d, int f, int esize, bool backward) {
+  Plan p{};
+  p.comps = esize == 4 ? 3 : 1;
+  p.direct = esize == 2 && d % 8 == 0;
+  p.dp = (int)round_up(d, 8);
+  p.fp = (int)round_up(f, 64);
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at = round_up(at + bytes, 256);
+    return o;
+  };
+  if (!p.direct) {
+    p.x = take(p.comps * rows * p.dp * 2);
+    p.wg = take((int64_t)p.comps * f * p.dp * 2);
+    p.wu = take((int64_t)p.comps * f * p.dp * 2);
+  }
+  if (backward) {
+    const int nt = tile_n(d);
+    const int64_t tiles = (2 * (int64_t)p.fp + gemm::BM - 1) / gemm::BM * ((d + nt - 1) / nt);
+    p.splits = dw_splits(rows, tiles, sm_count());
+    p.dgu = take(p.comps * rows * 2 * p.fp * 2);
+    p.part = take((int64_t)p.splits * 2 * p.fp * d * 4);
+  }
+  p.total = at;
+  return p;
+}
+
 template <typename T>
-int gated_fwd(int64_t rows, int d, int f, const T* x, const T* wg, const T* wu, int act, T* h, T* gate, T* up,
-              cudaStream_t st) {
+int vec_bytes(int cols, const void* a) {
+  for (int v : {16, 4})
+    if ((int64_t)cols * (int64_t)sizeof(T) % v == 0 && aligned(a, v)) return v;
+  return sizeof(T);
+}
+
+struct Operands {
+  const void *x, *wg, *wu;
+};
+
+template <typename T>
+Operands pack_operands(const Plan& p, int64_t rows, int d, int f, const T* x, const T* wg, const T* wu, char* ws,
+                       cudaStream_t st) {
+  if (p.direct) return {x, wg, wu};
+  auto pack = [&](const T* src, int64_t off, int64_t n) {
+    const int64_t blocks = std::min<int64_t>((n * d + 255) / 256, 8 * (int64_t)sm_count());
+    pack_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(src, reinterpret_cast<bf16*>(ws + off), n, d, p.dp);
+    return (const void*)(ws + off);
+  };
+  return {pack(x, p.x, rows), pack(wg, p.wg, f), pack(wu, p.wu, f)};
+}
+
+// The two-projection kernel: forward, or dg | du.
+template <typename T, int MODE>
+int dual(const Plan& p, const Operands& o, int64_t rows, int d, int f, int act, void* out, const T* dh, bf16* dgu,
+         cudaStream_t st) {
+  gemm::Params q{};
+  q.M = rows;
+  q.N = f;
+  q.fp = p.fp;
+  q.kblocks = (d + gemm::BK - 1) / gemm::BK;
+  q.nterms = p.comps == 3 ? 6 : 1;
+  q.splits = 1;
+  q.mtiles = (int)((rows + gemm::BM - 1) / gemm::BM);
+  q.act = act;
+  q.out = out;
+  q.dh = dh;
+  q.dgu = dgu;
+  q.vec = vec_bytes<T>(f, MODE == gemm::kDact ? (const void*)dh : out);
+  const int cols = MODE == gemm::kDact ? p.fp : f;  // dg | du is written to its padded width
+  gemm::Maps maps;
+  auto run = [&](auto NT) {
+    constexpr int nt = decltype(NT)::value;
+    int rc = gemm::make_map(&maps.a, o.x, d, rows, p.comps, p.dp, gemm::BM);
+    if (!rc) rc = gemm::make_map(&maps.b0, o.wg, d, f, p.comps, p.dp, nt / 2);
+    if (!rc) rc = gemm::make_map(&maps.b1, o.wu, d, f, p.comps, p.dp, nt / 2);
+    if (rc) return rc;
+    q.ntiles = (cols + nt / 2 - 1) / (nt / 2);
+    return gemm::launch<T, MODE, nt>(maps, q, st);
+  };
+  // Few tokens: narrow tiles, so that the columns spread over more SMs.
+  if ((int64_t)q.mtiles * ((cols + 127) / 128) >= sm_count()) return run(std::integral_constant<int, 256>{});
+  return run(std::integral_constant<int, 64>{});
+}
+
+template <typename T>
+int gated_fwd(int64_t rows, int d, int f, const T* x, const T* wg, const T* wu, int act, T* h, void* ws,
+              size_t ws_bytes, cudaStream_t st) {
   const int rc = check_gated(rows, d, f, act);
   if (rc) return rc;
   if (rows == 0) return TMPC_OK;
-  if (!x || !wg || !wu || !h || (gate == nullptr) != (up == nullptr)) return TMPC_ERR_NULL_ARG;
-  gated_fwd_kernel<T><<<dim3((unsigned)((rows + 63) / 64), (f + 63) / 64), 256, 0, st>>>(x, wg, wu, h, gate, up, rows, d,
-                                                                                      f, act);
-  return (int)cudaPeekAtLastError();
+  if (!x || !wg || !wu || !h) return TMPC_ERR_NULL_ARG;
+  if (!aligned(x, 16) || !aligned(wg, 16) || !aligned(wu, 16)) return TMPC_ERR_UNSUPPORTED;
+  const Plan p = make_plan(rows, d, f, sizeof(T), false);
+  if (p.total > 0 && (!ws || (int64_t)ws_bytes < p.total || !aligned(ws, 16))) return TMPC_ERR_WORKSPACE;
+  const Operands o = pack_operands<T>(p, rows, d, f, x, wg, wu, static_cast<char*>(ws), st);
+  return dual<T, gemm::kAct>(p, o, rows, d, f, act, h, nullptr, nullptr, st);
 }
 
-inline size_t gated_bwd_ws(int64_t rows, int f, int esize) {
-  return rows > 0 && f > 0 ? (size_t)2 * rows * f * esize + 16 : 0;
+template <typename T, int MODE>
+int single(const gemm::Params& q0, int d, const void* a, int64_t a_inner, int64_t a_outer, int64_t a_pitch, int a_box,
+           const void* b0, const void* b1, int64_t b_outer, int64_t b_pitch, int comps, cudaStream_t st) {
+  auto run = [&](auto NT) {
+    constexpr int nt = decltype(NT)::value;
+    gemm::Params q = q0;
+    gemm::Maps maps;
+    int rc = gemm::make_map(&maps.a, a, a_inner, a_outer, comps, a_pitch, a_box);
+    if (!rc) rc = gemm::make_map(&maps.b0, b0, d, b_outer, comps, b_pitch, 64);
+    if (!rc) rc = gemm::make_map(&maps.b1, b1, d, b_outer, comps, b_pitch, 64);
+    if (rc) return rc;
+    q.mtiles = (int)((q.M + gemm::BM - 1) / gemm::BM);
+    q.ntiles = (d + nt - 1) / nt;
+    return gemm::launch<T, MODE, nt>(maps, q, st);
+  };
+  const int nt = tile_n(d);
+  if (nt == 256) return run(std::integral_constant<int, 256>{});
+  if (nt == 128) return run(std::integral_constant<int, 128>{});
+  return run(std::integral_constant<int, 64>{});
 }
 
 template <typename T>
-int gated_bwd(int64_t rows, int d, int f, const T* x, const T* wg, const T* wu, int act, const T* gate, const T* up,
-              const T* dh, T* dx, T* dwg, T* dwu, void* ws, size_t ws_bytes, cudaStream_t st) {
-  const int rc = check_gated(rows, d, f, act);
+int gated_bwd(int64_t rows, int d, int f, const T* x, const T* wg, const T* wu, int act, const T* dh, T* dx, T* dwg,
+              T* dwu, void* ws, size_t ws_bytes, cudaStream_t st) {
+  int rc = check_gated(rows, d, f, act);
   if (rc) return rc;
   if ((dwg == nullptr) != (dwu == nullptr)) return TMPC_ERR_NULL_ARG;
   if (rows == 0) {
@@ -139,20 +216,46 @@ int gated_bwd(int64_t rows, int d, int f, const T* x, const T* wg, const T* wu, 
     const cudaError_t e = cudaMemsetAsync(dwg, 0, (size_t)f * d * sizeof(T), st);
     return e != cudaSuccess ? (int)e : (int)cudaMemsetAsync(dwu, 0, (size_t)f * d * sizeof(T), st);
   }
-  if (!x || !wg || !wu || !gate || !up || !dh) return TMPC_ERR_NULL_ARG;
-  if (!ws || ws_bytes < gated_bwd_ws(rows, f, sizeof(T)) || !aligned(ws, 16)) return TMPC_ERR_WORKSPACE;
-  T* dg = static_cast<T*>(ws);
-  T* du = dg + rows * f;
-  gated_dact_kernel<T><<<8 * sm_count(), 256, 0, st>>>(gate, up, dh, dg, du, rows * f, act);
-  if (dx)
-    gemm_kernel<T><<<dim3((unsigned)((rows + 63) / 64), (d + 63) / 64), 256, 0, st>>>(dg, wg, du, wu, f, 1, 1, d, dx,
-                                                                                   rows, d, f);
+  if (!x || !wg || !wu || !dh) return TMPC_ERR_NULL_ARG;
+  if (!aligned(x, 16) || !aligned(wg, 16) || !aligned(wu, 16)) return TMPC_ERR_UNSUPPORTED;
+  const Plan p = make_plan(rows, d, f, sizeof(T), true);
+  if (!ws || (int64_t)ws_bytes < p.total || !aligned(ws, 16)) return TMPC_ERR_WORKSPACE;
+  char* w = static_cast<char*>(ws);
+  bf16* dgu = reinterpret_cast<bf16*>(w + p.dgu);
+  float* part = reinterpret_cast<float*>(w + p.part);
+  const Operands o = pack_operands<T>(p, rows, d, f, x, wg, wu, w, st);
+  rc = dual<T, gemm::kDact>(p, o, rows, d, f, act, nullptr, dh, dgu, st);
+  if (rc) return rc;
+  gemm::Params q{};
+  q.N = d;
+  q.fp = p.fp;
+  q.nterms = p.comps == 3 ? 6 : 1;
+  if (dx) {
+    q.M = rows;
+    q.kblocks = 2 * p.fp / gemm::BK;
+    q.splits = 1;
+    q.out = dx;
+    q.vec = vec_bytes<T>(d, dx);
+    rc = single<T, gemm::kDx>(q, d, dgu, 2 * p.fp, rows, 2 * p.fp, gemm::BM, o.wg, o.wu, f, p.dp, p.comps, st);
+    if (rc) return rc;
+  }
   if (dwg) {
-    const dim3 grid((f + 63) / 64, (d + 63) / 64);
-    gemm_kernel<T><<<grid, 256, 0, st>>>(dg, x, nullptr, nullptr, 1, f, 1, d, dwg, f, d, rows);
-    gemm_kernel<T><<<grid, 256, 0, st>>>(du, x, nullptr, nullptr, 1, f, 1, d, dwu, f, d, rows);
+    q.M = 2 * p.fp;
+    q.kblocks = (int)((rows + gemm::BK - 1) / gemm::BK);
+    q.splits = p.splits;
+    q.out = part;
+    q.vec = vec_bytes<float>(d, part);
+    rc = single<T, gemm::kDw>(q, d, dgu, 2 * p.fp, rows, 2 * p.fp, 64, o.x, o.x, rows, p.dp, p.comps, st);
+    if (rc) return rc;
+    const int64_t blocks = std::min<int64_t>(((int64_t)2 * f * d + 255) / 256, 16 * (int64_t)sm_count());
+    dw_sum_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(part, dwg, dwu, f, p.fp, d, p.splits);
   }
   return (int)cudaPeekAtLastError();
+}
+
+inline size_t gated_ws(int64_t rows, int d, int f, int esize, bool backward) {
+  if (rows <= 0 || check_gated(rows, d, f, TMPC_ACT_SILU) || (esize != 2 && esize != 4)) return 0;
+  return (size_t)make_plan(rows, d, f, esize, backward).total;
 }
 
 }  // namespace seq
@@ -162,31 +265,27 @@ extern "C" {
 
 #define TMPC_GATED_ENTRY(SUF, T)                                                                                     \
   int32_t tmpc_gated_linear_##SUF(int64_t rows, int32_t d, int32_t f, const void* x, const void* w_gate,             \
-                                  const void* w_up, int32_t act, void* h, void* gate, void* up, void* workspace,     \
-                                  size_t workspace_bytes, tmpc_stream_t stream) {                                    \
-    (void)workspace;                                                                                                 \
-    (void)workspace_bytes;                                                                                           \
-    return tmpc::seq::gated_fwd<T>(rows, d, f, (const T*)x, (const T*)w_gate, (const T*)w_up, act, (T*)h, (T*)gate,  \
-                                   (T*)up, (cudaStream_t)stream);                                                    \
+                                  const void* w_up, int32_t act, void* h, void* workspace, size_t workspace_bytes,   \
+                                  tmpc_stream_t stream) {                                                            \
+    return tmpc::seq::gated_fwd<T>(rows, d, f, (const T*)x, (const T*)w_gate, (const T*)w_up, act, (T*)h, workspace, \
+                                   workspace_bytes, (cudaStream_t)stream);                                           \
   }                                                                                                                  \
   int32_t tmpc_gated_linear_backward_##SUF(int64_t rows, int32_t d, int32_t f, const void* x, const void* w_gate,    \
-                                           const void* w_up, int32_t act, const void* gate, const void* up,          \
-                                           const void* dh, void* dx, void* dw_gate, void* dw_up, void* workspace,    \
-                                           size_t workspace_bytes, tmpc_stream_t stream) {                           \
-    return tmpc::seq::gated_bwd<T>(rows, d, f, (const T*)x, (const T*)w_gate, (const T*)w_up, act, (const T*)gate,   \
-                                   (const T*)up, (const T*)dh, (T*)dx, (T*)dw_gate, (T*)dw_up, workspace,            \
-                                   workspace_bytes, (cudaStream_t)stream);                                           \
+                                           const void* w_up, int32_t act, const void* dh, void* dx, void* dw_gate,   \
+                                           void* dw_up, void* workspace, size_t workspace_bytes,                     \
+                                           tmpc_stream_t stream) {                                                   \
+    return tmpc::seq::gated_bwd<T>(rows, d, f, (const T*)x, (const T*)w_gate, (const T*)w_up, act, (const T*)dh,     \
+                                   (T*)dx, (T*)dw_gate, (T*)dw_up, workspace, workspace_bytes,                       \
+                                   (cudaStream_t)stream);                                                            \
   }
 TMPC_GATED_ENTRY(f32, float)
 TMPC_GATED_ENTRY(bf16, __nv_bfloat16)
 
 size_t tmpc_gated_linear_workspace_bytes(int64_t rows, int32_t d, int32_t f, int32_t elem_size) {
-  (void)rows, (void)d, (void)f, (void)elem_size;
-  return 0;
+  return tmpc::seq::gated_ws(rows, d, f, elem_size, false);
 }
 size_t tmpc_gated_linear_backward_workspace_bytes(int64_t rows, int32_t d, int32_t f, int32_t elem_size) {
-  (void)d;
-  return tmpc::seq::gated_bwd_ws(rows, f, elem_size);
+  return tmpc::seq::gated_ws(rows, d, f, elem_size, true);
 }
 
 }  // extern "C"

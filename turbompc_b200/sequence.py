@@ -274,29 +274,33 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
 # ---------------------------------------------------------------------------
 # Gated linear layer
 # ---------------------------------------------------------------------------
-def _gated_forward(x2, w_gate, w_up, act, keep):
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous, and at an address the tensor-core kernels' copies can read."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _gated_forward(x2, w_gate, w_up, act):
     rows, d, f = x2.shape[0], x2.shape[1], w_gate.shape[0]
     h = torch.empty(rows, f, dtype=x2.dtype, device=x2.device)
-    gate, up = (torch.empty_like(h), torch.empty_like(h)) if keep else (None, None)
     need = int(_ffi.load().tmpc_gated_linear_workspace_bytes(rows, d, f, x2.element_size()))
     ws = _workspace(need, x2.device)
     _call(f"tmpc_gated_linear_{_suffix(x2.dtype)}", x2.device, rows, d, f, _p(x2), _p(w_gate), _p(w_up), act, _p(h),
-          _p(gate), _p(up), _p(ws), need)
-    return h, gate, up
+          _p(ws), need)
+    return h
 
 
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x2, w_gate, w_up, act):
-        h, gate, up = _gated_forward(x2, w_gate, w_up, act, True)
-        ctx.save_for_backward(x2, w_gate, w_up, gate, up)
+        ctx.save_for_backward(x2, w_gate, w_up)
         ctx.act = act
-        return h
+        return _gated_forward(x2, w_gate, w_up, act)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
-        x2, w_gate, w_up, gate, up = ctx.saved_tensors
+        x2, w_gate, w_up = ctx.saved_tensors
         rows, d, f = x2.shape[0], x2.shape[1], w_gate.shape[0]
         dh = dh.contiguous()
         dx = torch.empty(x2.shape, dtype=x2.dtype, device=x2.device) if ctx.needs_input_grad[0] else None
@@ -305,7 +309,7 @@ class _GatedLinear(torch.autograd.Function):
         need = int(_ffi.load().tmpc_gated_linear_backward_workspace_bytes(rows, d, f, x2.element_size()))
         ws = _workspace(need, x2.device)
         _call(f"tmpc_gated_linear_backward_{_suffix(x2.dtype)}", x2.device, rows, d, f, _p(x2), _p(w_gate), _p(w_up),
-              ctx.act, _p(gate), _p(up), _p(dh), _p(dx), _p(dwg), _p(dwu), _p(ws), need)
+              ctx.act, _p(dh), _p(dx), _p(dwg), _p(dwu), _p(ws), need)
         return dx, dwg, dwu, None
 
 
@@ -313,7 +317,8 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, acti
     """h = act(x w_gate^T) * (x w_up^T): both projections, the activation and
     the product of a gated feed-forward block.  x (..., d), w_gate and w_up
     (f, d); ``activation`` "silu" or "gelu" (the exact, erf form).  Returns h (..., f).
-    Differentiable with respect to x, w_gate and w_up."""
+    Differentiable with respect to x, w_gate and w_up; the projections are
+    recomputed in the backward pass, not kept."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
     if not isinstance(x, torch.Tensor):
@@ -329,10 +334,10 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, acti
         raise ValueError(f"shapes of x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)} and w_up {tuple(w_up.shape)} "
                          "do not fit")
     act = ACTIVATIONS[activation]
-    x2 = x.reshape(-1, x.shape[-1]).contiguous()
-    w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
+    x2 = _aligned(x.reshape(-1, x.shape[-1]))
+    w_gate, w_up = _aligned(w_gate), _aligned(w_up)
     if _grad_needed(x2, w_gate, w_up):
         h = _GatedLinear.apply(x2, w_gate, w_up, act)
     else:
-        h = _gated_forward(x2, w_gate, w_up, act, False)[0]
+        h = _gated_forward(x2, w_gate, w_up, act)
     return h.reshape(*x.shape[:-1], w_gate.shape[0])

@@ -9,41 +9,14 @@
 // a row (dq, dk).  dlog d needs no product of S and dS inside the sequence:
 // with q' = d^(t+1) q and k' = d^-(t+1) k the decay leaves every o_t, and
 //   dlog d = sum_t (t+1) (q_t . dq_t - k_t . dk_t) + L <S_L, dS_L>.
-#include "seq_common.cuh"
+#include "seq_attention.cuh"
 
 namespace tmpc {
 namespace seq {
+namespace rec {
 
 constexpr int kTile = 16;  // tokens staged in shared memory at a time
 constexpr int kCols = 128;
-
-struct LinAttnArgs {
-  TmpcSeqView q, k, v, o, gq, gk, gv;  // o: the output, or its gradient; gq, gk, gv: gradients of q, k, v
-  const float* log_decay;
-  const int32_t* lengths;
-  const float* state_in;
-  float* state_out;
-  const float* dstate_out;
-  float* dstate_in;
-  float* acc;     // [B][T][G][dk + dv]: dk, dv summed over a key head's query heads
-  double* dlog;   // [2][B][H]
-  int T, H, G, dk, dv;
-  float scale;
-};
-
-template <typename T>
-__device__ __forceinline__ const T* row_ptr(const TmpcSeqView& w, int64_t b, int64_t t, int64_t h) {
-  return static_cast<const T*>(w.ptr) + b * w.batch + t * w.token + h * w.head;
-}
-
-// log2 of the decay; the clamp keeps 0 * log(0) finite (2^-1e4 is 0 in float).
-__device__ __forceinline__ float log2_decay(const float* log_decay, int h) {
-  return fmaxf(log_decay[h] * 1.4426950408889634f, -1e4f);
-}
-
-__device__ __forceinline__ int seq_len(const LinAttnArgs& a, int b) {
-  return a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
-}
 
 // Tokens t0 .. t0 + n - 1 of one head into a [kTile][LD] tile, zero-padded.
 template <typename T, int LD>
@@ -78,11 +51,11 @@ __global__ void __launch_bounds__(kCols) fwd_kernel(const LinAttnArgs a) {
         S[i] = fmaf(dec, S[i], sk[t][i] * v);
         o = fmaf(sq[t][i], S[i], o);
       }
-      if (j < a.dv) const_cast<T*>(row_ptr<T>(a.o, b, t0 + t, h))[j] = from_f<T>(o * a.scale);
+      if (j < a.dv) (row_ptr<T>(a.o, b, t0 + t, h))[j] = from_f<T>(o * a.scale);
     }
   }
   if (j < a.dv)
-    for (int t = len; t < a.T; ++t) const_cast<T*>(row_ptr<T>(a.o, b, t, h))[j] = from_f<T>(0.f);
+    for (int t = len; t < a.T; ++t) (row_ptr<T>(a.o, b, t, h))[j] = from_f<T>(0.f);
   if (a.state_out && j < a.dv) {
 #pragma unroll
     for (int i = 0; i < D; ++i)
@@ -131,11 +104,11 @@ __global__ void __launch_bounds__(kCols) dq_kernel(const LinAttnArgs a) {
       }
       dq *= a.scale;
       dl += (double)(t0 + t + 1) * (double)(q * dq);
-      if (i < a.dk) const_cast<T*>(row_ptr<T>(a.gq, b, t0 + t, h))[i] = from_f<T>(dq);
+      if (i < a.dk) (row_ptr<T>(a.gq, b, t0 + t, h))[i] = from_f<T>(dq);
     }
   }
   if (i < a.dk)
-    for (int t = len; t < a.T; ++t) const_cast<T*>(row_ptr<T>(a.gq, b, t, h))[i] = from_f<T>(0.f);
+    for (int t = len; t < a.T; ++t) (row_ptr<T>(a.gq, b, t, h))[i] = from_f<T>(0.f);
   if (a.dstate_out && i < a.dk) {
     float e = 0.f;
 #pragma unroll
@@ -144,7 +117,7 @@ __global__ void __launch_bounds__(kCols) dq_kernel(const LinAttnArgs a) {
     dl += (double)len * (double)e;
   }
   dl = block_sum(dl, red);
-  if (a.dlog && i == 0) a.dlog[(size_t)b * a.H + h] = dl;
+  if (a.dlog && i == 0) reinterpret_cast<double*>(a.dlog)[(size_t)b * a.H + h] = dl;
 }
 
 // dk, dv: threads 0 .. 127 own a row of dS, threads 128 .. 255 a column.
@@ -191,7 +164,7 @@ __global__ void __launch_bounds__(2 * kCols) dkv_kernel(const LinAttnArgs a) {
           float* acc = a.acc + (((size_t)b * a.T + t0 + t) * a.G + g) * (a.dk + a.dv) + (is_row ? 0 : a.dk) + i;
           if (r > 0) y += *acc;
           if (r + 1 < rep) *acc = y;
-          else const_cast<T*>(row_ptr<T>(is_row ? a.gk : a.gv, b, t0 + t, g))[i] = from_f<T>(y);
+          else (row_ptr<T>(is_row ? a.gk : a.gv, b, t0 + t, g))[i] = from_f<T>(y);
         }
       }
     }
@@ -201,11 +174,11 @@ __global__ void __launch_bounds__(2 * kCols) dkv_kernel(const LinAttnArgs a) {
         if (j < a.dv) a.dstate_in[so + (size_t)i * a.dv + j] = dS[j];
     }
     dl = block_sum(dl, red);
-    if (a.dlog && threadIdx.x == 0) a.dlog[((size_t)gridDim.x + b) * a.H + h] = dl;
+    if (a.dlog && threadIdx.x == 0) reinterpret_cast<double*>(a.dlog)[((size_t)gridDim.x + b) * a.H + h] = dl;
   }
   if (i < mine)
     for (int t = len; t < a.T; ++t)
-      const_cast<T*>(row_ptr<T>(is_row ? a.gk : a.gv, b, t, g))[i] = from_f<T>(0.f);
+      (row_ptr<T>(is_row ? a.gk : a.gv, b, t, g))[i] = from_f<T>(0.f);
 }
 
 __global__ void dlog_kernel(const double* part, float* out, int n, int H) {
@@ -217,42 +190,72 @@ __global__ void dlog_kernel(const double* part, float* out, int n, int H) {
   if (threadIdx.x == 0) out[h] = (float)s;
 }
 
-inline int check_dims(const TmpcLinAttnDims* d) {
-  if (!d) return TMPC_ERR_NULL_ARG;
-  if (d->B < 0 || d->T < 0 || d->H < 1 || d->G < 1 || d->H % d->G || d->dk < 1 || d->dv < 1) return TMPC_ERR_BAD_DIMS;
-  if (d->dk > 128 || d->dv > 128 || d->H > 65535) return TMPC_ERR_UNSUPPORTED;
-  return TMPC_OK;
+}  // namespace rec
+
+template <>
+size_t LinAttn<float>::forward_ws(const TmpcLinAttnDims*) {
+  return 0;
 }
 
-template <typename F>
-int by_size(const TmpcLinAttnDims* d, F&& f) {
-  const int m = d->dk > d->dv ? d->dk : d->dv;
-  if (m <= 32) f(std::integral_constant<int, 32>{});
-  else if (m <= 64) f(std::integral_constant<int, 64>{});
-  else f(std::integral_constant<int, 128>{});
+template <>
+int LinAttn<float>::forward(LinAttnArgs a, const TmpcLinAttnDims* d, char*, cudaStream_t st) {
+  by_size(d, [&](auto dd) {
+    constexpr int D = decltype(dd)::value;
+    rec::fwd_kernel<float, D><<<dim3(a.B, a.H), rec::kCols, 0, st>>>(a);
+  });
   return (int)cudaPeekAtLastError();
+}
+
+template <>
+size_t LinAttn<float>::backward_ws(const TmpcLinAttnDims* d) {
+  return (size_t)2 * d->B * d->H * sizeof(double) +
+         (d->H > d->G ? (size_t)d->B * d->T * d->G * (d->dk + d->dv) * sizeof(float) : 0);
+}
+
+template <>
+int LinAttn<float>::backward(LinAttnArgs a, const TmpcLinAttnDims* d, float* dlog_decay, char* ws, cudaStream_t st) {
+  a.dlog = reinterpret_cast<float*>(ws);
+  a.acc = reinterpret_cast<float*>(ws + (size_t)2 * d->B * d->H * sizeof(double));
+  by_size(d, [&](auto dd) {
+    constexpr int D = decltype(dd)::value;
+    rec::dq_kernel<float, D><<<dim3(a.B, a.H), rec::kCols, 0, st>>>(a);
+    rec::dkv_kernel<float, D><<<dim3(a.B, a.G), 2 * rec::kCols, 0, st>>>(a);
+  });
+  if (dlog_decay)
+    rec::dlog_kernel<<<a.H, 128, 0, st>>>(reinterpret_cast<double*>(a.dlog), dlog_decay, 2 * a.B, a.H);
+  return (int)cudaPeekAtLastError();
+}
+
+// ---------------------------------------------------------------------------
+// Entry points
+// ---------------------------------------------------------------------------
+inline bool null_view(const TmpcSeqView* v, const TmpcLinAttnDims* d) { return !v || (d->T > 0 && !v->ptr); }
+
+inline LinAttnArgs make_args(const TmpcLinAttnDims* d, const TmpcSeqView* q, const TmpcSeqView* k, const TmpcSeqView* v,
+                             const TmpcSeqView* o, const float* log_decay, const int32_t* lengths,
+                             const float* state_in, double scale) {
+  LinAttnArgs a{};
+  a.q = *q, a.k = *k, a.v = *v, a.o = *o;
+  a.log_decay = log_decay, a.lengths = lengths, a.state_in = state_in;
+  a.B = d->B, a.T = d->T, a.H = d->H, a.G = d->G, a.dk = d->dk, a.dv = d->dv;
+  a.nseg = 1;
+  a.scale = (float)scale;
+  return a;
 }
 
 template <typename T>
 int forward(const TmpcLinAttnDims* d, const TmpcSeqView* q, const TmpcSeqView* k, const TmpcSeqView* v,
             const TmpcSeqView* o, const float* log_decay, const int32_t* lengths, const float* state_in,
-            float* state_out, double scale, cudaStream_t st) {
+            float* state_out, double scale, void* ws, size_t ws_bytes, cudaStream_t st) {
   const int rc = check_dims(d);
   if (rc) return rc;
   if (d->B == 0) return TMPC_OK;
-  if (!q || !k || !v || !o || !log_decay) return TMPC_ERR_NULL_ARG;
-  if (d->T > 0 && (!q->ptr || !k->ptr || !v->ptr || !o->ptr)) return TMPC_ERR_NULL_ARG;
-  LinAttnArgs a{};
-  a.q = *q; a.k = *k; a.v = *v; a.o = *o;
-  a.log_decay = log_decay; a.lengths = lengths; a.state_in = state_in; a.state_out = state_out;
-  a.T = d->T; a.H = d->H; a.G = d->G; a.dk = d->dk; a.dv = d->dv; a.scale = (float)scale;
-  return by_size(d, [&](auto D) { fwd_kernel<T, D><<<dim3(d->B, d->H), kCols, 0, st>>>(a); });
-}
-
-inline size_t backward_ws(const TmpcLinAttnDims* d) {
-  if (check_dims(d)) return 0;
-  const size_t dlog = (size_t)2 * d->B * d->H * sizeof(double);
-  return dlog + (d->H > d->G ? (size_t)d->B * d->T * d->G * (d->dk + d->dv) * sizeof(float) : 0);
+  if (null_view(q, d) || null_view(k, d) || null_view(v, d) || null_view(o, d) || !log_decay) return TMPC_ERR_NULL_ARG;
+  const size_t need = LinAttn<T>::forward_ws(d);
+  if (need > 0 && (!ws || ws_bytes < need || !aligned(ws, 16))) return TMPC_ERR_WORKSPACE;
+  LinAttnArgs a = make_args(d, q, k, v, o, log_decay, lengths, state_in, scale);
+  a.state_out = state_out;
+  return LinAttn<T>::forward(a, d, static_cast<char*>(ws), st);
 }
 
 template <typename T>
@@ -263,23 +266,15 @@ int backward(const TmpcLinAttnDims* d, const TmpcSeqView* q, const TmpcSeqView* 
   const int rc = check_dims(d);
   if (rc) return rc;
   if (d->B == 0) return dlog_decay ? (int)cudaMemsetAsync(dlog_decay, 0, d->H * sizeof(float), st) : TMPC_OK;
-  if (!q || !k || !v || !dout || !dq || !dk || !dv || !log_decay) return TMPC_ERR_NULL_ARG;
-  if (d->T > 0 && (!q->ptr || !k->ptr || !v->ptr || !dout->ptr || !dq->ptr || !dk->ptr || !dv->ptr))
+  if (null_view(q, d) || null_view(k, d) || null_view(v, d) || null_view(dout, d) || null_view(dq, d) ||
+      null_view(dk, d) || null_view(dv, d) || !log_decay)
     return TMPC_ERR_NULL_ARG;
-  if (!ws || ws_bytes < backward_ws(d) || !aligned(ws, 16)) return TMPC_ERR_WORKSPACE;
-  LinAttnArgs a{};
-  a.q = *q; a.k = *k; a.v = *v; a.o = *dout; a.gq = *dq; a.gk = *dk; a.gv = *dv;
-  a.log_decay = log_decay; a.lengths = lengths; a.state_in = state_in;
-  a.dstate_out = dstate_out; a.dstate_in = dstate_in;
-  a.dlog = static_cast<double*>(ws);
-  a.acc = reinterpret_cast<float*>(a.dlog + (size_t)2 * d->B * d->H);
-  a.T = d->T; a.H = d->H; a.G = d->G; a.dk = d->dk; a.dv = d->dv; a.scale = (float)scale;
-  by_size(d, [&](auto D) {
-    dq_kernel<T, D><<<dim3(d->B, d->H), kCols, 0, st>>>(a);
-    dkv_kernel<T, D><<<dim3(d->B, d->G), 2 * kCols, 0, st>>>(a);
-  });
-  if (dlog_decay) dlog_kernel<<<d->H, 128, 0, st>>>(a.dlog, dlog_decay, 2 * d->B, d->H);
-  return (int)cudaPeekAtLastError();
+  const size_t need = LinAttn<T>::backward_ws(d);
+  if (need > 0 && (!ws || ws_bytes < need || !aligned(ws, 16))) return TMPC_ERR_WORKSPACE;
+  LinAttnArgs a = make_args(d, q, k, v, dout, log_decay, lengths, state_in, scale);
+  a.gq = *dq, a.gk = *dk, a.gv = *dv;
+  a.dstate_out = dstate_out, a.dstate_in = dstate_in;
+  return LinAttn<T>::backward(a, d, dlog_decay, static_cast<char*>(ws), st);
 }
 
 }  // namespace seq
@@ -292,10 +287,8 @@ extern "C" {
                                       const TmpcSeqView* v, const TmpcSeqView* o, const float* log_decay,            \
                                       const int32_t* lengths, const float* state_in, float* state_out, double scale, \
                                       void* workspace, size_t workspace_bytes, tmpc_stream_t stream) {               \
-    (void)workspace;                                                                                                 \
-    (void)workspace_bytes;                                                                                           \
-    return tmpc::seq::forward<T>(dims, q, k, v, o, log_decay, lengths, state_in, state_out, scale,                   \
-                                 (cudaStream_t)stream);                                                              \
+    return tmpc::seq::forward<T>(dims, q, k, v, o, log_decay, lengths, state_in, state_out, scale, workspace,        \
+                                 workspace_bytes, (cudaStream_t)stream);                                             \
   }                                                                                                                  \
   int32_t tmpc_linear_attention_backward_##SUF(                                                                      \
       const TmpcLinAttnDims* dims, const TmpcSeqView* q, const TmpcSeqView* k, const TmpcSeqView* v,                 \
@@ -309,12 +302,16 @@ extern "C" {
 TMPC_LINATTN_ENTRY(f32, float)
 TMPC_LINATTN_ENTRY(bf16, __nv_bfloat16)
 
+// The larger of the two types' needs.
 size_t tmpc_linear_attention_workspace_bytes(const TmpcLinAttnDims* dims) {
-  (void)dims;
-  return 0;
+  using namespace tmpc::seq;
+  if (check_dims(dims)) return 0;
+  return std::max(LinAttn<float>::forward_ws(dims), LinAttn<bf16>::forward_ws(dims));
 }
 size_t tmpc_linear_attention_backward_workspace_bytes(const TmpcLinAttnDims* dims) {
-  return tmpc::seq::backward_ws(dims);
+  using namespace tmpc::seq;
+  if (check_dims(dims)) return 0;
+  return std::max(LinAttn<float>::backward_ws(dims), LinAttn<bf16>::backward_ws(dims));
 }
 
 }  // extern "C"

@@ -1,0 +1,846 @@
+// Linear attention with a decay per head, bfloat16, in chunks of 64 tokens.
+//
+// With S the state before a chunk and d the decay (tokens t, s counted from the
+// chunk's start, n of them valid):
+//     o_t  = scale ( sum_{s <= t} d^(t-s) (q_t . k_s) v_s  +  d^(t+1) S^T q_t )
+//     S'   = d^n S + sum_s d^(n-1-s) k_s v_s^T
+// dq is the same sum with (q, k, v) -> (do, v, k) and S^T, so one kernel serves
+// both.  dk and dv run backward in time with R, the adjoint of the state after
+// the chunk:
+//     dv_s = scale sum_{t >= s} d^(t-s) (k_s . q_t) do_t + d^(n-1-s) R^T k_s
+//     dk_s = scale sum_{t >= s} d^(t-s) (v_s . do_t) q_t + d^(n-1-s) R v_s
+//     R'   = d^n R + scale sum_t d^(t+1) q_t do_t^T
+//
+// A block holds one (sequence, head) and walks its chunks; the products run on
+// the warps' matrix instructions with their operands in registers, where the
+// masked scores turn into the next product's operand without leaving the
+// thread.  The state stays in float registers; for a product it is split into
+// two bfloat16 terms (together 2^-17), as is the decayed factor of the state's
+// update, because states and dlog d are float results.  Scores are rounded to
+// one bfloat16 (2^-9): their sums leave as bfloat16.
+//
+// dlog d is the sum over pairs of (t - s) times the pair's share.  Within a
+// chunk it is formed from the two float score matrices.  Across chunks the lag
+// is (t + 1) + (n - 1 - s) + the chunks between: the first two weigh the inter-
+// chunk parts of q . dq and k . dk, the last needs, per chunk, the share X of
+// the pairs that span it.  With E the share crossing the chunk's start,
+// X = E - sum q . dq and E' = X + sum k . dk (inter-chunk parts); X is exactly
+// dropped where d^n < 2^-20.
+#include "seq_attention.cuh"
+
+namespace tmpc {
+namespace seq {
+namespace la {
+
+constexpr int C = kChunk;
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void ldsm(uint32_t (&r)[4], const bf16* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_addr(p)));
+}
+__device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], const bf16* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_addr(p)));
+}
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+// (x, y) as hi + lo, two bfloat16 each.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = pack2(x, y);
+  const float2 h = unpack2(hi);
+  lo = pack2(x - h.x, y - h.y);
+}
+
+__device__ __forceinline__ void cp16(void* dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(on ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+template <int D>
+struct Shape {
+  static constexpr int LD = D + 8;                    // row pitch: eight 16-byte rows fall into different banks
+  static constexpr int NW = D == 128 ? 8 : 4;         // warps: 4 row groups of 16 tokens x column groups
+  static constexpr int NT = NW * 32;
+  static constexpr int OC = D == 128 ? 64 : D;        // output columns of a warp
+  static constexpr int SC = D == 32 ? 16 : D;         // state columns of a warp (16 rows)
+  static constexpr int TILE = C * LD;                 // elements
+  static constexpr int STATE = D * LD;
+};
+
+// Tokens t0 .. t0 + n - 1 of one head into a [C][LD] tile; the rest is zero.
+template <int D>
+__device__ __forceinline__ void load_tile(bf16* s, const TmpcSeqView& w, int b, int t0, int n, int h, int d, bool vec) {
+  using Z = Shape<D>;
+  const bf16* base = row_ptr<bf16>(w, b, t0, h);
+  if (vec) {
+    for (int u = threadIdx.x; u < C * D / 8; u += Z::NT) {
+      const int t = u / (D / 8), i = u % (D / 8) * 8;
+      const bool on = t < n && i < d;
+      cp16(s + t * Z::LD + i, on ? base + t * w.token + i : base, on);
+    }
+  } else {
+    for (int u = threadIdx.x; u < C * D; u += Z::NT) {
+      const int t = u / D, i = u % D;
+      s[t * Z::LD + i] = (t < n && i < d) ? base[t * w.token + i] : __float2bfloat16_rn(0.f);
+    }
+  }
+}
+
+// Fragment addresses: A (rows m, K k) of a row-major [m][k] tile; A of a tile
+// stored [k][m]; B (two 8-wide column tiles) of a tile stored [n][k], of one
+// stored [k][n].
+template <int LD>
+__device__ __forceinline__ const bf16* frag_a(const bf16* s, int m0, int k0) {
+  const int l = threadIdx.x & 31;
+  return s + (m0 + (l & 15)) * LD + k0 + (l >> 4) * 8;
+}
+template <int LD>
+__device__ __forceinline__ const bf16* frag_at(const bf16* s, int m0, int k0) {
+  const int l = threadIdx.x & 31;
+  return s + (k0 + (l & 7) + (l >> 4) * 8) * LD + m0 + ((l >> 3) & 1) * 8;
+}
+template <int LD>
+__device__ __forceinline__ const bf16* frag_bn(const bf16* s, int n0, int k0) {
+  const int l = threadIdx.x & 31;
+  return s + (n0 + (l & 7) + (l >> 4) * 8) * LD + k0 + ((l >> 3) & 1) * 8;
+}
+template <int LD>
+__device__ __forceinline__ const bf16* frag_bk(const bf16* s, int n0, int k0) {
+  const int l = threadIdx.x & 31;
+  return s + (k0 + (l & 7) + ((l >> 3) & 1) * 8) * LD + n0 + (l >> 4) * 8;
+}
+
+// The warp's 16 x SC part of the state, float registers: acc[j] is columns
+// col0 + 8 j .. + 7.
+template <int D>
+struct State {
+  using Z = Shape<D>;
+  float s[Z::SC / 8][4];
+  int row0, col0;
+  __device__ __forceinline__ State() {
+    const int w = threadIdx.x >> 5;
+    row0 = D == 32 ? (w & 1) * 16 : w * 16;
+    col0 = D == 32 ? (w >> 1) * 16 : 0;
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) {  // f(row, col, value&)
+    const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+#pragma unroll
+    for (int j = 0; j < Z::SC / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f(row0 + g + (e >> 1) * 8, col0 + j * 8 + 2 * t + (e & 1), s[j][e]);
+  }
+  // rows x cols of a float array, element (i, j) at p[i si + j sj]; zero elsewhere
+  __device__ __forceinline__ void load(const float* p, int rows, int cols, int si, int sj) {
+    each([&](int i, int j, float& v) { v = (p && i < rows && j < cols) ? p[(int64_t)i * si + (int64_t)j * sj] : 0.f; });
+  }
+  __device__ __forceinline__ void store(float* p, int rows, int cols, int si, int sj) {
+    each([&](int i, int j, float& v) {
+      if (i < rows && j < cols) p[(int64_t)i * si + (int64_t)j * sj] = v;
+    });
+  }
+  __device__ __forceinline__ void publish(bf16* hi, bf16* lo) {
+    const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+#pragma unroll
+    for (int j = 0; j < Z::SC / 8; ++j)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        uint32_t h, l;
+        split2(s[j][2 * r], s[j][2 * r + 1], h, l);
+        const int o = (row0 + g + r * 8) * Z::LD + col0 + j * 8 + 2 * t;
+        *reinterpret_cast<uint32_t*>(hi + o) = h;
+        *reinterpret_cast<uint32_t*>(lo + o) = l;
+      }
+  }
+  // s = keep s + sum over tokens of w(token) a_token b_token^T, tiles [token][.]
+  template <typename W>
+  __device__ __forceinline__ void update(const bf16* a, const bf16* b, float keep, int n, W&& w) {
+    const int t = threadIdx.x & 3;
+#pragma unroll
+    for (int j = 0; j < Z::SC / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[j][e] *= keep;
+    const int kt = (n + 15) / 16;
+#pragma unroll 1
+    for (int k = 0; k < kt; ++k) {
+      uint32_t f[4], hi[4], lo[4];
+      ldsm_t(f, frag_at<Z::LD>(a, row0, k * 16));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tok = k * 16 + 2 * t + (i >> 1) * 8;
+        const float2 x = unpack2(f[i]);
+        split2(x.x * w(tok), x.y * w(tok + 1), hi[i], lo[i]);
+      }
+#pragma unroll
+      for (int j = 0; j < Z::SC / 8; j += 2) {
+        uint32_t r[4];
+        ldsm_t(r, frag_bk<Z::LD>(b, col0 + j * 8, k * 16));
+        mma(s[j], hi, r[0], r[1]);
+        mma(s[j], lo, r[0], r[1]);
+        mma(s[j + 1], hi, r[2], r[3]);
+        mma(s[j + 1], lo, r[2], r[3]);
+      }
+    }
+  }
+};
+
+// The outputs' warp tile (16 tokens x OC columns) to global rows, through the
+// warp's rows of a tile nobody reads any more.
+template <int D>
+__device__ __forceinline__ void store_rows(const float (&o)[Shape<D>::OC / 8][4], bf16* stg, const TmpcSeqView& w, int b,
+                                           int t0, int n, int h, int d, bool vec) {
+  using Z = Shape<D>;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int row0 = (warp & 3) * 16, col0 = (warp >> 2) * Z::OC;
+#pragma unroll
+  for (int j = 0; j < Z::OC / 8; ++j) {
+    *reinterpret_cast<uint32_t*>(stg + (row0 + g) * Z::LD + col0 + j * 8 + 2 * t) = pack2(o[j][0], o[j][1]);
+    *reinterpret_cast<uint32_t*>(stg + (row0 + g + 8) * Z::LD + col0 + j * 8 + 2 * t) = pack2(o[j][2], o[j][3]);
+  }
+  __syncwarp();
+  bf16* base = row_ptr<bf16>(w, b, t0, h);
+  if (vec) {
+#pragma unroll
+    for (int u = lane; u < 16 * Z::OC / 8; u += 32) {
+      const int r = row0 + u / (Z::OC / 8), i = col0 + u % (Z::OC / 8) * 8;
+      if (r < n && i < d) *reinterpret_cast<uint4*>(base + r * w.token + i) = *reinterpret_cast<uint4*>(stg + r * Z::LD + i);
+    }
+  } else {
+    for (int u = lane; u < 16 * Z::OC; u += 32) {
+      const int r = row0 + u / Z::OC, i = col0 + u % Z::OC;
+      if (r < n && i < d) base[r * w.token + i] = stg[r * Z::LD + i];
+    }
+  }
+}
+
+// Rows t0 .. t1 - 1 of one head set to zero by the whole block.
+__device__ __forceinline__ void zero_rows(const TmpcSeqView& w, int b, int64_t t0, int64_t t1, int h, int d) {
+  for (int64_t u = threadIdx.x; u < (t1 - t0) * d; u += blockDim.x) {
+    const int64_t t = t0 + u / d;
+    row_ptr<bf16>(w, b, t, h)[u % d] = __float2bfloat16_rn(0.f);
+  }
+}
+
+// Roles of one pass of the forward kernel.
+struct FwdArgs {
+  TmpcSeqView q, k, v, o, x;  // x (dq only): the queries, for q . dq
+  const float* log_decay;
+  const int32_t* lengths;
+  const float* state_in;   // [B][H] x (e x f), element (i, j) at i si + j sj
+  float* state_out;
+  const float* seg_state;  // [B][H][nseg], same element order
+  float* part;             // dq only: [B][H][nseg * seg_len / C][2]: sum q . dq, sum (t + 1) q . dq
+  int T, H, G, e, f;       // key and value sizes of this pass
+  int si, sj;
+  int nseg, seg_len;
+  bool vec;
+  float scale;
+};
+
+template <int D>
+constexpr size_t fwd_smem(bool dq) {
+  using Z = Shape<D>;
+  return (size_t)(2 * (dq ? 4 : 3) * Z::TILE + 2 * Z::STATE) * 2 + (C + 1 + 16) * 4;
+}
+
+template <int D, bool DQ>
+__global__ void __launch_bounds__(Shape<D>::NT) fwd_kernel(const FwdArgs a) {
+  using Z = Shape<D>;
+  constexpr int NTILE = DQ ? 4 : 3;
+  extern __shared__ __align__(16) char raw[];
+  bf16* tiles = reinterpret_cast<bf16*>(raw);
+  bf16* s_hi = tiles + 2 * NTILE * Z::TILE;
+  bf16* s_lo = s_hi + Z::STATE;
+  float* pw = reinterpret_cast<float*>(s_lo + Z::STATE);  // d^i
+  float* red = pw + C + 1;
+
+  const int h = blockIdx.x % a.H;
+  const int seg = (blockIdx.x / a.H) % a.nseg, b = blockIdx.x / a.H / a.nseg;
+  const int g = h / (a.H / a.G);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gr = lane >> 2, tq = lane & 3;
+  const int row0 = (warp & 3) * 16, col0 = (warp >> 2) * Z::OC;
+  int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+  const int begin = seg * a.seg_len, stop = min(begin + a.seg_len, a.T);
+  len = min(max(len - begin, 0), stop - begin);  // valid tokens of the segment
+  const float g2 = log2_decay(a.log_decay, h);
+  for (int i = threadIdx.x; i <= C; i += Z::NT) pw[i] = exp2f(g2 * (float)i);
+
+  const int64_t bh = (int64_t)b * a.H + h, elems = (int64_t)a.e * a.f;
+  State<D> S;
+  const float* s0 = a.nseg > 1 ? a.seg_state + (bh * a.nseg + seg) * elems : a.state_in ? a.state_in + bh * elems : nullptr;
+  S.load(s0, a.e, a.f, a.si, a.sj);
+  S.publish(s_hi, s_lo);
+
+  auto load = [&](int i) {
+    bf16* buf = tiles + (i & 1) * NTILE * Z::TILE;
+    const int t0 = begin + i * C, n = min(C, len - i * C);
+    load_tile<D>(buf, a.q, b, t0, n, h, a.e, a.vec);
+    load_tile<D>(buf + Z::TILE, a.k, b, t0, n, g, a.e, a.vec);
+    load_tile<D>(buf + 2 * Z::TILE, a.v, b, t0, n, g, a.f, a.vec);
+    if constexpr (DQ) load_tile<D>(buf + 3 * Z::TILE, a.x, b, t0, n, h, a.f, a.vec);
+  };
+  const int chunks = (len + C - 1) / C;
+  if (chunks > 0) load(0);
+  cp_commit();
+  bool state_on = s0 != nullptr;
+  for (int i = 0; i < chunks; ++i) {
+    if (i + 1 < chunks) load(i + 1);
+    cp_commit();
+    cp_wait<1>();
+    __syncthreads();
+    bf16* sq = tiles + (i & 1) * NTILE * Z::TILE;
+    const bf16 *sk = sq + Z::TILE, *sv = sk + Z::TILE;
+    const int n = min(C, len - i * C);
+    if (row0 < n) {
+      uint32_t q[D / 16][4];
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) ldsm(q[k], frag_a<Z::LD>(sq, row0, k * 16));
+      float o[Z::OC / 8][4];
+#pragma unroll
+      for (int j = 0; j < Z::OC / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
+      if (state_on) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int j = 0; j < Z::OC / 8; j += 2) {
+            uint32_t r[4];
+            ldsm_t(r, frag_bk<Z::LD>(s_hi, col0 + j * 8, k * 16));
+            mma(o[j], q[k], r[0], r[1]);
+            mma(o[j + 1], q[k], r[2], r[3]);
+            ldsm_t(r, frag_bk<Z::LD>(s_lo, col0 + j * 8, k * 16));
+            mma(o[j], q[k], r[0], r[1]);
+            mma(o[j + 1], q[k], r[2], r[3]);
+          }
+        const float d0 = pw[row0 + gr + 1], d1 = pw[row0 + gr + 9];
+#pragma unroll
+        for (int j = 0; j < Z::OC / 8; ++j) o[j][0] *= d0, o[j][1] *= d0, o[j][2] *= d1, o[j][3] *= d1;
+      }
+      if constexpr (DQ) {
+        // q . dq of the part that comes from the state, rows weighted by t + 1 as well
+        const bf16* sx = sq + 3 * Z::TILE;
+        float p0 = 0.f, p1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < Z::OC / 8; ++j) {
+          const int c = col0 + j * 8 + 2 * tq;
+          const float2 x0 = unpack2(*reinterpret_cast<const uint32_t*>(sx + (row0 + gr) * Z::LD + c));
+          const float2 x1 = unpack2(*reinterpret_cast<const uint32_t*>(sx + (row0 + gr + 8) * Z::LD + c));
+          p0 = fmaf(x0.x, o[j][0], fmaf(x0.y, o[j][1], p0));
+          p1 = fmaf(x1.x, o[j][2], fmaf(x1.y, o[j][3], p1));
+        }
+        const float sum = warp_sum(p0 + p1);
+        const float wsum = warp_sum(p0 * (row0 + gr + 1) + p1 * (row0 + gr + 9));
+        if (lane == 0) red[warp] = sum, red[8 + warp] = wsum;
+      }
+      // scores against 16 tokens at a time, up to the warp's own
+#pragma unroll 1
+      for (int kt = 0; kt <= (warp & 3); ++kt) {
+        float s[2][4] = {};
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          uint32_t r[4];
+          ldsm(r, frag_bn<Z::LD>(sk, kt * 16, k * 16));
+          mma(s[0], q[k], r[0], r[1]);
+          mma(s[1], q[k], r[2], r[3]);
+        }
+        uint32_t p[4];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int lag = row0 + gr + (e >> 1) * 8 - (kt * 16 + c * 8 + 2 * tq + (e & 1));
+            s[c][e] = lag >= 0 ? s[c][e] * pw[max(lag, 0)] : 0.f;
+          }
+          p[2 * c] = pack2(s[c][0], s[c][1]);
+          p[2 * c + 1] = pack2(s[c][2], s[c][3]);
+        }
+#pragma unroll
+        for (int j = 0; j < Z::OC / 8; j += 2) {
+          uint32_t r[4];
+          ldsm_t(r, frag_bk<Z::LD>(sv, col0 + j * 8, kt * 16));
+          mma(o[j], p, r[0], r[1]);
+          mma(o[j + 1], p, r[2], r[3]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < Z::OC / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][e] *= a.scale;
+      // the queries' rows of this warp (of both column halves at D = 128) are free now
+      if constexpr (Z::NW == 8) asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
+      else __syncwarp();
+      store_rows<D>(o, sq, a.o, b, begin + i * C, n, h, a.f, a.vec);
+    } else if (DQ && lane == 0) {
+      red[warp] = 0.f, red[8 + warp] = 0.f;
+    }
+    if (i + 1 < chunks || a.state_out)
+      S.update(sk, sv, pw[n], n, [&](int s) { return pw[max(n - 1 - s, 0)]; });
+    state_on = true;
+    __syncthreads();
+    if (i + 1 < chunks) S.publish(s_hi, s_lo);
+    if constexpr (DQ) {
+      if (threadIdx.x < 2) {
+        float r = 0.f;
+        for (int w = 0; w < Z::NW; ++w) r += red[threadIdx.x * 8 + w];
+        a.part[((bh * a.nseg + seg) * (a.seg_len / C) + i) * 2 + threadIdx.x] = r * a.scale;
+      }
+    }
+  }
+  cp_wait<0>();
+  zero_rows(a.o, b, begin + len, stop, h, a.f);
+  if (a.state_out && seg == a.nseg - 1) S.store(a.state_out + bh * elems, a.e, a.f, a.si, a.sj);
+}
+
+// The state that a segment's tokens alone leave (REV false: sum d^(n-1-s) k v^T;
+// REV true: scale sum d^(t+1) q do^T, the adjoint they send back).
+template <int D, bool REV>
+__global__ void __launch_bounds__(Shape<D>::NT) segment_kernel(const LinAttnArgs a, float* out) {
+  using Z = Shape<D>;
+  extern __shared__ __align__(16) char raw[];
+  bf16* tiles = reinterpret_cast<bf16*>(raw);
+  float* pw = reinterpret_cast<float*>(tiles + 4 * Z::TILE);
+  const int h = blockIdx.x % a.H;
+  const int seg = (blockIdx.x / a.H) % a.nseg, b = blockIdx.x / a.H / a.nseg;
+  const int g = h / (a.H / a.G);
+  const int begin = seg * a.seg_len, stop = min(begin + a.seg_len, a.T);
+  const int len = min(max(seq_len(a, b) - begin, 0), stop - begin);
+  const float g2 = log2_decay(a.log_decay, h);
+  for (int i = threadIdx.x; i <= C; i += Z::NT) pw[i] = exp2f(g2 * (float)i);
+  State<D> S;
+  S.load(nullptr, 0, 0, 0, 0);
+  const int chunks = (len + C - 1) / C;
+  auto load = [&](int i) {
+    bf16* buf = tiles + (i & 1) * 2 * Z::TILE;
+    const int c = REV ? chunks - 1 - i : i, t0 = begin + c * C, n = min(C, len - c * C);
+    load_tile<D>(buf, REV ? a.q : a.k, b, t0, n, REV ? h : g, a.dk, a.vec);
+    load_tile<D>(buf + Z::TILE, REV ? a.o : a.v, b, t0, n, REV ? h : g, a.dv, a.vec);
+  };
+  if (chunks > 0) load(0);
+  cp_commit();
+  for (int i = 0; i < chunks; ++i) {
+    if (i + 1 < chunks) load(i + 1);
+    cp_commit();
+    cp_wait<1>();
+    __syncthreads();
+    const bf16* ta = tiles + (i & 1) * 2 * Z::TILE;
+    const int c = REV ? chunks - 1 - i : i, n = min(C, len - c * C);
+    S.update(ta, ta + Z::TILE, pw[n], n, [&](int t) { return REV ? pw[min(t + 1, C)] * a.scale : pw[max(n - 1 - t, 0)]; });
+    __syncthreads();
+  }
+  cp_wait<0>();
+  S.store(out + (((int64_t)b * a.H + h) * a.nseg + seg) * a.dk * a.dv, a.dk, a.dv, a.dv, 1);
+}
+
+// In place: what each segment leaves alone -> the state before each segment
+// (REV: the adjoint after each segment), starting from `first`.
+template <bool REV>
+__global__ void __launch_bounds__(256) scan_kernel(const LinAttnArgs a, float* seg, const float* first) {
+  const int64_t elems = (int64_t)a.dk * a.dv, bh = blockIdx.y;
+  const int b = (int)(bh / a.H), h = (int)(bh % a.H);
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= elems) return;
+  const int len = seq_len(a, b);
+  const float g2 = log2_decay(a.log_decay, h);
+  float s = first ? first[bh * elems + i] : 0.f;
+  for (int k = 0; k < a.nseg; ++k) {
+    const int m = REV ? a.nseg - 1 - k : k;
+    float* p = seg + (bh * a.nseg + m) * elems + i;
+    const int n = min(max(len - m * a.seg_len, 0), a.seg_len);
+    const float own = *p;
+    *p = s;
+    s = fmaf(exp2f(g2 * (float)n), s, own);
+  }
+}
+
+// dk and dv of one (sequence, key head, segment), backward in time; the query
+// heads of the key head one after another, their sums in a.acc until the last.
+struct DkvArgs {
+  LinAttnArgs a;
+  float* part;  // [B][H][chunks][3]: intra-chunk share of dlog d, sum k . dk, sum (n - 1 - s) k . dk
+  float* edge;  // [B][H][nseg]: <state before the segment's first token, its adjoint>, first segment only
+};
+
+template <int D>
+constexpr size_t dkv_smem() {
+  using Z = Shape<D>;
+  return (size_t)(4 * Z::TILE + 2 * Z::STATE) * 2 + (C + 1 + 24) * 4;
+}
+
+template <int D>
+__global__ void __launch_bounds__(Shape<D>::NT) dkv_kernel(const DkvArgs args) {
+  using Z = Shape<D>;
+  const LinAttnArgs& a = args.a;
+  extern __shared__ __align__(16) char raw[];
+  bf16* sq = reinterpret_cast<bf16*>(raw);
+  bf16 *sk = sq + Z::TILE, *sv = sk + Z::TILE, *sdo = sv + Z::TILE;
+  bf16* r_hi = sdo + Z::TILE;
+  bf16* r_lo = r_hi + Z::STATE;
+  float* pw = reinterpret_cast<float*>(r_lo + Z::STATE);
+  float* red = pw + C + 1;
+
+  const int g = blockIdx.x % a.G;
+  const int seg = (blockIdx.x / a.G) % a.nseg, b = blockIdx.x / a.G / a.nseg;
+  const int rep = a.H / a.G;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gr = lane >> 2, tq = lane & 3;
+  const int row0 = (warp & 3) * 16, col0 = (warp >> 2) * Z::OC;
+  const int begin = seg * a.seg_len, stop = min(begin + a.seg_len, a.T);
+  const int len = min(max(seq_len(a, b) - begin, 0), stop - begin);
+  const int chunks = (len + C - 1) / C, all_chunks = a.nseg * (a.seg_len / C);
+  const int64_t elems = (int64_t)a.dk * a.dv;
+
+  for (int r = 0; r < rep; ++r) {
+    const int h = g * rep + r;
+    const int64_t bh = (int64_t)b * a.H + h;
+    const float g2 = log2_decay(a.log_decay, h);
+    __syncthreads();
+    for (int i = threadIdx.x; i <= C; i += Z::NT) pw[i] = exp2f(g2 * (float)i);
+    State<D> R;
+    const float* r0 = a.nseg > 1 ? a.seg_dstate + (bh * a.nseg + seg) * elems
+                                 : a.dstate_out ? a.dstate_out + bh * elems : nullptr;
+    R.load(r0, a.dk, a.dv, a.dv, 1);
+    R.publish(r_hi, r_lo);
+    bool state_on = r0 != nullptr;
+    for (int i = chunks - 1; i >= 0; --i) {
+      const int t0 = begin + i * C, n = min(C, len - i * C);
+      load_tile<D>(sq, a.q, b, t0, n, h, a.dk, a.vec);
+      load_tile<D>(sk, a.k, b, t0, n, g, a.dk, a.vec);
+      load_tile<D>(sv, a.v, b, t0, n, g, a.dv, a.vec);
+      load_tile<D>(sdo, a.o, b, t0, n, h, a.dv, a.vec);
+      cp_commit();
+      cp_wait<0>();
+      __syncthreads();
+      float dk[Z::OC / 8][4], dv[Z::OC / 8][4];
+      float intra = 0.f, ksum = 0.f, kwsum = 0.f;
+      if (row0 < n) {
+#pragma unroll
+        for (int j = 0; j < Z::OC / 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dk[j][e] = dv[j][e] = 0.f;
+        if (state_on) {
+#pragma unroll 2
+          for (int k = 0; k < D / 16; ++k) {
+            uint32_t ka[4], va[4];
+            ldsm(ka, frag_a<Z::LD>(sk, row0, k * 16));
+            ldsm(va, frag_a<Z::LD>(sv, row0, k * 16));
+#pragma unroll
+            for (int j = 0; j < Z::OC / 8; j += 2) {
+              uint32_t f[4];
+              ldsm_t(f, frag_bk<Z::LD>(r_hi, col0 + j * 8, k * 16));  // R[dk][dv]: dv_s = R^T k_s
+              mma(dv[j], ka, f[0], f[1]);
+              mma(dv[j + 1], ka, f[2], f[3]);
+              ldsm(f, frag_bn<Z::LD>(r_hi, col0 + j * 8, k * 16));    // dk_s = R v_s
+              mma(dk[j], va, f[0], f[1]);
+              mma(dk[j + 1], va, f[2], f[3]);
+              ldsm(f, frag_bn<Z::LD>(r_lo, col0 + j * 8, k * 16));
+              mma(dk[j], va, f[0], f[1]);
+              mma(dk[j + 1], va, f[2], f[3]);
+            }
+          }
+          const int s0 = row0 + gr, s1 = s0 + 8;
+          const float d0 = pw[max(n - 1 - s0, 0)], d1 = pw[max(n - 1 - s1, 0)];
+          float p0 = 0.f, p1 = 0.f;
+#pragma unroll
+          for (int j = 0; j < Z::OC / 8; ++j) {
+            dv[j][0] *= d0, dv[j][1] *= d0, dv[j][2] *= d1, dv[j][3] *= d1;
+            dk[j][0] *= d0, dk[j][1] *= d0, dk[j][2] *= d1, dk[j][3] *= d1;
+            const int c = col0 + j * 8 + 2 * tq;
+            const float2 k0 = unpack2(*reinterpret_cast<const uint32_t*>(sk + s0 * Z::LD + c));
+            const float2 k1 = unpack2(*reinterpret_cast<const uint32_t*>(sk + s1 * Z::LD + c));
+            p0 = fmaf(k0.x, dk[j][0], fmaf(k0.y, dk[j][1], p0));
+            p1 = fmaf(k1.x, dk[j][2], fmaf(k1.y, dk[j][3], p1));
+          }
+          ksum = p0 + p1;
+          kwsum = p0 * (float)(n - 1 - s0) + p1 * (float)(n - 1 - s1);
+        }
+        // scores of the warp's 16 keys against 16 queries at a time, from its own on
+#pragma unroll 1
+        for (int kt = warp & 3; kt * 16 < n; ++kt) {
+          float s1[2][4] = {}, s2[2][4] = {};
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            uint32_t fa[4], f[4];
+            ldsm(fa, frag_a<Z::LD>(sk, row0, k * 16));
+            ldsm(f, frag_bn<Z::LD>(sq, kt * 16, k * 16));
+            mma(s1[0], fa, f[0], f[1]);
+            mma(s1[1], fa, f[2], f[3]);
+            ldsm(fa, frag_a<Z::LD>(sv, row0, k * 16));
+            ldsm(f, frag_bn<Z::LD>(sdo, kt * 16, k * 16));
+            mma(s2[0], fa, f[0], f[1]);
+            mma(s2[1], fa, f[2], f[3]);
+          }
+          uint32_t p1[4], p2[4];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int lag = kt * 16 + c * 8 + 2 * tq + (e & 1) - (row0 + gr + (e >> 1) * 8);
+              const float w = lag >= 0 ? pw[max(lag, 0)] * a.scale : 0.f;
+              s1[c][e] *= w;
+              if (col0 == 0) intra = fmaf((float)lag * s1[c][e], s2[c][e], intra);
+              s2[c][e] *= w;
+            }
+            p1[2 * c] = pack2(s1[c][0], s1[c][1]), p1[2 * c + 1] = pack2(s1[c][2], s1[c][3]);
+            p2[2 * c] = pack2(s2[c][0], s2[c][1]), p2[2 * c + 1] = pack2(s2[c][2], s2[c][3]);
+          }
+#pragma unroll
+          for (int j = 0; j < Z::OC / 8; j += 2) {
+            uint32_t f[4];
+            ldsm_t(f, frag_bk<Z::LD>(sdo, col0 + j * 8, kt * 16));
+            mma(dv[j], p1, f[0], f[1]);
+            mma(dv[j + 1], p1, f[2], f[3]);
+            ldsm_t(f, frag_bk<Z::LD>(sq, col0 + j * 8, kt * 16));
+            mma(dk[j], p2, f[0], f[1]);
+            mma(dk[j + 1], p2, f[2], f[3]);
+          }
+        }
+      }
+      intra = warp_sum(intra), ksum = warp_sum(ksum), kwsum = warp_sum(kwsum);
+      if (lane == 0) red[warp] = intra, red[8 + warp] = ksum, red[16 + warp] = kwsum;
+      if (i > 0 || a.dstate_in || args.edge)
+        R.update(sq, sdo, pw[n], n, [&](int t) { return pw[min(t + 1, C)] * a.scale; });
+      state_on = true;
+      __syncthreads();
+      if (i > 0) R.publish(r_hi, r_lo);
+      if (threadIdx.x < 3) {
+        float s = 0.f;
+        for (int w = 0; w < Z::NW; ++w) s += red[threadIdx.x * 8 + w];
+        args.part[(bh * all_chunks + seg * (a.seg_len / C) + i) * 3 + threadIdx.x] = s;
+      }
+      if (row0 < n) {
+        if (rep > 1) {  // the key head's sum so far, [token][dk | dv] float
+          float* acc = a.acc + ((int64_t)b * a.T + t0) * a.G * (a.dk + a.dv) + (int64_t)g * (a.dk + a.dv);
+          const int64_t pitch = (int64_t)a.G * (a.dk + a.dv);
+#pragma unroll
+          for (int j = 0; j < Z::OC / 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int s = row0 + gr + (e >> 1) * 8, c = col0 + j * 8 + 2 * tq + (e & 1);
+              if (s < n && c < a.dk) {
+                float* p = acc + s * pitch + c;
+                if (r > 0) dk[j][e] += *p;
+                if (r + 1 < rep) *p = dk[j][e];
+              }
+              if (s < n && c < a.dv) {
+                float* p = acc + s * pitch + a.dk + c;
+                if (r > 0) dv[j][e] += *p;
+                if (r + 1 < rep) *p = dv[j][e];
+              }
+            }
+        }
+        if (r + 1 == rep) {
+          store_rows<D>(dk, sk, a.gk, b, t0, n, g, a.dk, a.vec);
+          store_rows<D>(dv, sv, a.gv, b, t0, n, g, a.dv, a.vec);
+        }
+      }
+      __syncthreads();
+    }
+    if (seg == 0) {
+      if (args.edge) {
+        float e = 0.f;
+        if (a.state_in)
+          R.each([&](int i, int j, float& v) {
+            if (i < a.dk && j < a.dv) e = fmaf(v, a.state_in[bh * elems + (int64_t)i * a.dv + j], e);
+          });
+        e = warp_sum(e);
+        if (lane == 0) red[warp] = e;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+          float s = 0.f;
+          for (int w = 0; w < Z::NW; ++w) s += red[w];
+          args.edge[bh] = s;
+        }
+      }
+      if (a.dstate_in) R.store(a.dstate_in + bh * elems, a.dk, a.dv, a.dv, 1);
+    }
+  }
+  zero_rows(a.gk, b, begin + len, stop, g, a.dk);
+  zero_rows(a.gv, b, begin + len, stop, g, a.dv);
+}
+
+// dlog d per (sequence, head) from the chunks' shares, then the sum over the batch.
+__global__ void __launch_bounds__(256) dlog_kernel(const LinAttnArgs a, const float* pq, const float* pk,
+                                                  const float* edge, float* out) {
+  __shared__ double red[8];
+  const int h = blockIdx.x;
+  const float g2 = log2_decay(a.log_decay, h);
+  const int all_chunks = a.nseg * (a.seg_len / C);
+  double sum = 0;
+  for (int b = threadIdx.x; b < a.B; b += 256) {
+    const int64_t bh = (int64_t)b * a.H + h;
+    const int len = seq_len(a, b);
+    double e = edge[bh];
+    for (int i = 0; i * C < len; ++i) {
+      const int n = min(C, len - i * C);
+      const float *q = pq + (bh * all_chunks + i) * 2, *k = pk + (bh * all_chunks + i) * 3;
+      const double x = g2 * (float)n < -20.f ? 0.0 : e - (double)q[0];
+      sum += (double)k[0] + (double)q[1] + (double)k[2] + n * x;
+      e = x + (double)k[1];
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; ++i) sum += red[i];
+    out[h] = (float)sum;
+  }
+}
+
+template <typename K>
+int set_smem(K kern, size_t bytes) {
+  return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
+inline int64_t resident_blocks(const TmpcLinAttnDims* d) {
+  const int m = std::max(d->dk, d->dv);
+  return (int64_t)sm_count() * (m <= 64 ? 2 : 1);
+}
+
+// Two passes over a segment cost nearly twice one pass over the sequence, so
+// the cut pays from the point where the pairs fill less than half the device.
+template <bool REV>
+int run_segments(const LinAttnArgs& a, const TmpcLinAttnDims* d, float* seg, const float* first, cudaStream_t st) {
+  int rc = 0;
+  by_size(d, [&](auto dd) {
+    constexpr int D = decltype(dd)::value;
+    const size_t smem = (size_t)4 * Shape<D>::TILE * 2 + (C + 1) * 4;
+    rc = set_smem(segment_kernel<D, REV>, smem);
+    if (!rc)
+      segment_kernel<D, REV><<<(unsigned)((int64_t)a.B * a.nseg * a.H), Shape<D>::NT, smem, st>>>(a, seg);
+  });
+  if (rc) return rc;
+  scan_kernel<REV><<<dim3((unsigned)((a.dk * a.dv + 255) / 256), (unsigned)(a.B * a.H)), 256, 0, st>>>(a, seg, first);
+  return (int)cudaPeekAtLastError();
+}
+
+template <bool DQ>
+int run_fwd(const FwdArgs& f, const LinAttnArgs& a, const TmpcLinAttnDims* d, cudaStream_t st) {
+  int rc = 0;
+  by_size(d, [&](auto dd) {
+    constexpr int D = decltype(dd)::value;
+    rc = set_smem(fwd_kernel<D, DQ>, fwd_smem<D>(DQ));
+    if (!rc)
+      fwd_kernel<D, DQ><<<(unsigned)((int64_t)a.B * a.nseg * a.H), Shape<D>::NT, fwd_smem<D>(DQ), st>>>(f);
+  });
+  return rc ? rc : (int)cudaPeekAtLastError();
+}
+
+struct BackwardPlan {
+  size_t seg_state, seg_dstate, pq, pk, edge, acc, total;
+};
+
+inline BackwardPlan backward_plan(const LinAttnArgs& a, const TmpcLinAttnDims* d) {
+  BackwardPlan p{};
+  size_t at = 0;
+  auto take = [&](size_t floats) {
+    const size_t o = at;
+    at = (at + floats * 4 + 255) / 256 * 256;
+    return o;
+  };
+  const size_t bh = (size_t)d->B * d->H, chunks = (size_t)a.nseg * (a.seg_len / C), elems = (size_t)d->dk * d->dv;
+  if (a.nseg > 1) {
+    p.seg_state = take(bh * a.nseg * elems);
+    p.seg_dstate = take(bh * a.nseg * elems);
+  }
+  p.pq = take(bh * chunks * 2);
+  p.pk = take(bh * chunks * 3);
+  p.edge = take(bh);
+  p.acc = take(d->H > d->G ? (size_t)d->B * d->T * d->G * (d->dk + d->dv) : 0);
+  p.total = at;
+  return p;
+}
+
+inline LinAttnArgs sized(const TmpcLinAttnDims* d, int64_t heads) {
+  LinAttnArgs a{};
+  a.B = d->B, a.T = d->T, a.H = d->H, a.G = d->G, a.dk = d->dk, a.dv = d->dv;
+  set_segments(a, (int64_t)d->B * heads, resident_blocks(d));
+  return a;
+}
+
+}  // namespace la
+
+template <>
+size_t LinAttn<bf16>::forward_ws(const TmpcLinAttnDims* d) {
+  const LinAttnArgs a = la::sized(d, d->H);
+  return a.nseg > 1 ? (size_t)d->B * d->H * a.nseg * d->dk * d->dv * 4 : 0;
+}
+
+template <>
+int LinAttn<bf16>::forward(LinAttnArgs a, const TmpcLinAttnDims* d, char* ws, cudaStream_t st) {
+  const LinAttnArgs z = la::sized(d, d->H);
+  a.nseg = z.nseg, a.seg_len = z.seg_len;
+  a.vec = rows_aligned(a.q, d->dk, 2) && rows_aligned(a.k, d->dk, 2) && rows_aligned(a.v, d->dv, 2) &&
+          rows_aligned(a.o, d->dv, 2);
+  float* seg = reinterpret_cast<float*>(ws);
+  if (a.nseg > 1) {
+    const int rc = la::run_segments<false>(a, d, seg, a.state_in, st);
+    if (rc) return rc;
+  }
+  const la::FwdArgs f{a.q, a.k, a.v, a.o, a.o, a.log_decay, a.lengths, a.state_in, a.state_out, seg, nullptr,
+                      a.T, a.H, a.G, a.dk, a.dv, a.dv, 1, a.nseg, a.seg_len, a.vec, a.scale};
+  return la::run_fwd<false>(f, a, d, st);
+}
+
+template <>
+size_t LinAttn<bf16>::backward_ws(const TmpcLinAttnDims* d) {
+  return la::backward_plan(la::sized(d, d->G), d).total;
+}
+
+template <>
+int LinAttn<bf16>::backward(LinAttnArgs a, const TmpcLinAttnDims* d, float* dlog_decay, char* ws, cudaStream_t st) {
+  const LinAttnArgs z = la::sized(d, d->G);
+  a.nseg = z.nseg, a.seg_len = z.seg_len;
+  a.vec = rows_aligned(a.q, d->dk, 2) && rows_aligned(a.k, d->dk, 2) && rows_aligned(a.v, d->dv, 2) &&
+          rows_aligned(a.o, d->dv, 2) && rows_aligned(a.gq, d->dk, 2) && rows_aligned(a.gk, d->dk, 2) &&
+          rows_aligned(a.gv, d->dv, 2);
+  const la::BackwardPlan p = la::backward_plan(a, d);
+  auto at = [&](size_t o) { return reinterpret_cast<float*>(ws + o); };
+  if (a.nseg > 1) {
+    a.seg_state = at(p.seg_state);
+    a.seg_dstate = at(p.seg_dstate);
+    int rc = la::run_segments<false>(a, d, a.seg_state, a.state_in, st);
+    if (!rc) rc = la::run_segments<true>(a, d, a.seg_dstate, a.dstate_out, st);
+    if (rc) return rc;
+  }
+  a.acc = at(p.acc);
+  // dq: the forward sum over (do, v, k) with the transposed state
+  const la::FwdArgs f{a.o, a.v, a.k, a.gq, a.q, a.log_decay, a.lengths, a.state_in, nullptr, a.seg_state, at(p.pq),
+                      a.T, a.H, a.G, a.dv, a.dk, 1, a.dv, a.nseg, a.seg_len, a.vec, a.scale};
+  int rc = la::run_fwd<true>(f, a, d, st);
+  if (rc) return rc;
+  const la::DkvArgs k{a, at(p.pk), dlog_decay ? at(p.edge) : nullptr};
+  by_size(d, [&](auto dd) {
+    constexpr int D = decltype(dd)::value;
+    rc = la::set_smem(la::dkv_kernel<D>, la::dkv_smem<D>());
+    if (!rc)
+      la::dkv_kernel<D><<<(unsigned)((int64_t)a.B * a.nseg * a.G), la::Shape<D>::NT, la::dkv_smem<D>(), st>>>(k);
+  });
+  if (rc) return rc;
+  if (dlog_decay) la::dlog_kernel<<<a.H, 256, 0, st>>>(a, at(p.pq), at(p.pk), at(p.edge), dlog_decay);
+  return (int)cudaPeekAtLastError();
+}
+
+}  // namespace seq
+}  // namespace tmpc

@@ -1,0 +1,103 @@
+// Linear attention with a decay per head: what the float and the bfloat16
+// kernels share (arguments, segments, checks).
+#pragma once
+
+#include <algorithm>
+
+#include "seq_common.cuh"
+
+namespace tmpc {
+namespace seq {
+
+constexpr int kChunk = 64;  // tokens per chunk of the bfloat16 kernels; segments are multiples of it
+
+// Arguments of one call.  A sequence is cut into nseg segments of seg_len
+// tokens that run side by side; with nseg > 1 `seg_state` ([B][H][nseg] dk x
+// dv) holds the state before each segment, `seg_dstate` its adjoint after it.
+struct LinAttnArgs {
+  TmpcSeqView q, k, v, o, gq, gk, gv;  // o: the output, or its gradient; gq, gk, gv: gradients of q, k, v
+  const float* log_decay;
+  const int32_t* lengths;
+  const float* state_in;
+  float* state_out;
+  const float* dstate_out;
+  float* dstate_in;
+  float* seg_state;
+  float* seg_dstate;
+  float* acc;    // dk, dv summed over a key head's query heads: one slot of [T][dk + dv] per block, or per (b, g)
+  float* dlog;   // partial sums of dlog d
+  int B, T, H, G, dk, dv;
+  int nseg, seg_len;
+  bool vec;      // every row is a multiple of 16 bytes at 16-byte addresses
+  float scale;
+};
+
+template <typename T>
+__device__ __forceinline__ T* row_ptr(const TmpcSeqView& w, int64_t b, int64_t t, int64_t h) {
+  return static_cast<T*>(w.ptr) + b * w.batch + t * w.token + h * w.head;
+}
+
+// log2 of the decay; the clamp keeps 0 * log(0) finite (2^-1e4 is 0 in float).
+__device__ __forceinline__ float log2_decay(const float* log_decay, int h) {
+  return fmaxf(log_decay[h] * 1.4426950408889634f, -1e4f);
+}
+
+__device__ __forceinline__ int seq_len(const LinAttnArgs& a, int b) {
+  return a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+}
+
+inline int check_dims(const TmpcLinAttnDims* d) {
+  if (!d) return TMPC_ERR_NULL_ARG;
+  if (d->B < 0 || d->T < 0 || d->H < 1 || d->G < 1 || d->H % d->G || d->dk < 1 || d->dv < 1) return TMPC_ERR_BAD_DIMS;
+  if (d->dk > 128 || d->dv > 128 || d->H > 65535 || (int64_t)d->B * d->H > INT32_MAX)
+    return TMPC_ERR_UNSUPPORTED;
+  return TMPC_OK;
+}
+
+// Rows of d elements of esize bytes read and written 16 bytes at a time?
+inline bool rows_aligned(const TmpcSeqView& w, int d, int esize) {
+  const int n = 16 / esize;
+  return d % n == 0 && w.batch % n == 0 && w.token % n == 0 && w.head % n == 0 && aligned(w.ptr, 16);
+}
+
+// Calls f with the compiled head size, 32, 64 or 128.
+template <typename F>
+void by_size(const TmpcLinAttnDims* d, F&& f) {
+  const int m = d->dk > d->dv ? d->dk : d->dv;
+  if (m <= 32) f(std::integral_constant<int, 32>{});
+  else if (m <= 64) f(std::integral_constant<int, 64>{});
+  else f(std::integral_constant<int, 128>{});
+}
+
+// Segments of a call with `lanes` independent (sequence, head) pairs, of which
+// `resident` fit on the device at once: none while the pairs fill it; else
+// enough to fill it, each at least four chunks long.
+inline void set_segments(LinAttnArgs& a, int64_t lanes, int64_t resident) {
+  const int64_t chunks = ((int64_t)a.T + kChunk - 1) / kChunk;
+  int64_t n = lanes > 0 && lanes * 2 <= resident ? resident / lanes : 1;
+  n = std::max<int64_t>(1, std::min<int64_t>(n, chunks / 4));
+  const int64_t per = (chunks + n - 1) / n;
+  a.seg_len = (int)(std::max<int64_t>(per, 1) * kChunk);
+  a.nseg = (int)std::max<int64_t>(1, (chunks + per - 1) / std::max<int64_t>(per, 1));
+}
+
+// Forward and backward of each element type; ws sizes are in bytes, arguments checked.
+template <typename T>
+struct LinAttn {
+  static size_t forward_ws(const TmpcLinAttnDims* d);
+  static size_t backward_ws(const TmpcLinAttnDims* d);
+  static int forward(LinAttnArgs a, const TmpcLinAttnDims* d, char* ws, cudaStream_t st);
+  static int backward(LinAttnArgs a, const TmpcLinAttnDims* d, float* dlog_decay, char* ws, cudaStream_t st);
+};
+
+template <>
+size_t LinAttn<bf16>::forward_ws(const TmpcLinAttnDims* d);
+template <>
+size_t LinAttn<bf16>::backward_ws(const TmpcLinAttnDims* d);
+template <>
+int LinAttn<bf16>::forward(LinAttnArgs a, const TmpcLinAttnDims* d, char* ws, cudaStream_t st);
+template <>
+int LinAttn<bf16>::backward(LinAttnArgs a, const TmpcLinAttnDims* d, float* dlog_decay, char* ws, cudaStream_t st);
+
+}  // namespace seq
+}  // namespace tmpc

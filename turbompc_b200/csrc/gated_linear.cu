@@ -84,7 +84,10 @@ inline int dw_splits(int64_t rows, int64_t tiles, int sms) {
   return best;
 }
 
-inline int tile_n(int n) { return n > 128 ? 256 : n > 64 ? 128 : 64; }
+template <typename T>
+int tile_n(int n) {
+  return n > 128 && sizeof(T) == 2 ? 256 : n > 64 ? 128 : 64;
+}
 
 inline Plan make_plan(int64_t rows, int d, int f, int esize, bool backward) {
   Plan p{};
@@ -104,7 +107,7 @@ inline Plan make_plan(int64_t rows, int d, int f, int esize, bool backward) {
     p.wu = take((int64_t)p.comps * f * p.dp * 2);
   }
   if (backward) {
-    const int nt = tile_n(d);
+    const int nt = esize == 4 ? tile_n<float>(d) : tile_n<bf16>(d);
     const int64_t tiles = (2 * (int64_t)p.fp + gemm::BM - 1) / gemm::BM * ((d + nt - 1) / nt);
     p.splits = dw_splits(rows, tiles, sm_count());
     p.dgu = take(p.comps * rows * 2 * p.fp * 2);
@@ -115,10 +118,8 @@ inline Plan make_plan(int64_t rows, int d, int f, int esize, bool backward) {
 }
 
 template <typename T>
-int vec_bytes(int cols, const void* a) {
-  for (int v : {16, 4})
-    if ((int64_t)cols * (int64_t)sizeof(T) % v == 0 && aligned(a, v)) return v;
-  return sizeof(T);
+bool wide_rows(int cols, const void* a) {
+  return (int64_t)cols * (int64_t)sizeof(T) % 16 == 0 && aligned(a, 16);
 }
 
 struct Operands {
@@ -141,32 +142,35 @@ Operands pack_operands(const Plan& p, int64_t rows, int d, int f, const T* x, co
 template <typename T, int MODE>
 int dual(const Plan& p, const Operands& o, int64_t rows, int d, int f, int act, void* out, const T* dh, bf16* dgu,
          cudaStream_t st) {
+  constexpr int BK = gemm::kBK<T>;
   gemm::Params q{};
   q.M = rows;
   q.N = f;
   q.fp = p.fp;
-  q.kblocks = (d + gemm::BK - 1) / gemm::BK;
-  q.nterms = p.comps == 3 ? 6 : 1;
+  q.kblocks = (d + BK - 1) / BK;
   q.splits = 1;
   q.mtiles = (int)((rows + gemm::BM - 1) / gemm::BM);
-  q.act = act;
   q.out = out;
   q.dh = dh;
-  q.dgu = dgu;
-  q.vec = vec_bytes<T>(f, MODE == gemm::kDact ? (const void*)dh : out);
+  q.wide = wide_rows<T>(f, MODE == gemm::kDact ? (const void*)dh : out);
   const int cols = MODE == gemm::kDact ? p.fp : f;  // dg | du is written to its padded width
   gemm::Maps maps;
   auto run = [&](auto NT) {
     constexpr int nt = decltype(NT)::value;
-    int rc = gemm::make_map(&maps.a, o.x, d, rows, p.comps, p.dp, gemm::BM);
-    if (!rc) rc = gemm::make_map(&maps.b0, o.wg, d, f, p.comps, p.dp, nt / 2);
-    if (!rc) rc = gemm::make_map(&maps.b1, o.wu, d, f, p.comps, p.dp, nt / 2);
+    int rc = gemm::make_map(&maps.a, o.x, d, rows, p.comps, p.dp, BK, gemm::BM);
+    if (!rc) rc = gemm::make_map(&maps.b0, o.wg, d, f, p.comps, p.dp, BK, nt / 2);
+    if (!rc) rc = gemm::make_map(&maps.b1, o.wu, d, f, p.comps, p.dp, BK, nt / 2);
+    if (!rc && MODE == gemm::kDact)
+      rc = gemm::make_map(&maps.c, dgu, 2 * p.fp, rows, p.comps, 2 * p.fp, gemm::Config<T, MODE, nt>::kCols, 32);
     if (rc) return rc;
     q.ntiles = (cols + nt / 2 - 1) / (nt / 2);
-    return gemm::launch<T, MODE, nt>(maps, q, st);
+    return act == TMPC_ACT_SILU ? gemm::launch<T, MODE, nt, TMPC_ACT_SILU>(maps, q, st)
+                                : gemm::launch<T, MODE, nt, TMPC_ACT_GELU>(maps, q, st);
   };
   // Few tokens: narrow tiles, so that the columns spread over more SMs.
-  if ((int64_t)q.mtiles * ((cols + 127) / 128) >= sm_count()) return run(std::integral_constant<int, 256>{});
+  constexpr int kWide = sizeof(T) == 4 ? 128 : 256;
+  if ((int64_t)q.mtiles * ((cols + kWide / 2 - 1) / (kWide / 2)) >= sm_count())
+    return run(std::integral_constant<int, kWide>{});
   return run(std::integral_constant<int, 64>{});
 }
 
@@ -185,22 +189,25 @@ int gated_fwd(int64_t rows, int d, int f, const T* x, const T* wg, const T* wu, 
 }
 
 template <typename T, int MODE>
-int single(const gemm::Params& q0, int d, const void* a, int64_t a_inner, int64_t a_outer, int64_t a_pitch, int a_box,
+int single(const gemm::Params& q0, int d, const void* a, int64_t a_inner, int64_t a_outer, int64_t a_pitch,
            const void* b0, const void* b1, int64_t b_outer, int64_t b_pitch, int comps, cudaStream_t st) {
+  constexpr int BK = gemm::kBK<T>;
   auto run = [&](auto NT) {
     constexpr int nt = decltype(NT)::value;
     gemm::Params q = q0;
     gemm::Maps maps;
-    int rc = gemm::make_map(&maps.a, a, a_inner, a_outer, comps, a_pitch, a_box);
-    if (!rc) rc = gemm::make_map(&maps.b0, b0, d, b_outer, comps, b_pitch, 64);
-    if (!rc) rc = gemm::make_map(&maps.b1, b1, d, b_outer, comps, b_pitch, 64);
+    int rc = MODE == gemm::kDw ? gemm::make_map(&maps.a, a, a_inner, a_outer, comps, a_pitch, 64, BK)
+                               : gemm::make_map(&maps.a, a, a_inner, a_outer, comps, a_pitch, BK, gemm::BM);
+    if (!rc) rc = gemm::make_map(&maps.b0, b0, d, b_outer, comps, b_pitch, 64, BK);
+    if (!rc) rc = gemm::make_map(&maps.b1, b1, d, b_outer, comps, b_pitch, 64, BK);
     if (rc) return rc;
     q.mtiles = (int)((q.M + gemm::BM - 1) / gemm::BM);
     q.ntiles = (d + nt - 1) / nt;
-    return gemm::launch<T, MODE, nt>(maps, q, st);
+    return gemm::launch<T, MODE, nt, TMPC_ACT_SILU>(maps, q, st);
   };
-  const int nt = tile_n(d);
-  if (nt == 256) return run(std::integral_constant<int, 256>{});
+  const int nt = tile_n<T>(d);
+  if constexpr (sizeof(T) == 2)
+    if (nt == 256) return run(std::integral_constant<int, 256>{});
   if (nt == 128) return run(std::integral_constant<int, 128>{});
   return run(std::integral_constant<int, 64>{});
 }
@@ -229,23 +236,22 @@ int gated_bwd(int64_t rows, int d, int f, const T* x, const T* wg, const T* wu, 
   gemm::Params q{};
   q.N = d;
   q.fp = p.fp;
-  q.nterms = p.comps == 3 ? 6 : 1;
   if (dx) {
     q.M = rows;
-    q.kblocks = 2 * p.fp / gemm::BK;
+    q.kblocks = 2 * p.fp / gemm::kBK<T>;
     q.splits = 1;
     q.out = dx;
-    q.vec = vec_bytes<T>(d, dx);
-    rc = single<T, gemm::kDx>(q, d, dgu, 2 * p.fp, rows, 2 * p.fp, gemm::BM, o.wg, o.wu, f, p.dp, p.comps, st);
+    q.wide = wide_rows<T>(d, dx);
+    rc = single<T, gemm::kDx>(q, d, dgu, 2 * p.fp, rows, 2 * p.fp, o.wg, o.wu, f, p.dp, p.comps, st);
     if (rc) return rc;
   }
   if (dwg) {
     q.M = 2 * p.fp;
-    q.kblocks = (int)((rows + gemm::BK - 1) / gemm::BK);
+    q.kblocks = (int)((rows + gemm::kBK<T> - 1) / gemm::kBK<T>);
     q.splits = p.splits;
     q.out = part;
-    q.vec = vec_bytes<float>(d, part);
-    rc = single<T, gemm::kDw>(q, d, dgu, 2 * p.fp, rows, 2 * p.fp, 64, o.x, o.x, rows, p.dp, p.comps, st);
+    q.wide = wide_rows<float>(d, part);
+    rc = single<T, gemm::kDw>(q, d, dgu, 2 * p.fp, rows, 2 * p.fp, o.x, o.x, rows, p.dp, p.comps, st);
     if (rc) return rc;
     const int64_t blocks = std::min<int64_t>(((int64_t)2 * f * d + 255) / 256, 16 * (int64_t)sm_count());
     dw_sum_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(part, dwg, dwu, f, p.fp, d, p.splits);

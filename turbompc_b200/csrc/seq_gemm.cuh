@@ -1,12 +1,14 @@
 // Matrix products of the gated linear layer on the tensor cores (tcgen05):
-// one persistent kernel, out = sum over terms of A_term B_term with an epilogue
-// chosen at compile time.
+// one persistent kernel, out = A B with an epilogue chosen at compile time.
 //
-// Operands are bfloat16 arrays [component][outer][inner] read by TMA in 128-byte
+// Operands are bfloat16 arrays [component][outer][inner] read by TMA in
 // swizzled boxes.  bfloat16 tensors have one component.  A float tensor is held
 // as three, x = c0 + c1 + c2 exactly (8 mantissa bits each, by truncation), and
-// a float product is the sum of the six component products above 2^-24:
-// (0,0) (0,1) (1,0) (1,1) (0,2) (2,0); the accumulator is float in both cases.
+// a float product is the sum of the six component products above 2^-24, the
+// smallest first.  The tensor cores' accumulation does not round to nearest:
+// over one accumulator a float product of 128 terms came out 4.4e-6 off.  So for
+// float every 64 terms get an accumulator of their own, which the epilogue
+// warps add up in registers.
 //
 // A block computes 128 x NT tiles: warp 0 feeds a ring of stages by TMA, warp 1
 // issues the products (M 128, N NT, K 16 each) into one of two TMEM
@@ -25,7 +27,10 @@ namespace tmpc {
 namespace seq {
 namespace gemm {
 
-constexpr int BM = 128, BK = 64;
+constexpr int BM = 128;
+// K elements per stage: 128-byte rows for bfloat16; 64-byte rows of three components for float.
+template <typename T>
+constexpr int kBK = sizeof(T) == 2 ? 64 : 32;
 constexpr int kThreads = 384;
 constexpr int kEpiWarps = 8;
 constexpr int kSmemTotal = 227 * 1024;
@@ -38,31 +43,28 @@ enum Mode {
 };
 
 struct Maps {
-  CUtensorMap a, b0, b1;
+  CUtensorMap a, b0, b1, c;  // c (kDact): dg | du, stored
 };
 
 struct Params {
   int64_t M;        // output rows: tokens (kAct, kDact, kDx) or columns of dg | du (kDw)
   int N;            // output columns (kAct, kDact: f)
   int fp;           // columns of dg (and du) in dg | du, a multiple of 64
-  int kblocks;      // 64-wide blocks of the reduction axis
-  int nterms;       // 1 (bfloat16) or 6 (float)
+  int kblocks;      // blocks of the reduction axis
   int splits;       // kDw: parts of the reduction axis
   int mtiles, ntiles;
   int64_t tiles;
-  int act;
-  int vec;          // bytes per store of out (and load of dh): 16, 4 or 2
+  bool wide;        // rows of out (and dh) are multiples of 16 bytes at 16-byte addresses
   void* out;        // kAct, kDx: T [M][N]; kDw: float [splits][M][N]
-  bf16* dgu;        // kDact: [components][M][2 fp]
   const void* dh;   // kDact: T [M][N]
   uint32_t polls;
 };
 
 // act(g) and act'(g).  FAST: the hardware exponential and reciprocal, whose
 // errors of a few 2^-22 vanish in bfloat16 results.
-template <bool FAST>
-__device__ __forceinline__ void activation(int act, float g, float& a, float& da) {
-  if (act == TMPC_ACT_SILU) {
+template <int ACT, bool FAST>
+__device__ __forceinline__ void activation(float g, float& a, float& da) {
+  if constexpr (ACT == TMPC_ACT_SILU) {
     const float e = FAST ? __expf(-g) : expf(-g);  // inf for g < -88: s = 0
     const float s = FAST ? __fdividef(1.f, 1.f + fminf(e, 1e30f)) : 1.f / (1.f + e);
     a = g * s;
@@ -73,10 +75,6 @@ __device__ __forceinline__ void activation(int act, float g, float& a, float& da
     da = c + g * 0.39894228040143268f * (FAST ? __expf(-0.5f * g * g) : expf(-0.5f * g * g));
   }
 }
-
-// Component pairs of a float product, largest first.
-__device__ __forceinline__ int term_a(int t) { return t == 2 ? 1 : t == 3 ? 1 : t == 5 ? 2 : 0; }
-__device__ __forceinline__ int term_b(int t) { return t == 1 ? 1 : t == 3 ? 1 : t == 4 ? 2 : 0; }
 
 __device__ __forceinline__ void split3(float x, bf16 (&c)[3]) {
   // Truncation to the top 16 bits is exact to subtract and cannot overflow; a
@@ -101,13 +99,21 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
-// Shared-memory descriptor, 128-byte swizzle.  K-major: rows of 128 bytes (64 K
-// elements), groups of 8 rows 1024 bytes apart.  MN-major: each 64-wide box of
-// the M / N axis holds one 128-byte row per K; boxes lie 64 rows (8192 bytes)
-// apart, groups of 8 K rows 1024 bytes.
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int x, int y, int z, const void* src) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x),
+               "r"(y), "r"(z), "r"(smem_u32(src))
+               : "memory");
+}
+
+// Shared-memory descriptor.  K-major: rows of BK elements (BK = 64: 128-byte
+// swizzle, 32: 64-byte swizzle), groups of 8 rows adjacent.  MN-major: each
+// 64-wide box of the M / N axis holds one 128-byte row per K (128-byte
+// swizzle); boxes lie BK rows apart, groups of 8 K rows 1024 bytes.
+template <int BK>
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, bool mn_major) {
-  const uint64_t lbo = mn_major ? 8192 >> 4 : 1, sbo = 1024 >> 4;
-  return (uint64_t)((addr & 0x3ffff) >> 4) | lbo << 16 | sbo << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+  const uint64_t lbo = mn_major ? BK * 128 >> 4 : 1, sbo = (mn_major ? 1024 : 8 * BK * 2) >> 4;
+  const uint64_t swizzle = mn_major || BK == 64 ? 2 : 4;
+  return (uint64_t)((addr & 0x3ffff) >> 4) | lbo << 16 | sbo << 32 | (uint64_t)1 << 46 | swizzle << 61;
 }
 
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
@@ -155,78 +161,120 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, uint32_t po
   return false;
 }
 
-// A warp's 32 x CW chunk between its staging rows (one per lane) and global
-// memory, coalesced along the rows.
-template <typename E, int CW>
-struct Chunk {
-  static constexpr int kPitch = CW * (int)sizeof(E) + 16;  // 16-byte accesses of 8 rows fall into different banks
-  static __device__ __forceinline__ void put(char* stg, int lane, const E (&v)[CW]) {
-    constexpr int PER = 16 / sizeof(E);
+// A warp's chunk of an output (or of dh): 32 rows, one per lane, of CH elements,
+// in staging rows of kPitch bytes.  Rows of 2-byte elements may start at any
+// even address; a staging row then holds the row's aligned 4-byte words, i.e.
+// its elements shifted up by one place where the row starts odd.
+constexpr int kPitch = 144;  // 16-byte accesses of 8 rows fall into different banks
+
+template <typename E>
+__device__ __forceinline__ int odd_row(const E* row) {
+  return sizeof(E) == 2 ? (int)(reinterpret_cast<uintptr_t>(row) >> 1) & 1 : 0;
+}
+
+// Staging rows -> global rows, coalesced.  g: the chunk's first element.
+template <typename E, int CH>
+__device__ __forceinline__ void chunk_store(char* stg, int lane, E* g, int64_t pitch, int rows, int cols, bool wide) {
+  constexpr int W = CH * (int)sizeof(E) / 4;  // words of a row
+  __syncwarp();
+  if (wide) {
+    constexpr int U = W / 4, PER = 16 / sizeof(E);
+    const int u = lane % U;
 #pragma unroll
-    for (int i = 0; i < CW / PER; ++i) {
-      Pack<E, PER> p;
-#pragma unroll
-      for (int e = 0; e < PER; ++e) p.v[e] = v[i * PER + e];
-      *reinterpret_cast<Pack<E, PER>*>(stg + lane * kPitch + i * 16) = p;
-    }
-  }
-  static __device__ __forceinline__ void get(const char* stg, int lane, E (&v)[CW]) {
-    constexpr int PER = 16 / sizeof(E);
-#pragma unroll
-    for (int i = 0; i < CW / PER; ++i) {
-      const Pack<E, PER> p = *reinterpret_cast<const Pack<E, PER>*>(stg + lane * kPitch + i * 16);
-#pragma unroll
-      for (int e = 0; e < PER; ++e) v[i * PER + e] = p.v[e];
-    }
-  }
-  template <typename U, bool STORE>
-  static __device__ __forceinline__ void move(char* stg, int lane, E* g, int64_t pitch, int rows, int cols) {
-    constexpr int PER = sizeof(U) / sizeof(E), UPR = CW / PER;  // units per row
-    static_assert(UPR <= 32 && 32 % UPR == 0, "");
-    const int u = lane % UPR;
+    for (int r = lane / U; r < 32; r += 32 / U)
+      if (r < rows && u * PER < cols)
+        *reinterpret_cast<uint4*>(g + r * pitch + u * PER) = *reinterpret_cast<uint4*>(stg + r * kPitch + u * 16);
+  } else {
+    const int w = lane % W;
 #pragma unroll 8
-    for (int r = lane / UPR; r < 32; r += 32 / UPR) {
-      if (r < rows && u * PER < cols) {
-        U* gp = reinterpret_cast<U*>(g + r * pitch + u * PER);
-        U* sp = reinterpret_cast<U*>(stg + r * kPitch + u * sizeof(U));
-        if (STORE) *gp = *sp;
-        else *sp = *gp;
+    for (int r = lane / W; r < 32; r += 32 / W) {
+      E* row = g + r * pitch;
+      if constexpr (sizeof(E) == 4) {
+        if (r < rows && w < cols) row[w] = *reinterpret_cast<E*>(stg + r * kPitch + w * 4);
+      } else {
+        const int odd = odd_row(row);
+        if (r < rows && w >= odd && 2 * w + 1 - odd < cols)
+          *reinterpret_cast<uint32_t*>(row + 2 * w - odd) = *reinterpret_cast<uint32_t*>(stg + r * kPitch + w * 4);
+      }
+    }
+    if constexpr (sizeof(E) == 2) {  // the elements that share a word with a neighbour: one lane per row
+      E* row = g + lane * pitch;
+      const int odd = odd_row(row), n = cols < CH ? cols : CH;
+      const E* s = reinterpret_cast<const E*>(stg + lane * kPitch);
+      if (lane < rows && n > 0) {
+        if (odd) row[0] = s[1];
+        if ((n + odd) & 1) row[n - 1] = s[n - 1 + odd];
       }
     }
   }
-  template <bool STORE>
-  static __device__ __forceinline__ void move(char* stg, int lane, E* g, int64_t pitch, int rows, int cols, int vec) {
-    __syncwarp();
-    if (vec == 16) {
-      move<uint4, STORE>(stg, lane, g, pitch, rows, cols);
-    } else if constexpr (sizeof(E) == 4) {
-      move<uint32_t, STORE>(stg, lane, g, pitch, rows, cols);
-    } else {
-      if (vec == 4) move<uint32_t, STORE>(stg, lane, g, pitch, rows, cols);
-      else move<uint16_t, STORE>(stg, lane, g, pitch, rows, cols);
-    }
-    __syncwarp();
-  }
-  // E values, one row per lane, to g[row][col].
-  static __device__ __forceinline__ void store(char* stg, int lane, const E (&v)[CW], E* g, int64_t pitch, int rows,
-                                               int cols, int vec) {
-    put(stg, lane, v);
-    move<true>(stg, lane, g, pitch, rows, cols, vec);
-  }
-  static __device__ __forceinline__ void load(char* stg, int lane, E (&v)[CW], const E* g, int64_t pitch, int rows,
-                                              int cols, int vec) {
-    move<false>(stg, lane, const_cast<E*>(g), pitch, rows, cols, vec);
-    get(stg, lane, v);
-    __syncwarp();
-  }
-};
-
-template <int NT>
-constexpr int stages() {
-  constexpr int per = (BM + NT) * BK * 2;
-  constexpr int n = (kSmemTotal - 1024 - 1024 - kEpiWarps * 32 * 80) / per;
-  return n > 8 ? 8 : n;
+  __syncwarp();
 }
+
+// The other way, asynchronously (cp.async); the element past a row's last whole
+// word is returned and put in place by chunk_land.
+template <typename E, int CH>
+__device__ __forceinline__ E chunk_fetch(char* stg, int lane, const E* g, int64_t pitch, int rows, int cols, bool wide) {
+  constexpr int W = CH * (int)sizeof(E) / 4;
+  E tail{};
+  if (wide) {
+    constexpr int U = W / 4, PER = 16 / sizeof(E);
+    const int u = lane % U;
+#pragma unroll
+    for (int r = lane / U; r < 32; r += 32 / U)
+      if (r < rows && u * PER < cols)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(stg + r * kPitch + u * 16)),
+                     "l"(g + r * pitch + u * PER)
+                     : "memory");
+  } else {
+    const int w = lane % W;
+#pragma unroll 8
+    for (int r = lane / W; r < 32; r += 32 / W) {
+      const E* row = g + r * pitch;
+      const int odd = odd_row(row);
+      const bool on = r < rows && (sizeof(E) == 4 ? w < cols : 2 * w + 1 - odd < cols);
+      if (on)  // an odd row's first word begins with the element before it, which exists
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(stg + r * kPitch + w * 4)),
+                     "l"(reinterpret_cast<const char*>(row) + w * 4 - 2 * odd)
+                     : "memory");
+    }
+    if constexpr (sizeof(E) == 2) {
+      const E* row = g + lane * pitch;
+      const int odd = odd_row(row), n = cols < CH ? cols : CH;
+      if (lane < rows && n > 0 && ((n + odd) & 1)) tail = row[n - 1];
+    }
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  return tail;
+}
+
+template <typename E, int CH>
+__device__ __forceinline__ void chunk_land(char* stg, int lane, E tail, const E* row, int rows, int cols, bool wide) {
+  if constexpr (sizeof(E) == 2) {
+    const int odd = odd_row(row), n = cols < CH ? cols : CH;
+    if (!wide && lane < rows && n > 0 && ((n + odd) & 1)) reinterpret_cast<E*>(stg + lane * kPitch)[n - 1 + odd] = tail;
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncwarp();
+}
+
+template <typename T, int MODE, int NT>
+struct Config {
+  static constexpr bool kFloat = sizeof(T) == 4;
+  static constexpr int BK = kBK<T>, NC = kFloat ? 3 : 1;
+  static constexpr int kA = BM * BK * 2, kB = NT * BK * 2;  // one component
+  static constexpr int kStage = NC * (kA + kB);
+  static constexpr bool kDual = MODE == kAct || MODE == kDact;
+  static constexpr int kCols = (kDual ? NT / 2 : NT) / 2;   // columns (of each projection) of an epilogue warp
+  static constexpr bool kOutFloat = kFloat || MODE == kDw;
+  static constexpr int CH = kCols < (kOutFloat ? 32 : 64) ? kCols : (kOutFloat ? 32 : 64);
+  static constexpr int kStoreBytes = MODE == kDact ? 4096 : 0;            // TMA store of dg, du
+  static constexpr int kPad = 32 * kPitch;                                // staging of out or dh
+  static constexpr int kEpi = kEpiWarps * (kStoreBytes + kPad);
+  static constexpr int kFit = (kSmemTotal - 2048 - kEpi) / kStage;
+  static constexpr int ST = kFit > 8 ? 8 : kFit;
+  static constexpr int kSeg = kFloat ? 2 : 1 << 30;         // blocks of K per accumulator
+  static_assert(ST >= 2, "");
+};
 
 struct Barriers {
   uint64_t full[8], empty[8], acc_full[2], acc_empty[2], done;
@@ -234,20 +282,17 @@ struct Barriers {
   int abort_flag;
 };
 
-template <typename T, int MODE, int NT>
+template <typename T, int MODE, int NT, int ACT>
 __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Maps maps, const Params p) {
-  constexpr int ST = stages<NT>();
-  constexpr int kA = BM * BK * 2, kB = NT * BK * 2;
-  constexpr bool kAmn = MODE == kDw, kBmn = MODE == kDx || MODE == kDw;
-  constexpr bool kDual = MODE == kAct || MODE == kDact;
+  using F = Config<T, MODE, NT>;
+  constexpr int ST = F::ST, BK = F::BK, NC = F::NC, kA = F::kA, kB = F::kB, CH = F::CH;
+  constexpr bool kAmn = MODE == kDw, kBmn = MODE == kDx || MODE == kDw, kDual = F::kDual, kFloat = F::kFloat;
   constexpr uint32_t kIdesc = 1u << 4 | 1u << 7 | 1u << 10 | (kAmn ? 1u << 15 : 0u) | (kBmn ? 1u << 16 : 0u) |
                               (uint32_t)(NT / 8) << 17 | (uint32_t)(BM / 16) << 24;
   extern __shared__ char raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  char* sA = smem;
-  char* sB = smem + ST * kA;
-  char* stage_mem = sB + ST * kB;
-  Barriers& bar = *reinterpret_cast<Barriers*>(stage_mem + kEpiWarps * 32 * 80);
+  char* epi_mem = smem + ST * F::kStage;
+  Barriers& bar = *reinterpret_cast<Barriers*>(epi_mem + F::kEpi);
   volatile int* abort_flag = &bar.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -288,28 +333,28 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
     bool ok = true;
     for (int64_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x) {
       tile_of(t, m0, n0, kb0, kb1, split);
-      for (int term = 0; ok && term < p.nterms; ++term) {
-        const int ca = term_a(term), cb = term_b(term);
-        for (int kb = kb0; kb < kb1; ++kb, ++n) {
-          const int s = n % ST;
-          if (n >= ST && !(ok = wait(&bar.empty[s], (n / ST - 1) & 1, p.polls, abort_flag))) break;
-          uint64_t* full = &bar.full[s];
-          mbar_expect_tx(full, kA + kB);
-          char *a = sA + s * kA, *b = sB + s * kB;
+      for (int kb = kb0; kb < kb1; ++kb, ++n) {
+        const int s = n % ST;
+        if (n >= ST && !(ok = wait(&bar.empty[s], (n / ST - 1) & 1, p.polls, abort_flag))) break;
+        uint64_t* full = &bar.full[s];
+        mbar_expect_tx(full, F::kStage);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          char *a = smem + s * F::kStage + c * kA, *b = smem + s * F::kStage + NC * kA + c * kB;
           if (kAmn) {
-            tma_load_3d(a, &maps.a, (int)m0, kb * BK, ca, full);
-            tma_load_3d(a + 8192, &maps.a, (int)m0 + 64, kb * BK, ca, full);
+            tma_load_3d(a, &maps.a, (int)m0, kb * BK, c, full);
+            tma_load_3d(a + BK * 128, &maps.a, (int)m0 + 64, kb * BK, c, full);
           } else {
-            tma_load_3d(a, &maps.a, kb * BK, (int)m0, ca, full);
+            tma_load_3d(a, &maps.a, kb * BK, (int)m0, c, full);
           }
           if (kDual) {
-            tma_load_3d(b, &maps.b0, kb * BK, n0, cb, full);
-            tma_load_3d(b + kB / 2, &maps.b1, kb * BK, n0, cb, full);
+            tma_load_3d(b, &maps.b0, kb * BK, n0, c, full);
+            tma_load_3d(b + kB / 2, &maps.b1, kb * BK, n0, c, full);
           } else {
             const bool up = MODE == kDx && kb >= p.fp / BK;
             const int k = (up ? kb - p.fp / BK : kb) * BK;
             for (int j = 0; j < NT / 64; ++j)
-              tma_load_3d(b + j * 8192, up ? &maps.b1 : &maps.b0, n0 + j * 64, k, cb, full);
+              tma_load_3d(b + j * BK * 128, up ? &maps.b1 : &maps.b0, n0 + j * 64, k, c, full);
           }
         }
       }
@@ -320,120 +365,254 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
   } else if (warp == 1 && lane == 0) {  // products
     int64_t m0;
     int n0, kb0, kb1, split;
-    uint32_t n = 0, done_tiles = 0;
+    uint32_t n = 0, accs = 0;
     bool ok = true;
-    for (int64_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x, ++done_tiles) {
+    for (int64_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x) {
       tile_of(t, m0, n0, kb0, kb1, split);
-      const uint32_t buf = done_tiles & 1, d = tmem + buf * NT;
-      if (done_tiles >= 2 && !(ok = wait(&bar.acc_empty[buf], (done_tiles / 2 - 1) & 1, p.polls, abort_flag))) break;
-      fence_after();
-      const int iters = (kb1 - kb0) * p.nterms;
-      for (int it = 0; it < iters; ++it, ++n) {
-        const int s = n % ST;
-        if (!(ok = wait(&bar.full[s], (n / ST) & 1, p.polls, abort_flag))) break;
+      for (int seg = kb0; ok && seg < kb1; seg = kb1 - seg > F::kSeg ? seg + F::kSeg : kb1, ++accs) {
+        const int end = kb1 - seg > F::kSeg ? seg + F::kSeg : kb1;
+        const uint32_t buf = accs & 1, d = tmem + buf * NT;
+        if (accs >= 2 && !(ok = wait(&bar.acc_empty[buf], (accs / 2 - 1) & 1, p.polls, abort_flag))) break;
         fence_after();
-        const uint64_t da = smem_desc(smem_u32(sA + s * kA), kAmn), db = smem_desc(smem_u32(sB + s * kB), kBmn);
+        for (int kb = seg; kb < end; ++kb, ++n) {
+          const int s = n % ST;
+          if (!(ok = wait(&bar.full[s], (n / ST) & 1, p.polls, abort_flag))) break;
+          fence_after();
+          const uint32_t a = smem_u32(smem + s * F::kStage), b = a + NC * kA;
 #pragma unroll
-        for (int k = 0; k < BK / 16; ++k)  // 16 K elements: 32 bytes of a K-major row, 16 rows of an MN-major box
-          mma_f16(d, da + k * ((kAmn ? 2048 : 32) >> 4), db + k * ((kBmn ? 2048 : 32) >> 4), kIdesc, it > 0 || k > 0);
-        mma_commit(&bar.empty[s]);
+          for (int term = kFloat ? 0 : 5; term < 6; ++term) {  // (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
+            const int ca = term == 1 ? 2 : term == 2 || term == 4 ? 1 : 0;
+            const int cb = term == 0 ? 2 : term == 2 || term == 3 ? 1 : 0;
+            const uint64_t da = smem_desc<BK>(a + ca * kA, kAmn), db = smem_desc<BK>(b + cb * kB, kBmn);
+#pragma unroll
+            for (int k = 0; k < BK / 16; ++k)  // 16 K elements: 32 bytes of a K-major row, 16 rows of an MN-major box
+              mma_f16(d, da + k * ((kAmn ? 2048 : 32) >> 4), db + k * ((kBmn ? 2048 : 32) >> 4), kIdesc,
+                      kb > seg || term > (kFloat ? 0 : 5) || k > 0);
+          }
+          mma_commit(&bar.empty[s]);
+        }
+        if (ok) mma_commit(&bar.acc_full[buf]);
       }
-      if (ok) mma_commit(&bar.acc_full[buf]);
     }
     if (!ok) {  // TMEM may be freed only after the products in flight
       mma_commit(&bar.done);
       mbar_wait_bounded(&bar.done, 0, kTransferDrainPolls);
     }
   } else if (warp >= 4) {  // epilogue: lanes 32 (warp % 4) .. + 31, half of the columns each
-    constexpr int kCols = (kDual ? NT / 2 : NT) / 2;
-    constexpr int CW = kCols < 32 || sizeof(T) == 4 || MODE == kDw ? 16 : 32;
+    constexpr int kCols = F::kCols;
+    using E = typename std::conditional<F::kOutFloat, float, bf16>::type;
+    constexpr int RC = kFloat ? kCols : 16;  // accumulator columns held in registers
     const int quad = warp & 3, half = (warp - 4) >> 2;
-    char* stg = stage_mem + (warp - 4) * 32 * 80;
+    char* tst = epi_mem + (warp - 4) * F::kStoreBytes;
+    char* stg = epi_mem + kEpiWarps * F::kStoreBytes + (warp - 4) * F::kPad;
     int64_t m0;
     int n0, kb0, kb1, split;
-    uint32_t done_tiles = 0;
+    uint32_t accs = 0;
     bool ok = true;
     const float nan = __int_as_float(0x7fffffff);
-    for (int64_t t = blockIdx.x; t < p.tiles; t += gridDim.x, ++done_tiles) {
+    for (int64_t t = blockIdx.x; t < p.tiles; t += gridDim.x) {
       tile_of(t, m0, n0, kb0, kb1, split);
-      const uint32_t buf = done_tiles & 1;
-      if (ok) ok = wait(&bar.acc_full[buf], (done_tiles / 2) & 1, p.polls, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      fence_after();
-      const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + buf * NT + half * kCols;
       const int64_t row0 = m0 + quad * 32;
       const int rows = (int)(p.M - row0 < 32 ? p.M - row0 : 32);
-#pragma unroll 1
-      for (int c = 0; c < kCols; c += CW) {
-        const int col0 = n0 + half * kCols + c, cols = p.N - col0;
-        float v[CW], w[kDual ? CW : 1];
-        if (ok) {
+      const int colw = n0 + half * kCols;
+      T tail{};
+      const T* dh = nullptr;
+      if constexpr (MODE == kDact) {  // on its way while the products run
+        dh = static_cast<const T*>(p.dh) + row0 * p.N + colw;
+        tail = chunk_fetch<T, CH>(stg, lane, dh, p.N, rows, p.N - colw, p.wide);
+      }
+      float v[RC], w[kDual ? RC : 1];
+      uint32_t acc = 0;
+      if constexpr (kFloat) {
 #pragma unroll
-          for (int i = 0; i < CW; i += 16) {
-            tmem_ld16(acc + c + i, *reinterpret_cast<float(*)[16]>(&v[i]));
-            if constexpr (kDual) tmem_ld16(acc + NT / 2 + c + i, *reinterpret_cast<float(*)[16]>(&w[i]));
-          }
-          tmem_wait_ld();
-        } else {
-#pragma unroll
-          for (int i = 0; i < CW; ++i) {
-            v[i] = nan;
-            if constexpr (kDual) w[i] = nan;
-          }
-        }
-        constexpr bool kFast = sizeof(T) == 2;
-        if constexpr (MODE == kAct) {
-          T h[CW];
-#pragma unroll
-          for (int i = 0; i < CW; ++i) {
-            float a, da;
-            activation<kFast>(p.act, v[i], a, da);
-            h[i] = from_f<T>(a * w[i]);
-          }
-          Chunk<T, CW>::store(stg, lane, h, static_cast<T*>(p.out) + row0 * p.N + col0, p.N, rows, cols, p.vec);
-        } else if constexpr (MODE == kDact) {
-          T y[CW];
-          Chunk<T, CW>::load(stg, lane, y, static_cast<const T*>(p.dh) + row0 * p.N + col0, p.N, rows, cols, p.vec);
-          constexpr int NC = sizeof(T) == 4 ? 3 : 1;
-          bf16 g[NC][CW], u[NC][CW];
-#pragma unroll
-          for (int i = 0; i < CW; ++i) {
-            float a, da;
-            activation<kFast>(p.act, v[i], a, da);
-            const float dy = to_f(y[i]);
-            // columns f .. fp - 1 meet rows of zeros in the next products: they must not be NaN
-            const float dg = i < cols ? dy * w[i] * da : 0.f, du = i < cols ? dy * a : 0.f;
-            if constexpr (NC == 1) {
-              g[0][i] = from_f<bf16>(dg);
-              u[0][i] = from_f<bf16>(du);
-            } else {
-              bf16 s[3];
-              split3(dg, s);
-              g[0][i] = s[0], g[1][i] = s[1], g[2][i] = s[2];
-              split3(du, s);
-              u[0][i] = s[0], u[1][i] = s[1], u[2][i] = s[2];
-            }
-          }
-          const int64_t pitch = 2 * (int64_t)p.fp;
-          bf16* o = p.dgu + row0 * pitch + col0;
-#pragma unroll
-          for (int k = 0; k < NC; ++k) {
-            Chunk<bf16, CW>::store(stg, lane, g[k], o + k * p.M * pitch, pitch, rows, p.fp - col0, 16);
-            Chunk<bf16, CW>::store(stg, lane, u[k], o + k * p.M * pitch + p.fp, pitch, rows, p.fp - col0, 16);
-          }
-        } else if constexpr (MODE == kDx) {
-          T o[CW];
-#pragma unroll
-          for (int i = 0; i < CW; ++i) o[i] = from_f<T>(v[i]);
-          Chunk<T, CW>::store(stg, lane, o, static_cast<T*>(p.out) + row0 * p.N + col0, p.N, rows, cols, p.vec);
-        } else {
-          Chunk<float, CW>::store(stg, lane, v, static_cast<float*>(p.out) + (split * p.M + row0) * p.N + col0, p.N,
-                                  rows, cols, p.vec);
+        for (int i = 0; i < RC; ++i) {
+          v[i] = 0.f;
+          if constexpr (kDual) w[i] = 0.f;
         }
       }
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.acc_empty[buf]);
+      for (int seg = kb0; seg < kb1; seg = kb1 - seg > F::kSeg ? seg + F::kSeg : kb1, ++accs) {
+        const uint32_t buf = accs & 1;
+        if (ok) ok = wait(&bar.acc_full[buf], (accs / 2) & 1, p.polls, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        fence_after();
+        acc = tmem + ((uint32_t)(quad * 32) << 16) + buf * NT + half * kCols;
+        if constexpr (kFloat) {
+          if (ok) {
+#pragma unroll
+            for (int c = 0; c < kCols; c += 16) {
+              float x[16], y[16];
+              tmem_ld16(acc + c, x);
+              if constexpr (kDual) tmem_ld16(acc + NT / 2 + c, y);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                v[c + i] += x[i];
+                if constexpr (kDual) w[c + i] += y[i];
+              }
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < RC; ++i) {
+              v[i] = nan;
+              if constexpr (kDual) w[i] = nan;
+            }
+          }
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar.acc_empty[buf]);
+        }
+      }
+      if constexpr (MODE == kDact) chunk_land<T, CH>(stg, lane, tail, dh + (int64_t)lane * p.N, rows, p.N - colw, p.wide);
+      uint32_t gw[MODE == kDact && !kFloat ? kCols / 2 : 1], uw[MODE == kDact && !kFloat ? kCols / 2 : 1];
+#pragma unroll
+      for (int c0 = 0; c0 < kCols; c0 += CH) {
+        E* out = nullptr;
+        int odd = 0;
+        uint32_t carry = 0;
+        if constexpr (MODE != kDact) {
+          out = static_cast<E*>(p.out) + ((MODE == kDw ? split * p.M : 0) + row0) * p.N + colw + c0;
+          odd = odd_row(out + (int64_t)lane * p.N);
+        } else {
+          odd = odd_row(dh + (int64_t)lane * p.N);
+        }
+#pragma unroll
+        for (int c = 0; c < CH; c += 16) {
+          float(&vv)[16] = *reinterpret_cast<float(*)[16]>(&v[kFloat ? c0 + c : 0]);
+          float(&ww)[16] = *reinterpret_cast<float(*)[16]>(&w[kFloat && kDual ? c0 + c : 0]);
+          if constexpr (!kFloat) {
+            if (ok) {
+              tmem_ld16(acc + c0 + c, vv);
+              if constexpr (kDual) tmem_ld16(acc + NT / 2 + c0 + c, ww);
+              tmem_wait_ld();
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                vv[i] = nan;
+                if constexpr (kDual) ww[i] = nan;
+              }
+            }
+          }
+          if constexpr (kDual && MODE == kAct) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float a, da;
+              activation<ACT, !kFloat>(vv[i], a, da);
+              vv[i] = a * ww[i];
+            }
+          }
+          if constexpr (MODE != kDact) {
+            char* s = stg + lane * kPitch + c * sizeof(E);
+            if constexpr (F::kOutFloat) {
+#pragma unroll
+              for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<float4*>(s + i * 4) = make_float4(vv[i], vv[i + 1], vv[i + 2], vv[i + 3]);
+            } else {
+              uint32_t x[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const __nv_bfloat162 b2 = __floats2bfloat162_rn(vv[2 * i], vv[2 * i + 1]);
+                const uint32_t pr = *reinterpret_cast<const uint32_t*>(&b2);
+                x[i] = __funnelshift_l(carry, pr, odd * 16);
+                carry = pr;
+              }
+              *reinterpret_cast<uint4*>(s) = make_uint4(x[0], x[1], x[2], x[3]);
+              *reinterpret_cast<uint4*>(s + 16) = make_uint4(x[4], x[5], x[6], x[7]);
+            }
+          } else {  // dg, du in place of g, u
+            float y[16];
+            const char* s = stg + lane * kPitch + c * sizeof(T);
+            if constexpr (kFloat) {
+#pragma unroll
+              for (int i = 0; i < 16; i += 4) {
+                const float4 q = *reinterpret_cast<const float4*>(s + i * 4);
+                y[i] = q.x, y[i + 1] = q.y, y[i + 2] = q.z, y[i + 3] = q.w;
+              }
+            } else {
+              const uint4 q0 = *reinterpret_cast<const uint4*>(s), q1 = *reinterpret_cast<const uint4*>(s + 16);
+              const uint32_t x[9] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w,
+                                     *reinterpret_cast<const uint32_t*>(s + 32)};
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const uint32_t pr = __funnelshift_r(x[i], x[i + 1], odd * 16);
+                y[2 * i] = __uint_as_float(pr << 16);
+                y[2 * i + 1] = __uint_as_float(pr & 0xffff0000u);
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float a, da;
+              activation<ACT, !kFloat>(vv[i], a, da);
+              // columns f .. fp - 1 meet rows of zeros in the next products: they must not be NaN
+              const bool on = colw + c0 + c + i < p.N;
+              vv[i] = on ? y[i] * ww[i] * da : 0.f;
+              ww[i] = on ? y[i] * a : 0.f;
+            }
+            if constexpr (!kFloat) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const __nv_bfloat162 g2 = __floats2bfloat162_rn(vv[2 * i], vv[2 * i + 1]);
+                const __nv_bfloat162 u2 = __floats2bfloat162_rn(ww[2 * i], ww[2 * i + 1]);
+                gw[(c0 + c) / 2 + i] = *reinterpret_cast<const uint32_t*>(&g2);
+                uw[(c0 + c) / 2 + i] = *reinterpret_cast<const uint32_t*>(&u2);
+              }
+            }
+          }
+        }
+        if constexpr (!F::kOutFloat && MODE != kDact)  // an odd row's last element opens one more word
+          *reinterpret_cast<uint32_t*>(stg + lane * kPitch + CH * 2) = carry >> 16;
+        if constexpr (MODE != kDact) chunk_store<E, CH>(stg, lane, out, p.N, rows, p.N - colw - c0, p.wide);
+      }
+      if constexpr (!kFloat) {
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.acc_empty[(accs - 1) & 1]);
+      }
+      if constexpr (MODE == kDact) {
+        // Through the swizzled staging box to dg | du: 16-byte units of a row of
+        // kCols elements, permuted as the map's swizzle does.
+        constexpr int kRow = kCols * 2, U = kRow / 16;
+        const int sw = kRow == 128 ? lane & 7 : kRow == 64 ? (lane >> 1) & 3 : (lane >> 2) & 1;
+        auto box_store = [&](const uint32_t* words, int col, int comp) {
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          __syncwarp();
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            *reinterpret_cast<uint4*>(tst + lane * kRow + ((u ^ sw) * 16)) =
+                make_uint4(words[4 * u], words[4 * u + 1], words[4 * u + 2], words[4 * u + 3]);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0 && rows > 0 && colw < p.fp) {
+            tma_store_3d(&maps.c, col, (int)row0, comp, tst);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        };
+        if constexpr (!kFloat) {
+          box_store(gw, colw, 0);
+          box_store(uw, p.fp + colw, 0);
+        } else {
+          for (int k = 0; k < 3; ++k) {
+            uint32_t x[kCols / 2];
+            auto comp = [&](float (&f)[RC]) {  // the k-th component, and the rest in its place
+#pragma unroll
+              for (int i = 0; i < kCols / 2; ++i) {
+                bf16 c0[3], c1[3];
+                split3(f[2 * i], c0);
+                split3(f[2 * i + 1], c1);
+                x[i] = (uint32_t)__bfloat16_as_ushort(c0[0]) | (uint32_t)__bfloat16_as_ushort(c1[0]) << 16;
+                f[2 * i] = __bfloat162float(c0[1]) + __bfloat162float(c0[2]);
+                f[2 * i + 1] = __bfloat162float(c1[1]) + __bfloat162float(c1[2]);
+              }
+            };
+            comp(v);
+            box_store(x, colw, k);
+            comp(w);
+            box_store(x, p.fp + colw, k);
+          }
+        }
+      }
+    }
+    if constexpr (MODE == kDact) {
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
   }
   __syncwarp();
@@ -465,29 +644,33 @@ inline EncodeFn encode_fn() {
 }
 
 // A bfloat16 array [components][outer][inner], rows of `pitch` elements (a
-// multiple of 8, 16-byte aligned base), read in boxes of 64 x box_outer.
+// multiple of 8, 16-byte aligned base), moved in boxes of box_inner (64, 32 or
+// 16) x box_outer, swizzled over the box's row.
 inline int make_map(CUtensorMap* m, const void* base, int64_t inner, int64_t outer, int comps, int64_t pitch,
-                    int box_outer) {
+                    int box_inner, int box_outer) {
   const EncodeFn fn = encode_fn();
   if (!fn) return (int)cudaErrorNotSupported;
   const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)comps};
   const cuuint64_t strides[2] = {(cuuint64_t)pitch * 2, (cuuint64_t)pitch * 2 * (cuuint64_t)outer};
-  const cuuint32_t box[3] = {64, (cuuint32_t)box_outer, 1}, es[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer, 1}, es[3] = {1, 1, 1};
+  const CUtensorMapSwizzle sw = box_inner == 64   ? CU_TENSOR_MAP_SWIZZLE_128B
+                                : box_inner == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                  : CU_TENSOR_MAP_SWIZZLE_32B;
   const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, es,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
 }
 
-template <typename T, int MODE, int NT>
+template <typename T, int MODE, int NT, int ACT>
 int launch(const Maps& maps, Params p, cudaStream_t st) {
   p.tiles = (int64_t)p.mtiles * p.ntiles * p.splits;
   p.polls = transfer_poll_limit().load();
   const cudaError_t e =
-      cudaFuncSetAttribute(kernel<T, MODE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemTotal);
+      cudaFuncSetAttribute(kernel<T, MODE, NT, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemTotal);
   if (e != cudaSuccess) return (int)e;
   const int64_t sms = sm_count();
-  kernel<T, MODE, NT><<<(unsigned)(p.tiles < sms ? p.tiles : sms), kThreads, kSmemTotal, st>>>(maps, p);
+  kernel<T, MODE, NT, ACT><<<(unsigned)(p.tiles < sms ? p.tiles : sms), kThreads, kSmemTotal, st>>>(maps, p);
   return (int)cudaPeekAtLastError();
 }
 

@@ -7,7 +7,7 @@
 // a float product is the sum of the six component products above 2^-24, the
 // smallest first.  The tensor cores' accumulation does not round to nearest:
 // over one accumulator a float product of 128 terms came out 4.4e-6 off.  So for
-// float every 64 terms get an accumulator of their own, which the epilogue
+// float every 32 terms get an accumulator of their own, which the epilogue
 // warps add up in registers.
 //
 // A block computes 128 x NT tiles: warp 0 feeds a ring of stages by TMA, warp 1
@@ -60,19 +60,31 @@ struct Params {
   uint32_t polls;
 };
 
-// act(g) and act'(g).  FAST: the hardware exponential and reciprocal, whose
-// errors of a few 2^-22 vanish in bfloat16 results.
+// The hardware's exponential and reciprocal, a few 2^-22 off, denormals flushed.
+__device__ __forceinline__ float fast_exp(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  return y;
+}
+__device__ __forceinline__ float fast_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// act(g) and act'(g).  FAST: with the functions above, whose errors vanish in
+// bfloat16 results.
 template <int ACT, bool FAST>
 __device__ __forceinline__ void activation(float g, float& a, float& da) {
   if constexpr (ACT == TMPC_ACT_SILU) {
-    const float e = FAST ? __expf(-g) : expf(-g);  // inf for g < -88: s = 0
-    const float s = FAST ? __fdividef(1.f, 1.f + fminf(e, 1e30f)) : 1.f / (1.f + e);
+    // exp(-g) is infinite for g < -88 and s = 0 then, as it is in the limit
+    const float s = FAST ? fast_rcp(1.f + fast_exp(-g)) : 1.f / (1.f + expf(-g));
     a = g * s;
     da = s * (1.f + g * (1.f - s));
   } else {
     const float c = 0.5f * erfcf(-0.70710678118654752f * g);
     a = g * c;
-    da = c + g * 0.39894228040143268f * (FAST ? __expf(-0.5f * g * g) : expf(-0.5f * g * g));
+    da = c + g * 0.39894228040143268f * (FAST ? fast_exp(-0.5f * g * g) : expf(-0.5f * g * g));
   }
 }
 
@@ -184,6 +196,21 @@ __device__ __forceinline__ void chunk_store(char* stg, int lane, E* g, int64_t p
     for (int r = lane / U; r < 32; r += 32 / U)
       if (r < rows && u * PER < cols)
         *reinterpret_cast<uint4*>(g + r * pitch + u * PER) = *reinterpret_cast<uint4*>(stg + r * kPitch + u * 16);
+  } else if (W == 32 && rows == 32 && cols >= CH) {  // a whole chunk: no bounds
+    const char* s = stg + lane * 4;
+    char* p = reinterpret_cast<char*>(g) + lane * 4;
+#pragma unroll 16
+    for (int r = 0; r < 32; ++r) {
+      const uint32_t x = *reinterpret_cast<const uint32_t*>(s + r * kPitch);
+      const int odd = odd_row(reinterpret_cast<E*>(p));
+      if (sizeof(E) == 4 || lane >= odd) *reinterpret_cast<uint32_t*>(p - 2 * odd) = x;
+      p += pitch * sizeof(E);
+    }
+    if constexpr (sizeof(E) == 2) {
+      E* row = g + lane * pitch;
+      const E* t = reinterpret_cast<const E*>(stg + lane * kPitch);
+      if (odd_row(row)) row[0] = t[1], row[CH - 1] = t[CH];
+    }
   } else {
     const int w = lane % W;
 #pragma unroll 8
@@ -225,6 +252,19 @@ __device__ __forceinline__ E chunk_fetch(char* stg, int lane, const E* g, int64_
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(stg + r * kPitch + u * 16)),
                      "l"(g + r * pitch + u * PER)
                      : "memory");
+  } else if (W == 32 && rows == 32 && cols >= CH) {
+    const uint32_t s = smem_u32(stg) + lane * 4;
+    const char* p = reinterpret_cast<const char*>(g) + lane * 4;
+#pragma unroll 16
+    for (int r = 0; r < 32; ++r) {
+      const int odd = odd_row(reinterpret_cast<const E*>(p));
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s + r * kPitch), "l"(p - 2 * odd) : "memory");
+      p += pitch * sizeof(E);
+    }
+    if constexpr (sizeof(E) == 2) {
+      const E* row = g + lane * pitch;
+      if (odd_row(row)) tail = row[CH - 1];
+    }
   } else {
     const int w = lane % W;
 #pragma unroll 8
@@ -272,7 +312,7 @@ struct Config {
   static constexpr int kEpi = kEpiWarps * (kStoreBytes + kPad);
   static constexpr int kFit = (kSmemTotal - 2048 - kEpi) / kStage;
   static constexpr int ST = kFit > 8 ? 8 : kFit;
-  static constexpr int kSeg = kFloat ? 2 : 1 << 30;         // blocks of K per accumulator
+  static constexpr int kSeg = kFloat ? 1 : 1 << 30;         // blocks of K per accumulator
   static_assert(ST >= 2, "");
 };
 

@@ -109,9 +109,9 @@ for _s in ("f32", "f64"):
     _SIGS[f"tmpc_admm_solve_{_s}"] = (C.c_int32, [C.POINTER(TmpcDims), C.POINTER(TmpcQP),
                                                   C.POINTER(TmpcAdmmState), C.POINTER(TmpcAdmmState), _P,
                                                   C.POINTER(TmpcAdmmConfig), _P, _P, _P, _P, C.c_size_t, _P])
-# Sequence operators: float and bfloat16 elements.
-_V = C.POINTER(TmpcSeqView)
-_LA = C.POINTER(TmpcLinAttnDims)
+# Sequence operators: float and bfloat16 elements.  Structures go in by address
+# (a ctypes structure's byref, or its packed bytes).
+_V = _LA = _P
 _SIGS["tmpc_linear_attention_workspace_bytes"] = (C.c_size_t, [_LA])
 _SIGS["tmpc_linear_attention_backward_workspace_bytes"] = (C.c_size_t, [_LA])
 _SIGS["tmpc_add_rms_norm_workspace_bytes"] = (C.c_size_t, [C.c_int64, C.c_int32])

@@ -87,24 +87,40 @@ struct Shape {
   static constexpr int STATE = D * LD;
 };
 
-// Tokens t0 .. t0 + n - 1 of one head into a [C][LD] tile; the rest is zero.
+// One head's rows, chunk by chunk, into [C][LD] tiles: row r of a chunk's n
+// tokens, the rest zero.  A thread keeps its column and every kRows-th row.
 template <int D>
-__device__ __forceinline__ void load_tile(bf16* s, const TmpcSeqView& w, int b, int t0, int n, int h, int d, bool vec) {
+struct Loader {
   using Z = Shape<D>;
-  const bf16* base = row_ptr<bf16>(w, b, t0, h);
-  if (vec) {
-    for (int u = threadIdx.x; u < C * D / 8; u += Z::NT) {
-      const int t = u / (D / 8), i = u % (D / 8) * 8;
-      const bool on = t < n && i < d;
-      cp16(s + t * Z::LD + i, on ? base + t * w.token + i : base, on);
-    }
-  } else {
-    for (int u = threadIdx.x; u < C * D; u += Z::NT) {
-      const int t = u / D, i = u % D;
-      s[t * Z::LD + i] = (t < n && i < d) ? base[t * w.token + i] : __float2bfloat16_rn(0.f);
+  static constexpr int UPR = D / 8, kRows = Z::NT / UPR;  // 16-byte units per row, rows per pass
+  const bf16* base;  // the chunk's first row
+  int64_t token;
+  int d;
+  bool vec;
+  __device__ __forceinline__ Loader(const TmpcSeqView& w, int b, int64_t t0, int h, int d_, bool vec_)
+      : base(row_ptr<bf16>(w, b, t0, h)), token(w.token), d(d_), vec(vec_) {}
+  __device__ __forceinline__ void advance(int tokens) { base += tokens * token; }
+  __device__ __forceinline__ void load(bf16* s, int n) const {
+    if (vec) {
+      const int i = threadIdx.x % UPR * 8, r0 = threadIdx.x / UPR;
+      const bf16* p = base + r0 * token + i;
+      const int64_t step = kRows * token;
+      s += r0 * Z::LD + i;
+      const int m = i < d ? n : 0;
+#pragma unroll
+      for (int r = 0; r < C; r += kRows) {
+        const bool on = r0 + r < m;
+        cp16(s + r * Z::LD, on ? p : base, on);
+        p += step;
+      }
+    } else {
+      for (int u = threadIdx.x; u < C * D; u += Z::NT) {
+        const int t = u / D, i = u % D;
+        s[t * Z::LD + i] = (t < n && i < d) ? base[t * token + i] : __float2bfloat16_rn(0.f);
+      }
     }
   }
-}
+};
 
 // Fragment addresses: A (rows m, K k) of a row-major [m][k] tile; A of a tile
 // stored [k][m]; B (two 8-wide column tiles) of a tile stored [n][k], of one
@@ -152,12 +168,16 @@ struct State {
   }
   // rows x cols of a float array, element (i, j) at p[i si + j sj]; zero elsewhere
   __device__ __forceinline__ void load(const float* p, int rows, int cols, int si, int sj) {
-    each([&](int i, int j, float& v) { v = (p && i < rows && j < cols) ? p[(int64_t)i * si + (int64_t)j * sj] : 0.f; });
+    if (!p) each([&](int, int, float& v) { v = 0.f; });
+    else if (rows == D && cols == D) each([&](int i, int j, float& v) { v = p[i * si + j * sj]; });
+    else each([&](int i, int j, float& v) { v = i < rows && j < cols ? p[i * si + j * sj] : 0.f; });
   }
   __device__ __forceinline__ void store(float* p, int rows, int cols, int si, int sj) {
-    each([&](int i, int j, float& v) {
-      if (i < rows && j < cols) p[(int64_t)i * si + (int64_t)j * sj] = v;
-    });
+    if (rows == D && cols == D) each([&](int i, int j, float& v) { p[i * si + j * sj] = v; });
+    else
+      each([&](int i, int j, float& v) {
+        if (i < rows && j < cols) p[i * si + j * sj] = v;
+      });
   }
   __device__ __forceinline__ void publish(bf16* hi, bf16* lo) {
     const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
@@ -220,10 +240,15 @@ __device__ __forceinline__ void store_rows(const float (&o)[Shape<D>::OC / 8][4]
   __syncwarp();
   bf16* base = row_ptr<bf16>(w, b, t0, h);
   if (vec) {
+    constexpr int UPR = Z::OC / 8, kRows = 32 / UPR;
+    const int r0 = row0 + lane / UPR, i = col0 + lane % UPR * 8, m = i < d ? n : 0;
+    bf16* p = base + r0 * w.token + i;
+    const int64_t step = kRows * w.token;
+    stg += r0 * Z::LD + i;
 #pragma unroll
-    for (int u = lane; u < 16 * Z::OC / 8; u += 32) {
-      const int r = row0 + u / (Z::OC / 8), i = col0 + u % (Z::OC / 8) * 8;
-      if (r < n && i < d) *reinterpret_cast<uint4*>(base + r * w.token + i) = *reinterpret_cast<uint4*>(stg + r * Z::LD + i);
+    for (int r = 0; r < 16; r += kRows) {
+      if (r0 + r < m) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(stg + r * Z::LD);
+      p += step;
     }
   } else {
     for (int u = lane; u < 16 * Z::OC; u += 32) {
@@ -234,10 +259,15 @@ __device__ __forceinline__ void store_rows(const float (&o)[Shape<D>::OC / 8][4]
 }
 
 // Rows t0 .. t1 - 1 of one head set to zero by the whole block.
-__device__ __forceinline__ void zero_rows(const TmpcSeqView& w, int b, int64_t t0, int64_t t1, int h, int d) {
-  for (int64_t u = threadIdx.x; u < (t1 - t0) * d; u += blockDim.x) {
-    const int64_t t = t0 + u / d;
-    row_ptr<bf16>(w, b, t, h)[u % d] = __float2bfloat16_rn(0.f);
+__device__ __forceinline__ void zero_rows(const TmpcSeqView& w, int b, int64_t t0, int64_t t1, int h, int d, bool vec) {
+  if (t0 >= t1) return;
+  const int upr = vec ? d / 8 : d, rows = blockDim.x / upr, r0 = threadIdx.x / upr;  // d <= 128 <= the block
+  if (r0 >= rows) return;
+  bf16* p = row_ptr<bf16>(w, b, t0 + r0, h) + (threadIdx.x - r0 * upr) * (vec ? 8 : 1);
+  const int64_t step = rows * w.token;
+  for (int64_t t = t0 + r0; t < t1; t += rows, p += step) {
+    if (vec) *reinterpret_cast<uint4*>(p) = make_uint4(0, 0, 0, 0);
+    else *p = __float2bfloat16_rn(0.f);
   }
 }
 
@@ -291,13 +321,14 @@ __global__ void __launch_bounds__(Shape<D>::NT) fwd_kernel(const FwdArgs a) {
   S.load(s0, a.e, a.f, a.si, a.sj);
   S.publish(s_hi, s_lo);
 
+  Loader<D> lq(a.q, b, begin, h, a.e, a.vec), lk(a.k, b, begin, g, a.e, a.vec), lv(a.v, b, begin, g, a.f, a.vec),
+      lx(a.x, b, begin, h, a.f, a.vec);
   auto load = [&](int i) {
     bf16* buf = tiles + (i & 1) * NTILE * Z::TILE;
-    const int t0 = begin + i * C, n = min(C, len - i * C);
-    load_tile<D>(buf, a.q, b, t0, n, h, a.e, a.vec);
-    load_tile<D>(buf + Z::TILE, a.k, b, t0, n, g, a.e, a.vec);
-    load_tile<D>(buf + 2 * Z::TILE, a.v, b, t0, n, g, a.f, a.vec);
-    if constexpr (DQ) load_tile<D>(buf + 3 * Z::TILE, a.x, b, t0, n, h, a.f, a.vec);
+    const int n = min(C, len - i * C);
+    lq.load(buf, n), lk.load(buf + Z::TILE, n), lv.load(buf + 2 * Z::TILE, n);
+    lq.advance(C), lk.advance(C), lv.advance(C);
+    if constexpr (DQ) lx.load(buf + 3 * Z::TILE, n), lx.advance(C);
   };
   const int chunks = (len + C - 1) / C;
   if (chunks > 0) load(0);
@@ -408,7 +439,7 @@ __global__ void __launch_bounds__(Shape<D>::NT) fwd_kernel(const FwdArgs a) {
     }
   }
   cp_wait<0>();
-  zero_rows(a.o, b, begin + len, stop, h, a.f);
+  zero_rows(a.o, b, begin + len, stop, h, a.f, a.vec);
   if (a.state_out && seg == a.nseg - 1) S.store(a.state_out + bh * elems, a.e, a.f, a.si, a.sj);
 }
 
@@ -430,11 +461,13 @@ __global__ void __launch_bounds__(Shape<D>::NT) segment_kernel(const LinAttnArgs
   State<D> S;
   S.load(nullptr, 0, 0, 0, 0);
   const int chunks = (len + C - 1) / C;
+  const int first = REV ? begin + max(chunks - 1, 0) * C : begin;
+  Loader<D> lk(REV ? a.q : a.k, b, first, REV ? h : g, a.dk, a.vec), lv(REV ? a.o : a.v, b, first, REV ? h : g, a.dv, a.vec);
   auto load = [&](int i) {
     bf16* buf = tiles + (i & 1) * 2 * Z::TILE;
-    const int c = REV ? chunks - 1 - i : i, t0 = begin + c * C, n = min(C, len - c * C);
-    load_tile<D>(buf, REV ? a.q : a.k, b, t0, n, REV ? h : g, a.dk, a.vec);
-    load_tile<D>(buf + Z::TILE, REV ? a.o : a.v, b, t0, n, REV ? h : g, a.dv, a.vec);
+    const int c = REV ? chunks - 1 - i : i, n = min(C, len - c * C);
+    lk.load(buf, n), lv.load(buf + Z::TILE, n);
+    lk.advance(REV ? -C : C), lv.advance(REV ? -C : C);
   };
   if (chunks > 0) load(0);
   cp_commit();
@@ -521,12 +554,13 @@ __global__ void __launch_bounds__(Shape<D>::NT) dkv_kernel(const DkvArgs args) {
     R.load(r0, a.dk, a.dv, a.dv, 1);
     R.publish(r_hi, r_lo);
     bool state_on = r0 != nullptr;
+    const int last = begin + max(chunks - 1, 0) * C;
+    Loader<D> lq(a.q, b, last, h, a.dk, a.vec), lk(a.k, b, last, g, a.dk, a.vec), lv(a.v, b, last, g, a.dv, a.vec),
+        lo(a.o, b, last, h, a.dv, a.vec);
     for (int i = chunks - 1; i >= 0; --i) {
       const int t0 = begin + i * C, n = min(C, len - i * C);
-      load_tile<D>(sq, a.q, b, t0, n, h, a.dk, a.vec);
-      load_tile<D>(sk, a.k, b, t0, n, g, a.dk, a.vec);
-      load_tile<D>(sv, a.v, b, t0, n, g, a.dv, a.vec);
-      load_tile<D>(sdo, a.o, b, t0, n, h, a.dv, a.vec);
+      lq.load(sq, n), lk.load(sk, n), lv.load(sv, n), lo.load(sdo, n);
+      lq.advance(-C), lk.advance(-C), lv.advance(-C), lo.advance(-C);
       cp_commit();
       cp_wait<0>();
       __syncthreads();
@@ -674,8 +708,8 @@ __global__ void __launch_bounds__(Shape<D>::NT) dkv_kernel(const DkvArgs args) {
       if (a.dstate_in) R.store(a.dstate_in + bh * elems, a.dk, a.dv, a.dv, 1);
     }
   }
-  zero_rows(a.gk, b, begin + len, stop, g, a.dk);
-  zero_rows(a.gv, b, begin + len, stop, g, a.dv);
+  zero_rows(a.gk, b, begin + len, stop, g, a.dk, a.vec);
+  zero_rows(a.gv, b, begin + len, stop, g, a.dv, a.vec);
 }
 
 // dlog d per (sequence, head) from the chunks' shares, then the sum over the batch.
@@ -708,11 +742,6 @@ __global__ void __launch_bounds__(256) dlog_kernel(const LinAttnArgs a, const fl
   }
 }
 
-template <typename K>
-int set_smem(K kern, size_t bytes) {
-  return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-}
-
 inline int64_t resident_blocks(const TmpcLinAttnDims* d) {
   const int m = std::max(d->dk, d->dv);
   return (int64_t)sm_count() * (m <= 64 ? 2 : 1);
@@ -726,7 +755,7 @@ int run_segments(const LinAttnArgs& a, const TmpcLinAttnDims* d, float* seg, con
   by_size(d, [&](auto dd) {
     constexpr int D = decltype(dd)::value;
     const size_t smem = (size_t)4 * Shape<D>::TILE * 2 + (C + 1) * 4;
-    rc = set_smem(segment_kernel<D, REV>, smem);
+    rc = allow_smem<segment_kernel<D, REV>>((int)smem);
     if (!rc)
       segment_kernel<D, REV><<<(unsigned)((int64_t)a.B * a.nseg * a.H), Shape<D>::NT, smem, st>>>(a, seg);
   });
@@ -740,7 +769,7 @@ int run_fwd(const FwdArgs& f, const LinAttnArgs& a, const TmpcLinAttnDims* d, cu
   int rc = 0;
   by_size(d, [&](auto dd) {
     constexpr int D = decltype(dd)::value;
-    rc = set_smem(fwd_kernel<D, DQ>, fwd_smem<D>(DQ));
+    rc = allow_smem<fwd_kernel<D, DQ>>((int)fwd_smem<D>(DQ));
     if (!rc)
       fwd_kernel<D, DQ><<<(unsigned)((int64_t)a.B * a.nseg * a.H), Shape<D>::NT, fwd_smem<D>(DQ), st>>>(f);
   });
@@ -833,7 +862,7 @@ int LinAttn<bf16>::backward(LinAttnArgs a, const TmpcLinAttnDims* d, float* dlog
   const la::DkvArgs k{a, at(p.pk), dlog_decay ? at(p.edge) : nullptr};
   by_size(d, [&](auto dd) {
     constexpr int D = decltype(dd)::value;
-    rc = la::set_smem(la::dkv_kernel<D>, la::dkv_smem<D>());
+    rc = allow_smem<la::dkv_kernel<D>>((int)la::dkv_smem<D>());
     if (!rc)
       la::dkv_kernel<D><<<(unsigned)((int64_t)a.B * a.nseg * a.G), la::Shape<D>::NT, la::dkv_smem<D>(), st>>>(k);
   });

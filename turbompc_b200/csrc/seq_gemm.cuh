@@ -706,9 +706,8 @@ template <typename T, int MODE, int NT, int ACT>
 int launch(const Maps& maps, Params p, cudaStream_t st) {
   p.tiles = (int64_t)p.mtiles * p.ntiles * p.splits;
   p.polls = transfer_poll_limit().load();
-  const cudaError_t e =
-      cudaFuncSetAttribute(kernel<T, MODE, NT, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemTotal);
-  if (e != cudaSuccess) return (int)e;
+  const int rc = allow_smem<kernel<T, MODE, NT, ACT>>(kSmemTotal);
+  if (rc) return rc;
   const int64_t sms = sm_count();
   kernel<T, MODE, NT, ACT><<<(unsigned)(p.tiles < sms ? p.tiles : sms), kThreads, kSmemTotal, st>>>(maps, p);
   return (int)cudaPeekAtLastError();

@@ -10,24 +10,29 @@ once when a result is stored.  There is no CPU fallback.  ``linear_attention``,
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 from typing import Optional, Tuple
 
 import torch
 
 from . import _ffi
-from .ops import _stream
 
 ACTIVATIONS = {"silu": _ffi.ACT_SILU, "gelu": _ffi.ACT_GELU}
 MAX_HEAD_DIM = 128
 
+_SUFFIX = {torch.float32: "f32", torch.bfloat16: "bf16"}
+_ENTRIES = {}  # (entry point, dtype) -> (ctypes function, its name)
+# TmpcSeqView and TmpcLinAttnDims as packed bytes: a single token's launch is
+# shorter than the building of a few ctypes structures.
+_VIEW = struct.Struct("Pqqq").pack
+_DIMS = struct.Struct("6i").pack
+
 
 def _suffix(dtype: torch.dtype) -> str:
-    if dtype == torch.float32:
-        return "f32"
-    if dtype == torch.bfloat16:
-        return "bf16"
-    raise TypeError(f"sequence operators support float32/bfloat16, got {dtype}")
+    s = _SUFFIX.get(dtype)
+    if s is None:
+        raise TypeError(f"sequence operators support float32/bfloat16, got {dtype}")
+    return s
 
 
 def _check(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device) -> None:
@@ -47,32 +52,70 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _p(t: Optional[torch.Tensor]) -> Optional[int]:
-    return None if t is None or t.numel() == 0 else t.data_ptr()
+    return None if t is None else (t.data_ptr() or None)
 
 
-def _view(t: torch.Tensor) -> _ffi.TmpcSeqView:
-    if t.dim() == 3:  # (B, heads, dim): one token
-        return _ffi.TmpcSeqView(_p(t), t.stride(0), 0, t.stride(1))
-    return _ffi.TmpcSeqView(_p(t), t.stride(0), t.stride(1), t.stride(2))
+def _view(t: torch.Tensor) -> bytes:
+    st = t.stride()
+    if len(st) == 3:  # (B, heads, dim): one token
+        return _VIEW(t.data_ptr(), st[0], 0, st[1])
+    return _VIEW(t.data_ptr(), st[0], st[1], st[2])
+
+
+def _empty(shape, dtype, device) -> torch.Tensor:
+    return torch.empty(shape, dtype=dtype, device=device)
 
 
 def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
 
 
-def _call(name: str, device: torch.device, *args) -> None:
-    with torch.cuda.device(device):
-        _ffi.check(name, getattr(_ffi.load(), name)(*args, _stream(device)))
+def _call(entry: str, dtype: torch.dtype, device: torch.device, *args) -> None:
+    """One C call on the device's current stream."""
+    found = _ENTRIES.get((entry, dtype))
+    if found is None:
+        name = f"{entry}_{_suffix(dtype)}"
+        found = _ENTRIES[entry, dtype] = (getattr(_ffi.load(), name), name)
+    fn, name = found
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        code = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            code = fn(*args, stream)
+    if code:
+        raise _ffi.TmpcError(name, code)
 
 
 def _grad_needed(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
 
 
 # ---------------------------------------------------------------------------
 # Linear attention
 # ---------------------------------------------------------------------------
-def _attention_dims(q, k, v, log_decay, axes: str) -> _ffi.TmpcLinAttnDims:
+def _attention_dims(q, k, v, log_decay, axes: Tuple[str, ...]):
+    """(B, T, H, G, dk, dv) of checked arguments."""
+    try:
+        sq, sk, sv = q.shape, k.shape, v.shape
+        dtype, device = q.dtype, q.device
+        if (len(sq) == len(sk) == len(sv) == len(axes) and dtype in _SUFFIX and k.dtype == dtype and v.dtype == dtype
+                and q.is_cuda and k.device == device and v.device == device
+                and log_decay.dtype == torch.float32 and log_decay.device == device):
+            H, G, dk, dv = sq[-2], sk[-2], sq[-1], sv[-1]
+            if (sk[-1] == dk and sv[-2] == G and sk[0] == sq[0] == sv[0] and sk[1:-2] == sq[1:-2] == sv[1:-2]
+                    and log_decay.shape == (H,) and G > 0 and H > 0 and H % G == 0
+                    and 1 <= dk <= MAX_HEAD_DIM and 1 <= dv <= MAX_HEAD_DIM):
+                return sq[0], (sq[1] if len(axes) == 4 else 1), H, G, dk, dv
+    except AttributeError:
+        pass
+    # something is wrong: say what
     if not isinstance(q, torch.Tensor):
         raise TypeError(f"q must be a tensor, got {type(q).__name__}")
     _suffix(q.dtype)
@@ -88,28 +131,27 @@ def _attention_dims(q, k, v, log_decay, axes: str) -> _ffi.TmpcLinAttnDims:
     if not (1 <= dk <= MAX_HEAD_DIM and 1 <= dv <= MAX_HEAD_DIM):
         raise ValueError(f"head sizes {dk}, {dv} must be within 1..{MAX_HEAD_DIM}")
     _check(log_decay, "log_decay", torch.float32, q.device)
-    if tuple(log_decay.shape) != (H,):
-        raise ValueError(f"log_decay has shape {tuple(log_decay.shape)}, expected ({H},)")
-    T = q.shape[1] if len(axes) == 4 else 1
-    return _ffi.TmpcLinAttnDims(q.shape[0], T, H, G, dk, dv)
+    raise ValueError(f"log_decay has shape {tuple(log_decay.shape)}, expected ({H},)")
 
 
-def _check_state(t, name: str, dims, device, contiguous: bool = False) -> None:
+def _check_state(t, name: str, want, device, contiguous: bool = False) -> None:
     _check(t, name, torch.float32, device)
-    want = (dims.B, dims.H, dims.dk, dims.dv)
-    if tuple(t.shape) != want:
+    if t.shape != want:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {want}")
     if contiguous and not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
 
 
 def _attention_forward(dims, q, k, v, log_decay, lengths, initial, scale, want_state):
-    o = torch.empty(dims.B, dims.T, dims.H, dims.dv, dtype=q.dtype, device=q.device)
-    state = torch.empty(dims.B, dims.H, dims.dk, dims.dv, dtype=torch.float32, device=q.device) if want_state else None
-    need = int(_ffi.load().tmpc_linear_attention_workspace_bytes(C.byref(dims)))
-    ws = _workspace(need, q.device)
-    _call(f"tmpc_linear_attention_{_suffix(q.dtype)}", q.device, C.byref(dims), C.byref(_view(q)), C.byref(_view(k)),
-          C.byref(_view(v)), C.byref(_view(o)), _p(log_decay), _p(lengths), _p(initial), _p(state), scale, _p(ws), need)
+    B, T, H, _, dk, dv = dims
+    dtype, device = q.dtype, q.device
+    o = _empty((B, T, H, dv), dtype, device)
+    state = _empty((B, H, dk, dv), torch.float32, device) if want_state else None
+    packed = _DIMS(*dims)
+    need = _ffi.load().tmpc_linear_attention_workspace_bytes(packed)
+    ws = _workspace(need, device)
+    _call("tmpc_linear_attention", dtype, device, packed, _view(q), _view(k), _view(v), _view(o), _p(log_decay),
+          _p(lengths), _p(initial), _p(state), scale, _p(ws), need)
     return o, state
 
 
@@ -125,19 +167,19 @@ class _LinearAttention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, do, dstate):
         q, k, v, log_decay, initial, lengths = ctx.saved_tensors
-        dims, dev = ctx.dims, q.device
+        dims, dtype, dev = ctx.dims, q.dtype, q.device
         if do is None:
-            do = torch.zeros(dims.B, dims.T, dims.H, dims.dv, dtype=q.dtype, device=dev)
+            do = torch.zeros((dims[0], dims[1], dims[2], dims[5]), dtype=dtype, device=dev)
         do = _rows(do)
         dstate = None if dstate is None else dstate.contiguous()
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+        dq, dk, dv = _empty(q.shape, dtype, dev), _empty(k.shape, dtype, dev), _empty(v.shape, dtype, dev)
         dlog = torch.empty_like(log_decay) if ctx.needs_input_grad[3] else None
-        dinit = torch.empty(initial.shape, dtype=torch.float32, device=dev) if ctx.needs_input_grad[4] else None
-        need = int(_ffi.load().tmpc_linear_attention_backward_workspace_bytes(C.byref(dims)))
+        dinit = torch.empty_like(initial) if ctx.needs_input_grad[4] else None
+        packed = _DIMS(*dims)
+        need = _ffi.load().tmpc_linear_attention_backward_workspace_bytes(packed)
         ws = _workspace(need, dev)
-        _call(f"tmpc_linear_attention_backward_{_suffix(q.dtype)}", dev, C.byref(dims), C.byref(_view(q)),
-              C.byref(_view(k)), C.byref(_view(v)), C.byref(_view(do)), C.byref(_view(dq)), C.byref(_view(dk)),
-              C.byref(_view(dv)), _p(log_decay), _p(lengths), _p(initial), _p(dstate), _p(dlog), _p(dinit), ctx.scale,
+        _call("tmpc_linear_attention_backward", dtype, dev, packed, _view(q), _view(k), _view(v), _view(do), _view(dq),
+              _view(dk), _view(dv), _p(log_decay), _p(lengths), _p(initial), _p(dstate), _p(dlog), _p(dinit), ctx.scale,
               _p(ws), need)
         return dq, dk, dv, dlog, dinit, None, None, None, None
 
@@ -162,14 +204,15 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     Differentiable with respect to q, k, v, log_decay and initial_state.
     """
     dims = _attention_dims(q, k, v, log_decay, ("B", "T", "H", "D"))
-    scale = float(dims.dk ** -0.5 if scale is None else scale)
+    B, _, H, _, dk, dv = dims
+    scale = dk ** -0.5 if scale is None else float(scale)
     if initial_state is not None:
-        _check_state(initial_state, "initial_state", dims, q.device)
+        _check_state(initial_state, "initial_state", (B, H, dk, dv), q.device)
         initial_state = initial_state.contiguous()
     if lengths is not None:
         _check(lengths, "lengths", torch.int32, q.device)
-        if tuple(lengths.shape) != (dims.B,):
-            raise ValueError(f"lengths has shape {tuple(lengths.shape)}, expected ({dims.B},)")
+        if lengths.shape != (B,):
+            raise ValueError(f"lengths has shape {tuple(lengths.shape)}, expected ({B},)")
         lengths = lengths.contiguous()
     q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
     if _grad_needed(q, k, v, log_decay, initial_state):
@@ -188,17 +231,20 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     ``state_out``.  Returns o (B, H, dv).  Not differentiable: a call that
     needs gradients is refused (use ``linear_attention`` with T = 1)."""
     dims = _attention_dims(q, k, v, log_decay, ("B", "H", "D"))
+    B, _, H, _, dk, dv = dims
+    dtype, device = q.dtype, q.device
     out_state = state if state_out is None else state_out
-    _check_state(state, "state", dims, q.device, contiguous=True)
-    _check_state(out_state, "state_out", dims, q.device, contiguous=True)
+    _check_state(state, "state", (B, H, dk, dv), device, contiguous=True)
+    if state_out is not None:
+        _check_state(out_state, "state_out", (B, H, dk, dv), device, contiguous=True)
     if _grad_needed(q, k, v, log_decay, state, out_state):
         raise RuntimeError("linear_attention_step has no gradient; call it under torch.no_grad(), or use "
                            "linear_attention with T = 1")
-    scale = float(dims.dk ** -0.5 if scale is None else scale)
+    scale = dk ** -0.5 if scale is None else float(scale)
     q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
-    o = torch.empty(dims.B, dims.H, dims.dv, dtype=q.dtype, device=q.device)
-    _call(f"tmpc_linear_attention_step_{_suffix(q.dtype)}", q.device, C.byref(dims), C.byref(_view(q)),
-          C.byref(_view(k)), C.byref(_view(v)), C.byref(_view(o)), _p(log_decay), _p(state), _p(out_state), scale)
+    o = _empty((B, H, dv), dtype, device)
+    _call("tmpc_linear_attention_step", dtype, device, _DIMS(*dims), _view(q), _view(k), _view(v), _view(o),
+          _p(log_decay), _p(state), _p(out_state), scale)
     return o
 
 
@@ -206,15 +252,18 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
 # Residual addition and root-mean-square norm
 # ---------------------------------------------------------------------------
 def _norm_forward(x, residual, weight, eps, want_inv):
-    d = x.shape[-1]
-    x2 = _rows(x.reshape(-1, d))
-    r2 = None if residual is None else _rows(residual.reshape(-1, d))
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    s = None if residual is None else torch.empty_like(y)
+    shape, dtype, device = x.shape, x.dtype, x.device
+    d = shape[-1]
+    x2 = _rows(x if len(shape) == 2 else x.reshape(-1, d))
+    y = _empty(shape, dtype, device)
+    r2 = s = None
+    if residual is not None:
+        r2 = _rows(residual if len(shape) == 2 else residual.reshape(-1, d))
+        s = _empty(shape, dtype, device)
     rows = x2.shape[0]
-    inv = torch.empty(rows, dtype=torch.float32, device=x.device) if want_inv else None
-    _call(f"tmpc_add_rms_norm_{_suffix(x.dtype)}", x.device, rows, d, _p(x2), x2.stride(0), _p(r2),
-          0 if r2 is None else r2.stride(0), _p(weight), eps, _p(y), _p(s), _p(inv))
+    inv = _empty((rows,), torch.float32, device) if want_inv else None
+    _call("tmpc_add_rms_norm", dtype, device, rows, d, _p(x2), x2.stride(0), _p(r2), 0 if r2 is None else r2.stride(0),
+          _p(weight), eps, _p(y), _p(s), _p(inv))
     return y, s, inv
 
 
@@ -236,11 +285,11 @@ class _AddRmsNorm(torch.autograd.Function):
             dy = torch.zeros(ctx.shape, dtype=t.dtype, device=t.device)
         dy = dy.contiguous()
         ds = None if ds is None else ds.contiguous()
-        dx, dw = torch.empty(ctx.shape, dtype=t.dtype, device=t.device), torch.empty_like(weight)
-        need = int(_ffi.load().tmpc_add_rms_norm_workspace_bytes(rows, d))
+        dx, dw = _empty(ctx.shape, t.dtype, t.device), torch.empty_like(weight)
+        need = _ffi.load().tmpc_add_rms_norm_workspace_bytes(rows, d)
         ws = _workspace(need, t.device)
-        _call(f"tmpc_add_rms_norm_backward_{_suffix(t.dtype)}", t.device, rows, d, _p(dy), _p(ds), _p(t), _p(weight),
-              _p(inv), _p(dx), _p(dw), _p(ws), need)
+        _call("tmpc_add_rms_norm_backward", t.dtype, t.device, rows, d, _p(dy), _p(ds), _p(t), _p(weight), _p(inv),
+              _p(dx), _p(dw), _p(ws), need)
         return dx, (dx if ctx.has_residual else None), dw, None
 
 
@@ -252,17 +301,18 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
     Differentiable with respect to x, residual and weight."""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"x must be a tensor, got {type(x).__name__}")
-    _suffix(x.dtype)
-    _check(x, "x", x.dtype, x.device)
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= 16384:
-        raise ValueError(f"x must have 1..16384 elements on its last axis, got shape {tuple(x.shape)}")
+    dtype, device, shape = x.dtype, x.device, x.shape
+    _suffix(dtype)
+    _check(x, "x", dtype, device)
+    if len(shape) < 1 or not 1 <= shape[-1] <= 16384:
+        raise ValueError(f"x must have 1..16384 elements on its last axis, got shape {tuple(shape)}")
     if residual is not None:
-        _check(residual, "residual", x.dtype, x.device)
-        if residual.shape != x.shape:
-            raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {tuple(x.shape)}")
-    _check(weight, "weight", x.dtype, x.device)
-    if tuple(weight.shape) != (x.shape[-1],):
-        raise ValueError(f"weight has shape {tuple(weight.shape)}, expected ({x.shape[-1]},)")
+        _check(residual, "residual", dtype, device)
+        if residual.shape != shape:
+            raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {tuple(shape)}")
+    _check(weight, "weight", dtype, device)
+    if weight.shape != shape[-1:]:
+        raise ValueError(f"weight has shape {tuple(weight.shape)}, expected ({shape[-1]},)")
     weight = weight.contiguous()
     if _grad_needed(x, residual, weight):
         y, s = _AddRmsNorm.apply(x, residual, weight, float(eps))
@@ -282,11 +332,11 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 def _gated_forward(x2, w_gate, w_up, act):
     rows, d, f = x2.shape[0], x2.shape[1], w_gate.shape[0]
-    h = torch.empty(rows, f, dtype=x2.dtype, device=x2.device)
-    need = int(_ffi.load().tmpc_gated_linear_workspace_bytes(rows, d, f, x2.element_size()))
-    ws = _workspace(need, x2.device)
-    _call(f"tmpc_gated_linear_{_suffix(x2.dtype)}", x2.device, rows, d, f, _p(x2), _p(w_gate), _p(w_up), act, _p(h),
-          _p(ws), need)
+    dtype, device = x2.dtype, x2.device
+    h = _empty((rows, f), dtype, device)
+    need = _ffi.load().tmpc_gated_linear_workspace_bytes(rows, d, f, x2.element_size())
+    ws = _workspace(need, device)
+    _call("tmpc_gated_linear", dtype, device, rows, d, f, _p(x2), _p(w_gate), _p(w_up), act, _p(h), _p(ws), need)
     return h
 
 
@@ -303,13 +353,13 @@ class _GatedLinear(torch.autograd.Function):
         x2, w_gate, w_up = ctx.saved_tensors
         rows, d, f = x2.shape[0], x2.shape[1], w_gate.shape[0]
         dh = dh.contiguous()
-        dx = torch.empty(x2.shape, dtype=x2.dtype, device=x2.device) if ctx.needs_input_grad[0] else None
+        dx = torch.empty_like(x2) if ctx.needs_input_grad[0] else None
         want_w = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         dwg, dwu = (torch.empty_like(w_gate), torch.empty_like(w_up)) if want_w else (None, None)
-        need = int(_ffi.load().tmpc_gated_linear_backward_workspace_bytes(rows, d, f, x2.element_size()))
+        need = _ffi.load().tmpc_gated_linear_backward_workspace_bytes(rows, d, f, x2.element_size())
         ws = _workspace(need, x2.device)
-        _call(f"tmpc_gated_linear_backward_{_suffix(x2.dtype)}", x2.device, rows, d, f, _p(x2), _p(w_gate), _p(w_up),
-              ctx.act, _p(dh), _p(dx), _p(dwg), _p(dwu), _p(ws), need)
+        _call("tmpc_gated_linear_backward", x2.dtype, x2.device, rows, d, f, _p(x2), _p(w_gate), _p(w_up), ctx.act,
+              _p(dh), _p(dx), _p(dwg), _p(dwu), _p(ws), need)
         return dx, dwg, dwu, None
 
 
@@ -334,10 +384,10 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, acti
         raise ValueError(f"shapes of x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)} and w_up {tuple(w_up.shape)} "
                          "do not fit")
     act = ACTIVATIONS[activation]
-    x2 = _aligned(x.reshape(-1, x.shape[-1]))
+    x2 = _aligned(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
     w_gate, w_up = _aligned(w_gate), _aligned(w_up)
     if _grad_needed(x2, w_gate, w_up):
         h = _GatedLinear.apply(x2, w_gate, w_up, act)
     else:
         h = _gated_forward(x2, w_gate, w_up, act)
-    return h.reshape(*x.shape[:-1], w_gate.shape[0])
+    return h if x.dim() == 2 else h.reshape(*x.shape[:-1], w_gate.shape[0])

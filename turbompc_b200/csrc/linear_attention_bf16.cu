@@ -84,11 +84,13 @@ struct Shape {
   static constexpr int OC = D == 128 ? 64 : D;        // output columns of a warp
   static constexpr int SC = D == 32 ? 16 : D;         // state columns of a warp (16 rows)
   static constexpr int TILE = C * LD;                 // elements
+  static constexpr int kBlocks = D == 32 ? 5 : D == 64 ? 3 : 1;     // blocks per SM that the registers allow
+  static constexpr int kBlocksDkv = D == 32 ? 4 : D == 64 ? 3 : 1;
   static constexpr int STATE = D * LD;
 };
 
-// One head's rows, chunk by chunk, into [C][LD] tiles: row r of a chunk's n
-// tokens, the rest zero.  A thread keeps its column and every kRows-th row.
+// One head's n tokens from t0 on into a [C][LD] tile, the rest zero.  A thread
+// has one 16-byte column and every kRows-th row.
 template <int D>
 struct Loader {
   using Z = Shape<D>;
@@ -99,7 +101,6 @@ struct Loader {
   bool vec;
   __device__ __forceinline__ Loader(const TmpcSeqView& w, int b, int64_t t0, int h, int d_, bool vec_)
       : base(row_ptr<bf16>(w, b, t0, h)), token(w.token), d(d_), vec(vec_) {}
-  __device__ __forceinline__ void advance(int tokens) { base += tokens * token; }
   __device__ __forceinline__ void load(bf16* s, int n) const {
     if (vec) {
       const int i = threadIdx.x % UPR * 8, r0 = threadIdx.x / UPR;
@@ -166,14 +167,29 @@ struct State {
 #pragma unroll
       for (int e = 0; e < 4; ++e) f(row0 + g + (e >> 1) * 8, col0 + j * 8 + 2 * t + (e & 1), s[j][e]);
   }
+  template <typename F>
+  __device__ __forceinline__ void pairs(F&& f) {  // f(row, col, two values)
+    const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+#pragma unroll
+    for (int j = 0; j < Z::SC / 8; ++j)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) f(row0 + g + r * 8, col0 + j * 8 + 2 * t, &s[j][2 * r]);
+  }
+  static __device__ __forceinline__ bool aligned8(const float* p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; }
   // rows x cols of a float array, element (i, j) at p[i si + j sj]; zero elsewhere
   __device__ __forceinline__ void load(const float* p, int rows, int cols, int si, int sj) {
     if (!p) each([&](int, int, float& v) { v = 0.f; });
+    else if (rows == D && cols == D && sj == 1 && aligned8(p)) pairs([&](int i, int j, float* v) {
+      const float2 x = *reinterpret_cast<const float2*>(p + i * si + j);
+      v[0] = x.x, v[1] = x.y;
+    });
     else if (rows == D && cols == D) each([&](int i, int j, float& v) { v = p[i * si + j * sj]; });
     else each([&](int i, int j, float& v) { v = i < rows && j < cols ? p[i * si + j * sj] : 0.f; });
   }
   __device__ __forceinline__ void store(float* p, int rows, int cols, int si, int sj) {
-    if (rows == D && cols == D) each([&](int i, int j, float& v) { p[i * si + j * sj] = v; });
+    if (rows == D && cols == D && sj == 1 && aligned8(p))
+      pairs([&](int i, int j, float* v) { *reinterpret_cast<float2*>(p + i * si + j) = make_float2(v[0], v[1]); });
+    else if (rows == D && cols == D) each([&](int i, int j, float& v) { p[i * si + j * sj] = v; });
     else
       each([&](int i, int j, float& v) {
         if (i < rows && j < cols) p[i * si + j * sj] = v;
@@ -288,18 +304,17 @@ struct FwdArgs {
 };
 
 template <int D>
-constexpr size_t fwd_smem(bool dq) {
+constexpr size_t fwd_smem() {
   using Z = Shape<D>;
-  return (size_t)(2 * (dq ? 4 : 3) * Z::TILE + 2 * Z::STATE) * 2 + (C + 1 + 16) * 4;
+  return (size_t)(2 * 3 * Z::TILE + 2 * Z::STATE) * 2 + (C + 1 + 16) * 4;
 }
 
 template <int D, bool DQ>
-__global__ void __launch_bounds__(Shape<D>::NT) fwd_kernel(const FwdArgs a) {
+__global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocks) fwd_kernel(const FwdArgs a) {
   using Z = Shape<D>;
-  constexpr int NTILE = DQ ? 4 : 3;
   extern __shared__ __align__(16) char raw[];
   bf16* tiles = reinterpret_cast<bf16*>(raw);
-  bf16* s_hi = tiles + 2 * NTILE * Z::TILE;
+  bf16* s_hi = tiles + 2 * 3 * Z::TILE;
   bf16* s_lo = s_hi + Z::STATE;
   float* pw = reinterpret_cast<float*>(s_lo + Z::STATE);  // d^i
   float* red = pw + C + 1;
@@ -321,14 +336,12 @@ __global__ void __launch_bounds__(Shape<D>::NT) fwd_kernel(const FwdArgs a) {
   S.load(s0, a.e, a.f, a.si, a.sj);
   S.publish(s_hi, s_lo);
 
-  Loader<D> lq(a.q, b, begin, h, a.e, a.vec), lk(a.k, b, begin, g, a.e, a.vec), lv(a.v, b, begin, g, a.f, a.vec),
-      lx(a.x, b, begin, h, a.f, a.vec);
   auto load = [&](int i) {
-    bf16* buf = tiles + (i & 1) * NTILE * Z::TILE;
-    const int n = min(C, len - i * C);
-    lq.load(buf, n), lk.load(buf + Z::TILE, n), lv.load(buf + 2 * Z::TILE, n);
-    lq.advance(C), lk.advance(C), lv.advance(C);
-    if constexpr (DQ) lx.load(buf + 3 * Z::TILE, n), lx.advance(C);
+    bf16* buf = tiles + (i & 1) * 3 * Z::TILE;
+    const int t0 = begin + i * C, n = min(C, len - i * C);
+    Loader<D>(a.q, b, t0, h, a.e, a.vec).load(buf, n);
+    Loader<D>(a.k, b, t0, g, a.e, a.vec).load(buf + Z::TILE, n);
+    Loader<D>(a.v, b, t0, g, a.f, a.vec).load(buf + 2 * Z::TILE, n);
   };
   const int chunks = (len + C - 1) / C;
   if (chunks > 0) load(0);
@@ -339,13 +352,32 @@ __global__ void __launch_bounds__(Shape<D>::NT) fwd_kernel(const FwdArgs a) {
     cp_commit();
     cp_wait<1>();
     __syncthreads();
-    bf16* sq = tiles + (i & 1) * NTILE * Z::TILE;
+    bf16* sq = tiles + (i & 1) * 3 * Z::TILE;
     const bf16 *sk = sq + Z::TILE, *sv = sk + Z::TILE;
     const int n = min(C, len - i * C);
     if (row0 < n) {
       uint32_t q[D / 16][4];
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) ldsm(q[k], frag_a<Z::LD>(sq, row0, k * 16));
+      uint32_t x[DQ ? Z::OC / 4 : 1];  // the queries in the layout of o, on their way during the products
+      if constexpr (DQ) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int row = row0 + gr + r * 8;
+          const bf16* p = row_ptr<bf16>(a.x, b, begin + i * C + row, h) + col0 + 2 * tq;
+#pragma unroll
+          for (int j = 0; j < Z::OC / 8; ++j) {
+            const int c = col0 + j * 8 + 2 * tq;
+            uint32_t v = 0;
+            if (row < n && c < a.f) {
+              if (a.vec) v = *reinterpret_cast<const uint32_t*>(p + j * 8);
+              else v = (uint32_t)__bfloat16_as_ushort(p[j * 8]) |
+                       (c + 1 < a.f ? (uint32_t)__bfloat16_as_ushort(p[j * 8 + 1]) << 16 : 0u);
+            }
+            x[2 * j + r] = v;
+          }
+        }
+      }
       float o[Z::OC / 8][4];
 #pragma unroll
       for (int j = 0; j < Z::OC / 8; ++j)
@@ -370,13 +402,10 @@ __global__ void __launch_bounds__(Shape<D>::NT) fwd_kernel(const FwdArgs a) {
       }
       if constexpr (DQ) {
         // q . dq of the part that comes from the state, rows weighted by t + 1 as well
-        const bf16* sx = sq + 3 * Z::TILE;
         float p0 = 0.f, p1 = 0.f;
 #pragma unroll
         for (int j = 0; j < Z::OC / 8; ++j) {
-          const int c = col0 + j * 8 + 2 * tq;
-          const float2 x0 = unpack2(*reinterpret_cast<const uint32_t*>(sx + (row0 + gr) * Z::LD + c));
-          const float2 x1 = unpack2(*reinterpret_cast<const uint32_t*>(sx + (row0 + gr + 8) * Z::LD + c));
+          const float2 x0 = unpack2(x[2 * j]), x1 = unpack2(x[2 * j + 1]);
           p0 = fmaf(x0.x, o[j][0], fmaf(x0.y, o[j][1], p0));
           p1 = fmaf(x1.x, o[j][2], fmaf(x1.y, o[j][3], p1));
         }
@@ -461,13 +490,11 @@ __global__ void __launch_bounds__(Shape<D>::NT) segment_kernel(const LinAttnArgs
   State<D> S;
   S.load(nullptr, 0, 0, 0, 0);
   const int chunks = (len + C - 1) / C;
-  const int first = REV ? begin + max(chunks - 1, 0) * C : begin;
-  Loader<D> lk(REV ? a.q : a.k, b, first, REV ? h : g, a.dk, a.vec), lv(REV ? a.o : a.v, b, first, REV ? h : g, a.dv, a.vec);
   auto load = [&](int i) {
     bf16* buf = tiles + (i & 1) * 2 * Z::TILE;
-    const int c = REV ? chunks - 1 - i : i, n = min(C, len - c * C);
-    lk.load(buf, n), lv.load(buf + Z::TILE, n);
-    lk.advance(REV ? -C : C), lv.advance(REV ? -C : C);
+    const int c = REV ? chunks - 1 - i : i, t0 = begin + c * C, n = min(C, len - c * C);
+    Loader<D>(REV ? a.q : a.k, b, t0, REV ? h : g, a.dk, a.vec).load(buf, n);
+    Loader<D>(REV ? a.o : a.v, b, t0, REV ? h : g, a.dv, a.vec).load(buf + Z::TILE, n);
   };
   if (chunks > 0) load(0);
   cp_commit();
@@ -521,7 +548,7 @@ constexpr size_t dkv_smem() {
 }
 
 template <int D>
-__global__ void __launch_bounds__(Shape<D>::NT) dkv_kernel(const DkvArgs args) {
+__global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocksDkv) dkv_kernel(const DkvArgs args) {
   using Z = Shape<D>;
   const LinAttnArgs& a = args.a;
   extern __shared__ __align__(16) char raw[];
@@ -554,13 +581,12 @@ __global__ void __launch_bounds__(Shape<D>::NT) dkv_kernel(const DkvArgs args) {
     R.load(r0, a.dk, a.dv, a.dv, 1);
     R.publish(r_hi, r_lo);
     bool state_on = r0 != nullptr;
-    const int last = begin + max(chunks - 1, 0) * C;
-    Loader<D> lq(a.q, b, last, h, a.dk, a.vec), lk(a.k, b, last, g, a.dk, a.vec), lv(a.v, b, last, g, a.dv, a.vec),
-        lo(a.o, b, last, h, a.dv, a.vec);
     for (int i = chunks - 1; i >= 0; --i) {
       const int t0 = begin + i * C, n = min(C, len - i * C);
-      lq.load(sq, n), lk.load(sk, n), lv.load(sv, n), lo.load(sdo, n);
-      lq.advance(-C), lk.advance(-C), lv.advance(-C), lo.advance(-C);
+      Loader<D>(a.q, b, t0, h, a.dk, a.vec).load(sq, n);
+      Loader<D>(a.k, b, t0, g, a.dk, a.vec).load(sk, n);
+      Loader<D>(a.v, b, t0, g, a.dv, a.vec).load(sv, n);
+      Loader<D>(a.o, b, t0, h, a.dv, a.vec).load(sdo, n);
       cp_commit();
       cp_wait<0>();
       __syncthreads();
@@ -662,25 +688,23 @@ __global__ void __launch_bounds__(Shape<D>::NT) dkv_kernel(const DkvArgs args) {
         args.part[(bh * all_chunks + seg * (a.seg_len / C) + i) * 3 + threadIdx.x] = s;
       }
       if (row0 < n) {
-        if (rep > 1) {  // the key head's sum so far, [token][dk | dv] float
-          float* acc = a.acc + ((int64_t)b * a.T + t0) * a.G * (a.dk + a.dv) + (int64_t)g * (a.dk + a.dv);
-          const int64_t pitch = (int64_t)a.G * (a.dk + a.dv);
+        if (rep > 1) {  // the key head's sum so far, as this thread left it
+          float4* acc = reinterpret_cast<float4*>(a.acc) +
+                        ((((int64_t)b * a.G + g) * all_chunks + seg * (a.seg_len / C) + i) * Z::NW + warp) *
+                            (Z::OC / 4 * 32) + lane;
 #pragma unroll
-          for (int j = 0; j < Z::OC / 8; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int s = row0 + gr + (e >> 1) * 8, c = col0 + j * 8 + 2 * tq + (e & 1);
-              if (s < n && c < a.dk) {
-                float* p = acc + s * pitch + c;
-                if (r > 0) dk[j][e] += *p;
-                if (r + 1 < rep) *p = dk[j][e];
-              }
-              if (s < n && c < a.dv) {
-                float* p = acc + s * pitch + a.dk + c;
-                if (r > 0) dv[j][e] += *p;
-                if (r + 1 < rep) *p = dv[j][e];
-              }
+          for (int j = 0; j < Z::OC / 8; ++j) {
+            float4 *pk = acc + 2 * j * 32, *pv = pk + 32;
+            if (r > 0) {
+              const float4 x = *pk, y = *pv;
+              dk[j][0] += x.x, dk[j][1] += x.y, dk[j][2] += x.z, dk[j][3] += x.w;
+              dv[j][0] += y.x, dv[j][1] += y.y, dv[j][2] += y.z, dv[j][3] += y.w;
             }
+            if (r + 1 < rep) {
+              *pk = make_float4(dk[j][0], dk[j][1], dk[j][2], dk[j][3]);
+              *pv = make_float4(dv[j][0], dv[j][1], dv[j][2], dv[j][3]);
+            }
+          }
         }
         if (r + 1 == rep) {
           store_rows<D>(dk, sk, a.gk, b, t0, n, g, a.dk, a.vec);
@@ -769,9 +793,9 @@ int run_fwd(const FwdArgs& f, const LinAttnArgs& a, const TmpcLinAttnDims* d, cu
   int rc = 0;
   by_size(d, [&](auto dd) {
     constexpr int D = decltype(dd)::value;
-    rc = allow_smem<fwd_kernel<D, DQ>>((int)fwd_smem<D>(DQ));
+    rc = allow_smem<fwd_kernel<D, DQ>>((int)fwd_smem<D>());
     if (!rc)
-      fwd_kernel<D, DQ><<<(unsigned)((int64_t)a.B * a.nseg * a.H), Shape<D>::NT, fwd_smem<D>(DQ), st>>>(f);
+      fwd_kernel<D, DQ><<<(unsigned)((int64_t)a.B * a.nseg * a.H), Shape<D>::NT, fwd_smem<D>(), st>>>(f);
   });
   return rc ? rc : (int)cudaPeekAtLastError();
 }
@@ -796,7 +820,9 @@ inline BackwardPlan backward_plan(const LinAttnArgs& a, const TmpcLinAttnDims* d
   p.pq = take(bh * chunks * 2);
   p.pk = take(bh * chunks * 3);
   p.edge = take(bh);
-  p.acc = take(d->H > d->G ? (size_t)d->B * d->T * d->G * (d->dk + d->dv) : 0);
+  size_t chunk_floats = 0;
+  by_size(d, [&](auto dd) { chunk_floats = (size_t)C * 2 * decltype(dd)::value; });
+  p.acc = take(d->H > d->G ? (size_t)d->B * d->G * chunks * chunk_floats : 0);
   p.total = at;
   return p;
 }

@@ -15,9 +15,11 @@
 // the warps' matrix instructions with their operands in registers, where the
 // masked scores turn into the next product's operand without leaving the
 // thread.  The state stays in float registers; for a product it is split into
-// two bfloat16 terms (together 2^-17), as is the decayed factor of the state's
-// update, because states and dlog d are float results.  Scores are rounded to
-// one bfloat16 (2^-9): their sums leave as bfloat16.
+// bfloat16 terms, as is the decayed factor of the state's update: three terms
+// (2^-27) where the result is float (states and their adjoints, dlog d, whose
+// telescoping sums came out 1e-5 off with two), two towards o and dq and one
+// towards dk and dv where only those are asked for.  Scores are rounded to one
+// bfloat16 (2^-9): their sums leave as bfloat16.
 //
 // dlog d is the sum over pairs of (t - s) times the pair's share.  Within a
 // chunk it is formed from the two float score matrices.  Across chunks the lag
@@ -59,11 +61,15 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 __device__ __forceinline__ float2 unpack2(uint32_t v) {
   return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
-// (x, y) as hi + lo, two bfloat16 each.
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  hi = pack2(x, y);
-  const float2 h = unpack2(hi);
-  lo = pack2(x - h.x, y - h.y);
+// (x, y) as a sum of N pairs of bfloat16: 2^-9, 2^-18 or 2^-27 off.
+template <int N>
+__device__ __forceinline__ void split(float x, float y, uint32_t (&t)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    t[i] = pack2(x, y);
+    const float2 h = unpack2(t[i]);
+    x -= h.x, y -= h.y;
+  }
 }
 
 __device__ __forceinline__ void cp16(void* dst, const void* src, bool on) {
@@ -78,18 +84,26 @@ __device__ __forceinline__ void cp_wait() {
 
 template <int D>
 struct Shape {
-  static constexpr int LD = D + 8;                    // row pitch: eight 16-byte rows fall into different banks
   static constexpr int NW = D == 128 ? 8 : 4;         // warps: 4 row groups of 16 tokens x column groups
   static constexpr int NT = NW * 32;
   static constexpr int OC = D == 128 ? 64 : D;        // output columns of a warp
   static constexpr int SC = D == 32 ? 16 : D;         // state columns of a warp (16 rows)
-  static constexpr int TILE = C * LD;                 // elements
+  static constexpr int TILE = C * D;                  // elements
   static constexpr int kBlocks = D == 32 ? 5 : D == 64 ? 3 : 1;     // blocks per SM that the registers allow
   static constexpr int kBlocksDkv = D == 32 ? 4 : D == 64 ? 3 : 1;
-  static constexpr int STATE = D * LD;
+  static constexpr int STATE = D * D;
 };
 
-// One head's n tokens from t0 on into a [C][LD] tile, the rest zero.  A thread
+// Element (row, col) of a tile of D-wide rows: the 16-byte units of a row are
+// permuted by the row's number, so that eight rows' units of one column fall
+// into different banks.
+template <int D>
+__device__ __forceinline__ int at(int row, int col) {
+  const int x = D == 32 ? (row >> 1) & 3 : row & 7;
+  return row * D + (((col >> 3) ^ x) << 3) + (col & 7);
+}
+
+// One head's n tokens from t0 on into a C x D tile, the rest zero.  A thread
 // has one 16-byte column and every kRows-th row.
 template <int D>
 struct Loader {
@@ -106,18 +120,19 @@ struct Loader {
       const int i = threadIdx.x % UPR * 8, r0 = threadIdx.x / UPR;
       const bf16* p = base + r0 * token + i;
       const int64_t step = kRows * token;
-      s += r0 * Z::LD + i;
+      static_assert(kRows % 8 == 0, "a thread's rows share their permutation");
+      s += at<D>(r0, i);
       const int m = i < d ? n : 0;
 #pragma unroll
       for (int r = 0; r < C; r += kRows) {
         const bool on = r0 + r < m;
-        cp16(s + r * Z::LD, on ? p : base, on);
+        cp16(s + r * D, on ? p : base, on);
         p += step;
       }
     } else {
       for (int u = threadIdx.x; u < C * D; u += Z::NT) {
         const int t = u / D, i = u % D;
-        s[t * Z::LD + i] = (t < n && i < d) ? base[t * token + i] : __float2bfloat16_rn(0.f);
+        s[at<D>(t, i)] = (t < n && i < d) ? base[t * token + i] : __float2bfloat16_rn(0.f);
       }
     }
   }
@@ -126,25 +141,25 @@ struct Loader {
 // Fragment addresses: A (rows m, K k) of a row-major [m][k] tile; A of a tile
 // stored [k][m]; B (two 8-wide column tiles) of a tile stored [n][k], of one
 // stored [k][n].
-template <int LD>
+template <int D>
 __device__ __forceinline__ const bf16* frag_a(const bf16* s, int m0, int k0) {
   const int l = threadIdx.x & 31;
-  return s + (m0 + (l & 15)) * LD + k0 + (l >> 4) * 8;
+  return s + at<D>(m0 + (l & 15), k0 + (l >> 4) * 8);
 }
-template <int LD>
+template <int D>
 __device__ __forceinline__ const bf16* frag_at(const bf16* s, int m0, int k0) {
   const int l = threadIdx.x & 31;
-  return s + (k0 + (l & 7) + (l >> 4) * 8) * LD + m0 + ((l >> 3) & 1) * 8;
+  return s + at<D>(k0 + (l & 7) + (l >> 4) * 8, m0 + ((l >> 3) & 1) * 8);
 }
-template <int LD>
+template <int D>
 __device__ __forceinline__ const bf16* frag_bn(const bf16* s, int n0, int k0) {
   const int l = threadIdx.x & 31;
-  return s + (n0 + (l & 7) + (l >> 4) * 8) * LD + k0 + ((l >> 3) & 1) * 8;
+  return s + at<D>(n0 + (l & 7) + (l >> 4) * 8, k0 + ((l >> 3) & 1) * 8);
 }
-template <int LD>
+template <int D>
 __device__ __forceinline__ const bf16* frag_bk(const bf16* s, int n0, int k0) {
   const int l = threadIdx.x & 31;
-  return s + (k0 + (l & 7) + ((l >> 3) & 1) * 8) * LD + n0 + (l >> 4) * 8;
+  return s + at<D>(k0 + (l & 7) + ((l >> 3) & 1) * 8, n0 + (l >> 4) * 8);
 }
 
 // The warp's 16 x SC part of the state, float registers: acc[j] is columns
@@ -195,21 +210,24 @@ struct State {
         if (i < rows && j < cols) p[i * si + j * sj] = v;
       });
   }
-  __device__ __forceinline__ void publish(bf16* hi, bf16* lo) {
+  // as N bfloat16 terms, one D x D tile each
+  template <int N>
+  __device__ __forceinline__ void publish(bf16* out) {
     const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
 #pragma unroll
     for (int j = 0; j < Z::SC / 8; ++j)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        uint32_t h, l;
-        split2(s[j][2 * r], s[j][2 * r + 1], h, l);
-        const int o = (row0 + g + r * 8) * Z::LD + col0 + j * 8 + 2 * t;
-        *reinterpret_cast<uint32_t*>(hi + o) = h;
-        *reinterpret_cast<uint32_t*>(lo + o) = l;
+        uint32_t x[N];
+        split(s[j][2 * r], s[j][2 * r + 1], x);
+        const int o = at<D>(row0 + g + r * 8, col0 + j * 8) + 2 * t;
+#pragma unroll
+        for (int i = 0; i < N; ++i) *reinterpret_cast<uint32_t*>(out + i * Z::STATE + o) = x[i];
       }
   }
-  // s = keep s + sum over tokens of w(token) a_token b_token^T, tiles [token][.]
-  template <typename W>
+  // s = keep s + sum over tokens of w(token) a_token b_token^T, tiles [token][.];
+  // w a is split into N terms
+  template <int N, typename W>
   __device__ __forceinline__ void update(const bf16* a, const bf16* b, float keep, int n, W&& w) {
     const int t = threadIdx.x & 3;
 #pragma unroll
@@ -219,22 +237,26 @@ struct State {
     const int kt = (n + 15) / 16;
 #pragma unroll 1
     for (int k = 0; k < kt; ++k) {
-      uint32_t f[4], hi[4], lo[4];
-      ldsm_t(f, frag_at<Z::LD>(a, row0, k * 16));
+      uint32_t f[4], x[N][4];
+      ldsm_t(f, frag_at<D>(a, row0, k * 16));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int tok = k * 16 + 2 * t + (i >> 1) * 8;
-        const float2 x = unpack2(f[i]);
-        split2(x.x * w(tok), x.y * w(tok + 1), hi[i], lo[i]);
+        const float2 v = unpack2(f[i]);
+        uint32_t y[N];
+        split(v.x * w(tok), v.y * w(tok + 1), y);
+#pragma unroll
+        for (int m = 0; m < N; ++m) x[m][i] = y[m];
       }
 #pragma unroll
       for (int j = 0; j < Z::SC / 8; j += 2) {
         uint32_t r[4];
-        ldsm_t(r, frag_bk<Z::LD>(b, col0 + j * 8, k * 16));
-        mma(s[j], hi, r[0], r[1]);
-        mma(s[j], lo, r[0], r[1]);
-        mma(s[j + 1], hi, r[2], r[3]);
-        mma(s[j + 1], lo, r[2], r[3]);
+        ldsm_t(r, frag_bk<D>(b, col0 + j * 8, k * 16));
+#pragma unroll
+        for (int m = 0; m < N; ++m) {
+          mma(s[j], x[m], r[0], r[1]);
+          mma(s[j + 1], x[m], r[2], r[3]);
+        }
       }
     }
   }
@@ -250,8 +272,8 @@ __device__ __forceinline__ void store_rows(const float (&o)[Shape<D>::OC / 8][4]
   const int row0 = (warp & 3) * 16, col0 = (warp >> 2) * Z::OC;
 #pragma unroll
   for (int j = 0; j < Z::OC / 8; ++j) {
-    *reinterpret_cast<uint32_t*>(stg + (row0 + g) * Z::LD + col0 + j * 8 + 2 * t) = pack2(o[j][0], o[j][1]);
-    *reinterpret_cast<uint32_t*>(stg + (row0 + g + 8) * Z::LD + col0 + j * 8 + 2 * t) = pack2(o[j][2], o[j][3]);
+    *reinterpret_cast<uint32_t*>(stg + at<D>(row0 + g, col0 + j * 8) + 2 * t) = pack2(o[j][0], o[j][1]);
+    *reinterpret_cast<uint32_t*>(stg + at<D>(row0 + g + 8, col0 + j * 8) + 2 * t) = pack2(o[j][2], o[j][3]);
   }
   __syncwarp();
   bf16* base = row_ptr<bf16>(w, b, t0, h);
@@ -260,16 +282,15 @@ __device__ __forceinline__ void store_rows(const float (&o)[Shape<D>::OC / 8][4]
     const int r0 = row0 + lane / UPR, i = col0 + lane % UPR * 8, m = i < d ? n : 0;
     bf16* p = base + r0 * w.token + i;
     const int64_t step = kRows * w.token;
-    stg += r0 * Z::LD + i;
 #pragma unroll
     for (int r = 0; r < 16; r += kRows) {
-      if (r0 + r < m) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(stg + r * Z::LD);
+      if (r0 + r < m) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(stg + at<D>(r0 + r, i));
       p += step;
     }
   } else {
     for (int u = lane; u < 16 * Z::OC; u += 32) {
       const int r = row0 + u / Z::OC, i = col0 + u % Z::OC;
-      if (r < n && i < d) base[r * w.token + i] = stg[r * Z::LD + i];
+      if (r < n && i < d) base[r * w.token + i] = stg[at<D>(r, i)];
     }
   }
 }
@@ -303,20 +324,25 @@ struct FwdArgs {
   float scale;
 };
 
-template <int D>
+// What a pass computes: o, dq, or dq and its part of dlog d, whose products
+// with the state are taken to float accuracy.
+enum Pass { kOut = 0, kDq = 1, kDqLog = 2 };
+
+template <int D, int PASS>
 constexpr size_t fwd_smem() {
   using Z = Shape<D>;
-  return (size_t)(2 * 3 * Z::TILE + 2 * Z::STATE) * 2 + (C + 1 + 16) * 4;
+  return (size_t)(2 * 3 * Z::TILE + (PASS == kDqLog ? 3 : 2) * Z::STATE) * 2 + (C + 1 + 16) * 4;
 }
 
-template <int D, bool DQ>
+template <int D, int PASS>
 __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocks) fwd_kernel(const FwdArgs a) {
   using Z = Shape<D>;
+  constexpr bool DQ = PASS == kDqLog;
+  constexpr int NS = DQ ? 3 : 2;  // terms of the state in a product
   extern __shared__ __align__(16) char raw[];
   bf16* tiles = reinterpret_cast<bf16*>(raw);
-  bf16* s_hi = tiles + 2 * 3 * Z::TILE;
-  bf16* s_lo = s_hi + Z::STATE;
-  float* pw = reinterpret_cast<float*>(s_lo + Z::STATE);  // d^i
+  bf16* st = tiles + 2 * 3 * Z::TILE;
+  float* pw = reinterpret_cast<float*>(st + NS * Z::STATE);  // d^i
   float* red = pw + C + 1;
 
   const int h = blockIdx.x % a.H;
@@ -334,7 +360,7 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocks) fwd_kernel(co
   State<D> S;
   const float* s0 = a.nseg > 1 ? a.seg_state + (bh * a.nseg + seg) * elems : a.state_in ? a.state_in + bh * elems : nullptr;
   S.load(s0, a.e, a.f, a.si, a.sj);
-  S.publish(s_hi, s_lo);
+  S.template publish<NS>(st);
 
   auto load = [&](int i) {
     bf16* buf = tiles + (i & 1) * 3 * Z::TILE;
@@ -358,7 +384,7 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocks) fwd_kernel(co
     if (row0 < n) {
       uint32_t q[D / 16][4];
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) ldsm(q[k], frag_a<Z::LD>(sq, row0, k * 16));
+      for (int k = 0; k < D / 16; ++k) ldsm(q[k], frag_a<D>(sq, row0, k * 16));
       uint32_t x[DQ ? Z::OC / 4 : 1];  // the queries in the layout of o, on their way during the products
       if constexpr (DQ) {
 #pragma unroll
@@ -387,15 +413,14 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocks) fwd_kernel(co
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
 #pragma unroll
-          for (int j = 0; j < Z::OC / 8; j += 2) {
-            uint32_t r[4];
-            ldsm_t(r, frag_bk<Z::LD>(s_hi, col0 + j * 8, k * 16));
-            mma(o[j], q[k], r[0], r[1]);
-            mma(o[j + 1], q[k], r[2], r[3]);
-            ldsm_t(r, frag_bk<Z::LD>(s_lo, col0 + j * 8, k * 16));
-            mma(o[j], q[k], r[0], r[1]);
-            mma(o[j + 1], q[k], r[2], r[3]);
-          }
+          for (int j = 0; j < Z::OC / 8; j += 2)
+#pragma unroll
+            for (int m = 0; m < NS; ++m) {
+              uint32_t r[4];
+              ldsm_t(r, frag_bk<D>(st + m * Z::STATE, col0 + j * 8, k * 16));
+              mma(o[j], q[k], r[0], r[1]);
+              mma(o[j + 1], q[k], r[2], r[3]);
+            }
         const float d0 = pw[row0 + gr + 1], d1 = pw[row0 + gr + 9];
 #pragma unroll
         for (int j = 0; j < Z::OC / 8; ++j) o[j][0] *= d0, o[j][1] *= d0, o[j][2] *= d1, o[j][3] *= d1;
@@ -420,7 +445,7 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocks) fwd_kernel(co
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           uint32_t r[4];
-          ldsm(r, frag_bn<Z::LD>(sk, kt * 16, k * 16));
+          ldsm(r, frag_bn<D>(sk, kt * 16, k * 16));
           mma(s[0], q[k], r[0], r[1]);
           mma(s[1], q[k], r[2], r[3]);
         }
@@ -438,7 +463,7 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocks) fwd_kernel(co
 #pragma unroll
         for (int j = 0; j < Z::OC / 8; j += 2) {
           uint32_t r[4];
-          ldsm_t(r, frag_bk<Z::LD>(sv, col0 + j * 8, kt * 16));
+          ldsm_t(r, frag_bk<D>(sv, col0 + j * 8, kt * 16));
           mma(o[j], p, r[0], r[1]);
           mma(o[j + 1], p, r[2], r[3]);
         }
@@ -454,11 +479,12 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocks) fwd_kernel(co
     } else if (DQ && lane == 0) {
       red[warp] = 0.f, red[8 + warp] = 0.f;
     }
-    if (i + 1 < chunks || a.state_out)
-      S.update(sk, sv, pw[n], n, [&](int s) { return pw[max(n - 1 - s, 0)]; });
+    const auto w = [&](int s) { return pw[max(n - 1 - s, 0)]; };
+    // three terms for o as well, so that it does not depend on whether the state is asked for
+    if (i + 1 < chunks || a.state_out) S.template update<PASS == kDq ? 2 : 3>(sk, sv, pw[n], n, w);
     state_on = true;
     __syncthreads();
-    if (i + 1 < chunks) S.publish(s_hi, s_lo);
+    if (i + 1 < chunks) S.template publish<NS>(st);
     if constexpr (DQ) {
       if (threadIdx.x < 2) {
         float r = 0.f;
@@ -505,7 +531,7 @@ __global__ void __launch_bounds__(Shape<D>::NT) segment_kernel(const LinAttnArgs
     __syncthreads();
     const bf16* ta = tiles + (i & 1) * 2 * Z::TILE;
     const int c = REV ? chunks - 1 - i : i, n = min(C, len - c * C);
-    S.update(ta, ta + Z::TILE, pw[n], n, [&](int t) { return REV ? pw[min(t + 1, C)] * a.scale : pw[max(n - 1 - t, 0)]; });
+    S.template update<3>(ta, ta + Z::TILE, pw[n], n, [&](int t) { return REV ? pw[min(t + 1, C)] * a.scale : pw[max(n - 1 - t, 0)]; });
     __syncthreads();
   }
   cp_wait<0>();
@@ -541,22 +567,23 @@ struct DkvArgs {
   float* edge;  // [B][H][nseg]: <state before the segment's first token, its adjoint>, first segment only
 };
 
-template <int D>
+// LOG: with dlog d or dstate_in, so the adjoint state's products to float accuracy.
+template <int D, bool LOG>
 constexpr size_t dkv_smem() {
   using Z = Shape<D>;
-  return (size_t)(4 * Z::TILE + 2 * Z::STATE) * 2 + (C + 1 + 24) * 4;
+  return (size_t)(4 * Z::TILE + (LOG ? 3 : 1) * Z::STATE) * 2 + (C + 1 + 24) * 4;
 }
 
-template <int D>
+template <int D, bool LOG>
 __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocksDkv) dkv_kernel(const DkvArgs args) {
   using Z = Shape<D>;
+  constexpr int NS = LOG ? 3 : 1;  // terms of the adjoint state in dk's product; dv's takes the first
   const LinAttnArgs& a = args.a;
   extern __shared__ __align__(16) char raw[];
   bf16* sq = reinterpret_cast<bf16*>(raw);
   bf16 *sk = sq + Z::TILE, *sv = sk + Z::TILE, *sdo = sv + Z::TILE;
-  bf16* r_hi = sdo + Z::TILE;
-  bf16* r_lo = r_hi + Z::STATE;
-  float* pw = reinterpret_cast<float*>(r_lo + Z::STATE);
+  bf16* st = sdo + Z::TILE;
+  float* pw = reinterpret_cast<float*>(st + NS * Z::STATE);
   float* red = pw + C + 1;
 
   const int g = blockIdx.x % a.G;
@@ -579,7 +606,7 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocksDkv) dkv_kernel
     const float* r0 = a.nseg > 1 ? a.seg_dstate + (bh * a.nseg + seg) * elems
                                  : a.dstate_out ? a.dstate_out + bh * elems : nullptr;
     R.load(r0, a.dk, a.dv, a.dv, 1);
-    R.publish(r_hi, r_lo);
+    R.template publish<NS>(st);
     bool state_on = r0 != nullptr;
     for (int i = chunks - 1; i >= 0; --i) {
       const int t0 = begin + i * C, n = min(C, len - i * C);
@@ -601,37 +628,42 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocksDkv) dkv_kernel
 #pragma unroll 2
           for (int k = 0; k < D / 16; ++k) {
             uint32_t ka[4], va[4];
-            ldsm(ka, frag_a<Z::LD>(sk, row0, k * 16));
-            ldsm(va, frag_a<Z::LD>(sv, row0, k * 16));
+            ldsm(ka, frag_a<D>(sk, row0, k * 16));
+            ldsm(va, frag_a<D>(sv, row0, k * 16));
 #pragma unroll
             for (int j = 0; j < Z::OC / 8; j += 2) {
               uint32_t f[4];
-              ldsm_t(f, frag_bk<Z::LD>(r_hi, col0 + j * 8, k * 16));  // R[dk][dv]: dv_s = R^T k_s
+              ldsm_t(f, frag_bk<D>(st, col0 + j * 8, k * 16));  // R[dk][dv]: dv_s = R^T k_s
               mma(dv[j], ka, f[0], f[1]);
               mma(dv[j + 1], ka, f[2], f[3]);
-              ldsm(f, frag_bn<Z::LD>(r_hi, col0 + j * 8, k * 16));    // dk_s = R v_s
-              mma(dk[j], va, f[0], f[1]);
-              mma(dk[j + 1], va, f[2], f[3]);
-              ldsm(f, frag_bn<Z::LD>(r_lo, col0 + j * 8, k * 16));
-              mma(dk[j], va, f[0], f[1]);
-              mma(dk[j + 1], va, f[2], f[3]);
+#pragma unroll
+              for (int m = 0; m < NS; ++m) {
+                ldsm(f, frag_bn<D>(st + m * Z::STATE, col0 + j * 8, k * 16));  // dk_s = R v_s
+                mma(dk[j], va, f[0], f[1]);
+                mma(dk[j + 1], va, f[2], f[3]);
+              }
             }
           }
           const int s0 = row0 + gr, s1 = s0 + 8;
           const float d0 = pw[max(n - 1 - s0, 0)], d1 = pw[max(n - 1 - s1, 0)];
-          float p0 = 0.f, p1 = 0.f;
 #pragma unroll
           for (int j = 0; j < Z::OC / 8; ++j) {
             dv[j][0] *= d0, dv[j][1] *= d0, dv[j][2] *= d1, dv[j][3] *= d1;
             dk[j][0] *= d0, dk[j][1] *= d0, dk[j][2] *= d1, dk[j][3] *= d1;
-            const int c = col0 + j * 8 + 2 * tq;
-            const float2 k0 = unpack2(*reinterpret_cast<const uint32_t*>(sk + s0 * Z::LD + c));
-            const float2 k1 = unpack2(*reinterpret_cast<const uint32_t*>(sk + s1 * Z::LD + c));
-            p0 = fmaf(k0.x, dk[j][0], fmaf(k0.y, dk[j][1], p0));
-            p1 = fmaf(k1.x, dk[j][2], fmaf(k1.y, dk[j][3], p1));
           }
-          ksum = p0 + p1;
-          kwsum = p0 * (float)(n - 1 - s0) + p1 * (float)(n - 1 - s1);
+          if constexpr (LOG) {
+            float p0 = 0.f, p1 = 0.f;
+#pragma unroll
+            for (int j = 0; j < Z::OC / 8; ++j) {
+              const int c = col0 + j * 8 + 2 * tq;
+              const float2 k0 = unpack2(*reinterpret_cast<const uint32_t*>(sk + at<D>(s0, c)));
+              const float2 k1 = unpack2(*reinterpret_cast<const uint32_t*>(sk + at<D>(s1, c)));
+              p0 = fmaf(k0.x, dk[j][0], fmaf(k0.y, dk[j][1], p0));
+              p1 = fmaf(k1.x, dk[j][2], fmaf(k1.y, dk[j][3], p1));
+            }
+            ksum = p0 + p1;
+            kwsum = p0 * (float)(n - 1 - s0) + p1 * (float)(n - 1 - s1);
+          }
         }
         // scores of the warp's 16 keys against 16 queries at a time, from its own on
 #pragma unroll 1
@@ -640,12 +672,12 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocksDkv) dkv_kernel
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             uint32_t fa[4], f[4];
-            ldsm(fa, frag_a<Z::LD>(sk, row0, k * 16));
-            ldsm(f, frag_bn<Z::LD>(sq, kt * 16, k * 16));
+            ldsm(fa, frag_a<D>(sk, row0, k * 16));
+            ldsm(f, frag_bn<D>(sq, kt * 16, k * 16));
             mma(s1[0], fa, f[0], f[1]);
             mma(s1[1], fa, f[2], f[3]);
-            ldsm(fa, frag_a<Z::LD>(sv, row0, k * 16));
-            ldsm(f, frag_bn<Z::LD>(sdo, kt * 16, k * 16));
+            ldsm(fa, frag_a<D>(sv, row0, k * 16));
+            ldsm(f, frag_bn<D>(sdo, kt * 16, k * 16));
             mma(s2[0], fa, f[0], f[1]);
             mma(s2[1], fa, f[2], f[3]);
           }
@@ -657,7 +689,7 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocksDkv) dkv_kernel
               const int lag = kt * 16 + c * 8 + 2 * tq + (e & 1) - (row0 + gr + (e >> 1) * 8);
               const float w = lag >= 0 ? pw[max(lag, 0)] * a.scale : 0.f;
               s1[c][e] *= w;
-              if (col0 == 0) intra = fmaf((float)lag * s1[c][e], s2[c][e], intra);
+              if (LOG && col0 == 0) intra = fmaf((float)lag * s1[c][e], s2[c][e], intra);
               s2[c][e] *= w;
             }
             p1[2 * c] = pack2(s1[c][0], s1[c][1]), p1[2 * c + 1] = pack2(s1[c][2], s1[c][3]);
@@ -666,23 +698,23 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocksDkv) dkv_kernel
 #pragma unroll
           for (int j = 0; j < Z::OC / 8; j += 2) {
             uint32_t f[4];
-            ldsm_t(f, frag_bk<Z::LD>(sdo, col0 + j * 8, kt * 16));
+            ldsm_t(f, frag_bk<D>(sdo, col0 + j * 8, kt * 16));
             mma(dv[j], p1, f[0], f[1]);
             mma(dv[j + 1], p1, f[2], f[3]);
-            ldsm_t(f, frag_bk<Z::LD>(sq, col0 + j * 8, kt * 16));
+            ldsm_t(f, frag_bk<D>(sq, col0 + j * 8, kt * 16));
             mma(dk[j], p2, f[0], f[1]);
             mma(dk[j + 1], p2, f[2], f[3]);
           }
         }
       }
-      intra = warp_sum(intra), ksum = warp_sum(ksum), kwsum = warp_sum(kwsum);
-      if (lane == 0) red[warp] = intra, red[8 + warp] = ksum, red[16 + warp] = kwsum;
+      if constexpr (LOG) intra = warp_sum(intra), ksum = warp_sum(ksum), kwsum = warp_sum(kwsum);
+      if (LOG && lane == 0) red[warp] = intra, red[8 + warp] = ksum, red[16 + warp] = kwsum;
       if (i > 0 || a.dstate_in || args.edge)
-        R.update(sq, sdo, pw[n], n, [&](int t) { return pw[min(t + 1, C)] * a.scale; });
+        R.template update<LOG ? 3 : 2>(sq, sdo, pw[n], n, [&](int t) { return pw[min(t + 1, C)] * a.scale; });
       state_on = true;
       __syncthreads();
-      if (i > 0) R.publish(r_hi, r_lo);
-      if (threadIdx.x < 3) {
+      if (i > 0) R.template publish<NS>(st);
+      if (LOG && threadIdx.x < 3) {
         float s = 0.f;
         for (int w = 0; w < Z::NW; ++w) s += red[threadIdx.x * 8 + w];
         args.part[(bh * all_chunks + seg * (a.seg_len / C) + i) * 3 + threadIdx.x] = s;
@@ -788,14 +820,14 @@ int run_segments(const LinAttnArgs& a, const TmpcLinAttnDims* d, float* seg, con
   return (int)cudaPeekAtLastError();
 }
 
-template <bool DQ>
+template <int PASS>
 int run_fwd(const FwdArgs& f, const LinAttnArgs& a, const TmpcLinAttnDims* d, cudaStream_t st) {
   int rc = 0;
   by_size(d, [&](auto dd) {
     constexpr int D = decltype(dd)::value;
-    rc = allow_smem<fwd_kernel<D, DQ>>((int)fwd_smem<D>());
+    rc = allow_smem<fwd_kernel<D, PASS>>((int)fwd_smem<D, PASS>());
     if (!rc)
-      fwd_kernel<D, DQ><<<(unsigned)((int64_t)a.B * a.nseg * a.H), Shape<D>::NT, fwd_smem<D>(), st>>>(f);
+      fwd_kernel<D, PASS><<<(unsigned)((int64_t)a.B * a.nseg * a.H), Shape<D>::NT, fwd_smem<D, PASS>(), st>>>(f);
   });
   return rc ? rc : (int)cudaPeekAtLastError();
 }
@@ -855,7 +887,7 @@ int LinAttn<bf16>::forward(LinAttnArgs a, const TmpcLinAttnDims* d, char* ws, cu
   }
   const la::FwdArgs f{a.q, a.k, a.v, a.o, a.o, a.log_decay, a.lengths, a.state_in, a.state_out, seg, nullptr,
                       a.T, a.H, a.G, a.dk, a.dv, a.dv, 1, a.nseg, a.seg_len, a.vec, a.scale};
-  return la::run_fwd<false>(f, a, d, st);
+  return la::run_fwd<la::kOut>(f, a, d, st);
 }
 
 template <>
@@ -883,14 +915,20 @@ int LinAttn<bf16>::backward(LinAttnArgs a, const TmpcLinAttnDims* d, float* dlog
   // dq: the forward sum over (do, v, k) with the transposed state
   const la::FwdArgs f{a.o, a.v, a.k, a.gq, a.q, a.log_decay, a.lengths, a.state_in, nullptr, a.seg_state, at(p.pq),
                       a.T, a.H, a.G, a.dv, a.dk, 1, a.dv, a.nseg, a.seg_len, a.vec, a.scale};
-  int rc = la::run_fwd<true>(f, a, d, st);
+  int rc = dlog_decay ? la::run_fwd<la::kDqLog>(f, a, d, st) : la::run_fwd<la::kDq>(f, a, d, st);
   if (rc) return rc;
   const la::DkvArgs k{a, at(p.pk), dlog_decay ? at(p.edge) : nullptr};
   by_size(d, [&](auto dd) {
     constexpr int D = decltype(dd)::value;
-    rc = allow_smem<la::dkv_kernel<D>>((int)la::dkv_smem<D>());
-    if (!rc)
-      la::dkv_kernel<D><<<(unsigned)((int64_t)a.B * a.nseg * a.G), la::Shape<D>::NT, la::dkv_smem<D>(), st>>>(k);
+    auto run = [&](auto log) {
+      constexpr bool LOG = decltype(log)::value;
+      rc = allow_smem<la::dkv_kernel<D, LOG>>((int)la::dkv_smem<D, LOG>());
+      if (!rc)
+        la::dkv_kernel<D, LOG><<<(unsigned)((int64_t)a.B * a.nseg * a.G), la::Shape<D>::NT, la::dkv_smem<D, LOG>(),
+                                 st>>>(k);
+    };
+    if (dlog_decay || a.dstate_in) run(std::true_type{});
+    else run(std::false_type{});
   });
   if (rc) return rc;
   if (dlog_decay) la::dlog_kernel<<<a.H, 256, 0, st>>>(a, at(p.pq), at(p.pk), at(p.edge), dlog_decay);

@@ -1,14 +1,23 @@
-// Linear attention with a decay per head, token by token: forward, backward.
+// Linear attention with a decay per head: the entry points, and the float
+// kernel, token by token.
 //
-//   S_t = d S_{t-1} + k_t v_t^T,   o_t = s S_t^T q_t
-//   dS_t = d dS_{t+1} + s q_t do_t^T,   dq_t = s S_t do_t,
-//   dk_t = dS_t v_t,   dv_t = dS_t^T k_t
-//   dlog d = sum_t <dS_t, d S_{t-1}>
+// One pass computes, forward or backward in time,
+//     S_t = d S_{t-1} + b_t c_t^T,   out_t = S_t^T a_t
+// which is o for (a, b, c) = (q, k, v), dq for (do, v, k) and the transposed
+// state, and, run backward, dv for (k, q, do) and dk for (v, do, q).  With
+// M_t = dS_t / dlog d = d (M_{t-1} + S_{t-1}) carried beside S in the dq pass,
+//     dlog d = sum_t scale q_t^T M_t do_t + <dS_L, M_L>
+// has no cancelling terms.
 //
-// The state lives in registers: a thread owns a column of S (forward, dv) or
-// a row (dq, dk).  dlog d needs no product of S and dS inside the sequence:
-// with q' = d^(t+1) q and k' = d^-(t+1) k the decay leaves every o_t, and
-//   dlog d = sum_t (t+1) (q_t . dq_t - k_t . dk_t) + L <S_L, dS_L>.
+// Bound by the float units: 2 operations per state element and token.  A thread
+// keeps 8 x 4 elements of S; a token costs it 5 shared-memory loads and 64
+// multiply-adds.  The decay is taken out of the inner loop: within 16 tokens
+// the state is held as d^-u S, with a and b scaled by d^u and d^-u as they are
+// staged; where d^-16 could overflow (d < 2^-6) the state is rescaled at every
+// token instead.  The read-outs of four tokens are summed over the lanes that
+// share a column group together, each lane keeping its share.
+#include <type_traits>
+
 #include "seq_attention.cuh"
 
 namespace tmpc {
@@ -16,213 +25,390 @@ namespace seq {
 namespace rec {
 
 constexpr int kTile = 16;  // tokens staged in shared memory at a time
-constexpr int kCols = 128;
 
-// Tokens t0 .. t0 + n - 1 of one head into a [kTile][LD] tile, zero-padded.
-template <typename T, int LD>
-__device__ __forceinline__ void stage(float (*s)[LD], const TmpcSeqView& w, int b, int t0, int n, int h, int d) {
-  for (int e = threadIdx.x; e < kTile * LD; e += blockDim.x) {
-    const int t = e / LD, i = e % LD;
-    s[t][i] = (t < n && i < d) ? to_f(row_ptr<T>(w, b, t0 + t, h)[i]) : 0.f;
-  }
-}
+struct Args {
+  TmpcSeqView a, b, c, o, x;  // x (LOG): q, against the read-out of M
+  bool a_key, b_key, c_key;   // indexed by the key head instead of the query head
+  const float* log_decay;
+  const int32_t* lengths;
+  const float* state_in;      // element (i, j) of a head's state at i si + j sj
+  float* state_out;
+  const float* seg_state;     // [B][H][nseg]; with OUT off: where to leave a segment's own state
+  const float* seg_m;         // LOG: the same for M
+  const float* dstate_out;    // LOG
+  float* dlog;                // LOG: [B][H][nseg]
+  int64_t units;              // B * heads * nseg
+  int T, H, G, rep, e, f, si, sj, nseg, seg_len;  // rep: query heads per unit (dk, dv), else 1
+  bool vec;
+  float a_scale, b_scale;
+};
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kCols) fwd_kernel(const LinAttnArgs a) {
-  __shared__ __align__(16) float sq[kTile][D], sk[kTile][D];
-  const int h = blockIdx.y, b = blockIdx.x, g = h / (a.H / a.G), j = threadIdx.x;
-  const float dec = exp2f(log2_decay(a.log_decay, h));
-  const int len = seq_len(a, b);
-  const size_t so = ((size_t)b * a.H + h) * a.dk * a.dv;
-  float S[D];
+template <int D>
+struct Shape {
+  static constexpr int NW = D * D / 1024;               // warps per state
+  static constexpr int UNITS = NW >= 4 ? 1 : 4 / NW;    // states per block
+  static constexpr int NT = NW * 32;                    // threads per state
+  static constexpr int BLOCK = NT * UNITS;
+  static constexpr int RG = D / 8;                      // lanes that share a column group
+};
+
+template <int D, bool REV, bool LOG, bool OUT>
+__global__ void __launch_bounds__(Shape<D>::BLOCK) pass_kernel(const Args p) {
+  using Z = Shape<D>;
+  __shared__ __align__(16) float smem[Z::UNITS][LOG ? 4 : 3][kTile][D];
+  const int sub = threadIdx.x / Z::NT, tid = threadIdx.x % Z::NT, lane = threadIdx.x & 31;
+  const int64_t unit = (int64_t)blockIdx.x * Z::UNITS + sub;
+  if (unit >= p.units) return;  // whole warps; a block of several states has no block-wide barrier
+  auto sync = [&] {
+    if constexpr (Z::UNITS > 1) __syncwarp();
+    else __syncthreads();
+  };
+  float(*sa)[D] = smem[sub][0], (*sb)[D] = smem[sub][1], (*sc)[D] = smem[sub][2], (*sx)[D] = smem[sub][LOG ? 3 : 0];
+  const int heads = p.H / p.rep;
+  const int hu = (int)(unit % heads), seg = (int)(unit / heads % p.nseg);
+  const int b = (int)(unit / heads / p.nseg);
+  int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+  const int begin = seg * p.seg_len, stop = min(begin + p.seg_len, p.T);
+  len = min(max(len - begin, 0), stop - begin);
+  const int rg = lane % Z::RG, cg = (tid / 32) * (32 / Z::RG) + lane / Z::RG, j0 = cg * 4;
+  const int64_t elems = (int64_t)p.e * p.f;
+  auto row_of = [&](int r) { return (r >> 2) * (D / 2) + rg * 4 + (r & 3); };  // r = 0 .. 7
+
+  for (int r0 = 0; r0 < p.rep; ++r0) {
+    const int h = hu * p.rep + r0, g = h / (p.H / p.G);
+    const int64_t bh = (int64_t)b * p.H + h;
+    const float g2 = log2_decay(p.log_decay, h);
+    const int rn = g2 < -6.f ? 1 : kTile;  // tokens between rescalings of the state
+    float S[8][4], M[LOG ? 8 : 1][4], dlog = 0.f;
+    const float* s0 = !OUT ? nullptr
+                      : p.nseg > 1 ? p.seg_state + (bh * p.nseg + seg) * elems
+                      : p.state_in ? p.state_in + bh * elems : nullptr;
+    const float* m0 = LOG && OUT && p.nseg > 1 ? p.seg_m + (bh * p.nseg + seg) * elems : nullptr;
 #pragma unroll
-  for (int i = 0; i < D; ++i) S[i] = (a.state_in && i < a.dk && j < a.dv) ? a.state_in[so + (size_t)i * a.dv + j] : 0.f;
-  for (int t0 = 0; t0 < len; t0 += kTile) {
-    const int n = min(kTile, len - t0);
-    __syncthreads();
-    stage<T, D>(sq, a.q, b, t0, n, h, a.dk);
-    stage<T, D>(sk, a.k, b, t0, n, g, a.dk);
-    __syncthreads();
-    for (int t = 0; t < n; ++t) {
-      const float v = j < a.dv ? to_f(row_ptr<T>(a.v, b, t0 + t, g)[j]) : 0.f;
-      float o = 0.f;
+    for (int r = 0; r < 8; ++r)
 #pragma unroll
-      for (int i = 0; i < D; ++i) {
-        S[i] = fmaf(dec, S[i], sk[t][i] * v);
-        o = fmaf(sq[t][i], S[i], o);
+      for (int c = 0; c < 4; ++c) {
+        const int i = row_of(r), j = j0 + c;
+        const bool on = i < p.e && j < p.f;
+        S[r][c] = s0 && on ? s0[i * p.si + j * p.sj] : 0.f;
+        if constexpr (LOG) M[r][c] = m0 && on ? m0[i * p.si + j * p.sj] : 0.f;
       }
-      if (j < a.dv) (row_ptr<T>(a.o, b, t0 + t, h))[j] = from_f<T>(o * a.scale);
-    }
-  }
-  if (j < a.dv)
-    for (int t = len; t < a.T; ++t) (row_ptr<T>(a.o, b, t, h))[j] = from_f<T>(0.f);
-  if (a.state_out && j < a.dv) {
-#pragma unroll
-    for (int i = 0; i < D; ++i)
-      if (i < a.dk) a.state_out[so + (size_t)i * a.dv + j] = S[i];
-  }
-}
+    int pending = REV ? 0 : 1;  // powers of d due on S before the next token; afterwards the tokens since a rescaling
 
-__device__ __forceinline__ double block_sum(double v, double* red) {
+    // a tile's rows in registers, one tile ahead
+    constexpr int NV = kTile * D / 4 / Z::NT, NTEN = LOG ? 4 : 3;
+    float4 next[NTEN][NV];
+    auto fetch = [&](int u0) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0;
-  for (int i = 0; i < (int)blockDim.x / 32; ++i) v += red[i];
-  return v;
-}
-
-// dq: thread i owns row i of S.
-template <typename T, int D>
-__global__ void __launch_bounds__(kCols) dq_kernel(const LinAttnArgs a) {
-  __shared__ __align__(16) float sv[kTile][D], sdo[kTile][D];
-  __shared__ double red[4];
-  const int h = blockIdx.y, b = blockIdx.x, g = h / (a.H / a.G), i = threadIdx.x;
-  const float dec = exp2f(log2_decay(a.log_decay, h));
-  const int len = seq_len(a, b);
-  const size_t so = ((size_t)b * a.H + h) * a.dk * a.dv;
-  float S[D];
+      for (int w = 0; w < NTEN; ++w) {
+        const TmpcSeqView& v = w == 0 ? p.a : w == 1 ? p.b : w == 2 ? p.c : p.x;
+        const int head = w == 0 ? (p.a_key ? g : h) : w == 1 ? (p.b_key ? g : h) : w == 2 ? (p.c_key ? g : h) : h;
+        const int d = w < 2 ? p.e : p.f;
 #pragma unroll
-  for (int j = 0; j < D; ++j) S[j] = (a.state_in && i < a.dk && j < a.dv) ? a.state_in[so + (size_t)i * a.dv + j] : 0.f;
-  double dl = 0;
-  for (int t0 = 0; t0 < len; t0 += kTile) {
-    const int n = min(kTile, len - t0);
-    __syncthreads();
-    stage<T, D>(sv, a.v, b, t0, n, g, a.dv);
-    stage<T, D>(sdo, a.o, b, t0, n, h, a.dv);
-    __syncthreads();
-    for (int t = 0; t < n; ++t) {
-      const float k = i < a.dk ? to_f(row_ptr<T>(a.k, b, t0 + t, g)[i]) : 0.f;
-      const float q = i < a.dk ? to_f(row_ptr<T>(a.q, b, t0 + t, h)[i]) : 0.f;
-      float dq = 0.f;
-#pragma unroll
-      for (int j = 0; j < D; ++j) {
-        S[j] = fmaf(dec, S[j], sv[t][j] * k);
-        dq = fmaf(sdo[t][j], S[j], dq);
-      }
-      dq *= a.scale;
-      dl += (double)(t0 + t + 1) * (double)(q * dq);
-      if (i < a.dk) (row_ptr<T>(a.gq, b, t0 + t, h))[i] = from_f<T>(dq);
-    }
-  }
-  if (i < a.dk)
-    for (int t = len; t < a.T; ++t) (row_ptr<T>(a.gq, b, t, h))[i] = from_f<T>(0.f);
-  if (a.dstate_out && i < a.dk) {
-    float e = 0.f;
-#pragma unroll
-    for (int j = 0; j < D; ++j)
-      if (j < a.dv) e = fmaf(S[j], a.dstate_out[so + (size_t)i * a.dv + j], e);
-    dl += (double)len * (double)e;
-  }
-  dl = block_sum(dl, red);
-  if (a.dlog && i == 0) reinterpret_cast<double*>(a.dlog)[(size_t)b * a.H + h] = dl;
-}
-
-// dk, dv: threads 0 .. 127 own a row of dS, threads 128 .. 255 a column.
-template <typename T, int D>
-__global__ void __launch_bounds__(2 * kCols) dkv_kernel(const LinAttnArgs a) {
-  __shared__ __align__(16) float sq[kTile][D], sk[kTile][D], sv[kTile][D], sdo[kTile][D];
-  __shared__ double red[8];
-  const int g = blockIdx.y, b = blockIdx.x, rep = a.H / a.G;
-  const bool is_row = threadIdx.x < kCols;
-  const int i = threadIdx.x % kCols;
-  const int mine = is_row ? a.dk : a.dv, other = is_row ? a.dv : a.dk;
-  const int len = seq_len(a, b);
-  for (int r = 0; r < rep; ++r) {
-    const int h = g * rep + r;
-    const float dec = exp2f(log2_decay(a.log_decay, h));
-    const size_t so = ((size_t)b * a.H + h) * a.dk * a.dv;
-    const size_t s_own = is_row ? (size_t)i * a.dv : i, s_step = is_row ? 1 : a.dv;
-    float dS[D];
-#pragma unroll
-    for (int j = 0; j < D; ++j)
-      dS[j] = (a.dstate_out && i < mine && j < other) ? a.dstate_out[so + s_own + j * s_step] : 0.f;
-    double dl = 0;
-    for (int t0 = (len - 1) / kTile * kTile; len > 0 && t0 >= 0; t0 -= kTile) {
-      const int n = min(kTile, len - t0);
-      __syncthreads();
-      stage<T, D>(sq, a.q, b, t0, n, h, a.dk);
-      stage<T, D>(sk, a.k, b, t0, n, g, a.dk);
-      stage<T, D>(sv, a.v, b, t0, n, g, a.dv);
-      stage<T, D>(sdo, a.o, b, t0, n, h, a.dv);
-      __syncthreads();
-      for (int t = n - 1; t >= 0; --t) {
-        const float* outer = is_row ? sdo[t] : sq[t];
-        const float* inner = is_row ? sv[t] : sk[t];
-        const float x = (i < mine ? (is_row ? sq[t][i] : sdo[t][i]) : 0.f) * a.scale;
-        float y = 0.f;
-#pragma unroll
-        for (int j = 0; j < D; ++j) {
-          dS[j] = fmaf(outer[j], x, dS[j]);
-          y = fmaf(dS[j], inner[j], y);
-          dS[j] *= dec;
-        }
-        if (is_row && i < mine) dl -= (double)(t0 + t + 1) * (double)(sk[t][i] * y);
-        if (i < mine) {
-          float* acc = a.acc + (((size_t)b * a.T + t0 + t) * a.G + g) * (a.dk + a.dv) + (is_row ? 0 : a.dk) + i;
-          if (r > 0) y += *acc;
-          if (r + 1 < rep) *acc = y;
-          else (row_ptr<T>(is_row ? a.gk : a.gv, b, t0 + t, g))[i] = from_f<T>(y);
+        for (int n = 0; n < NV; ++n) {
+          const int idx = tid + n * Z::NT, u = u0 + idx / (D / 4), i = idx % (D / 4) * 4;
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (u < len && i < d) {
+            const float* src = row_ptr<float>(v, b, begin + (REV ? len - 1 - u : u), head) + i;
+            if (p.vec) {
+              x = *reinterpret_cast<const float4*>(src);
+            } else {
+              x.x = src[0];
+              if (i + 1 < d) x.y = src[1];
+              if (i + 2 < d) x.z = src[2];
+              if (i + 3 < d) x.w = src[3];
+            }
+          }
+          next[w][n] = x;
         }
       }
-    }
-    if (a.dstate_in && is_row && i < a.dk) {
+    };
+    if (len > 0) fetch(0);
+    for (int u0 = 0; u0 < len; u0 += kTile) {
+      sync();  // the last tile has been read
 #pragma unroll
-      for (int j = 0; j < D; ++j)
-        if (j < a.dv) a.dstate_in[so + (size_t)i * a.dv + j] = dS[j];
+      for (int n = 0; n < NV; ++n) {
+        const int idx = tid + n * Z::NT, u = idx / (D / 4), i = idx % (D / 4) * 4;
+        const float pw = rn == 1 ? 1.f : exp2f(g2 * (float)u);
+        const float fa = pw * p.a_scale, fb = p.b_scale / pw;
+        const float4 x = next[0][n], y = next[1][n];
+        *reinterpret_cast<float4*>(&sa[u][i]) = make_float4(x.x * fa, x.y * fa, x.z * fa, x.w * fa);
+        *reinterpret_cast<float4*>(&sb[u][i]) = make_float4(y.x * fb, y.y * fb, y.z * fb, y.w * fb);
+        *reinterpret_cast<float4*>(&sc[u][i]) = next[2][n];
+        if constexpr (LOG) *reinterpret_cast<float4*>(&sx[u][i]) = next[3][n];
+      }
+      sync();
+      if (u0 + kTile < len) fetch(u0 + kTile);
+      const int m = min(kTile, len - u0);
+#pragma unroll 1
+      for (int v0 = 0; v0 < m; v0 += 4) {
+        float o[4][4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int u = v0 + q;  // rows past m are zero: they leave the state alone
+          if (u < m && (rn == 1 || u == 0)) {
+            const float w = exp2f(g2 * (float)pending);
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                if constexpr (LOG) M[r][c] = (M[r][c] + S[r][c]) * w;
+                S[r][c] *= w;
+              }
+            pending = 0;
+          } else if (LOG && u < m) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) M[LOG ? r : 0][c] += S[r][c];
+          }
+          if (u < m) ++pending;
+          float av[8], bv[8];
+          *reinterpret_cast<float4*>(av) = *reinterpret_cast<const float4*>(&sa[u][rg * 4]);
+          *reinterpret_cast<float4*>(av + 4) = *reinterpret_cast<const float4*>(&sa[u][D / 2 + rg * 4]);
+          *reinterpret_cast<float4*>(bv) = *reinterpret_cast<const float4*>(&sb[u][rg * 4]);
+          *reinterpret_cast<float4*>(bv + 4) = *reinterpret_cast<const float4*>(&sb[u][D / 2 + rg * 4]);
+          const float4 cv = *reinterpret_cast<const float4*>(&sc[u][j0]);
+          const float cc[4] = {cv.x, cv.y, cv.z, cv.w};
+          float xm[4] = {};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float acc = 0.f;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+              S[r][c] = fmaf(bv[r], cc[c], S[r][c]);
+              if constexpr (OUT) acc = fmaf(av[r], S[r][c], acc);
+              if constexpr (LOG && OUT) xm[c] = fmaf(av[r], M[r][c], xm[c]);
+            }
+            o[q][c] = acc;
+          }
+          if constexpr (LOG && OUT) {
+            const float4 xv = *reinterpret_cast<const float4*>(&sx[u][j0]);
+            dlog += xm[0] * xv.x + xm[1] * xv.y + xm[2] * xv.z + xm[3] * xv.w;
+          }
+        }
+        if constexpr (OUT) {
+          // 16 sums over the RG lanes: halve the values and the lanes together
+          float* x = &o[0][0];
+          int have = 16, first = 0;
+#pragma unroll
+          for (int bit = Z::RG / 2; bit > 0; bit >>= 1) {
+            have /= 2;
+            const bool up = rg & bit;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (i < have) {
+                const float give = up ? x[i] : x[i + have], keep = up ? x[i + have] : x[i];
+                x[i] = keep + __shfl_xor_sync(0xffffffffu, give, bit);
+              }
+            if (up) first += have;
+          }
+          constexpr int KEEP = 16 / Z::RG;  // values of this lane: token first / 4, columns j0 + first % 4 ..
+          const int u = u0 + v0 + first / 4, j = j0 + first % 4;
+          if (u < len && j < p.f) {
+            float* dst = row_ptr<float>(p.o, b, begin + (REV ? len - 1 - u : u), REV ? g : h) + j;
+            if (KEEP == 4 && p.vec) {
+              float4 v = make_float4(x[0], x[1], x[2], x[3]);
+              if (r0 > 0) {
+                const float4 w = *reinterpret_cast<float4*>(dst);
+                v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+              }
+              *reinterpret_cast<float4*>(dst) = v;
+            } else {
+#pragma unroll
+              for (int i = 0; i < KEEP; ++i)
+                if (j + i < p.f) dst[i] = r0 > 0 ? dst[i] + x[i] : x[i];
+            }
+          }
+        }
+      }
     }
-    dl = block_sum(dl, red);
-    if (a.dlog && threadIdx.x == 0) reinterpret_cast<double*>(a.dlog)[((size_t)gridDim.x + b) * a.H + h] = dl;
+    // the state after the last token (forward), or the adjoint before the first (backward)
+    const float w = exp2f(g2 * (float)(REV ? pending : pending - 1));
+    float* out = !OUT ? const_cast<float*>(p.seg_state) + (bh * p.nseg + seg) * elems
+                 : p.state_out && seg == (REV ? 0 : p.nseg - 1) ? p.state_out + bh * elems : nullptr;
+    float* mout = !OUT && LOG ? const_cast<float*>(p.seg_m) + (bh * p.nseg + seg) * elems : nullptr;
+    const float* dso = LOG && OUT && p.dstate_out && seg == p.nseg - 1 ? p.dstate_out + bh * elems : nullptr;
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int i = row_of(r), j = j0 + c;
+        if (i < p.e && j < p.f) {
+          if (out) out[i * p.si + j * p.sj] = S[r][c] * w;
+          if constexpr (LOG) {
+            if (mout) mout[i * p.si + j * p.sj] = M[r][c] * w;
+            if (dso) dlog = fmaf(M[r][c] * w, dso[i * p.si + j * p.sj], dlog);
+          }
+        }
+      }
+    if constexpr (LOG && OUT) {
+      dlog = warp_sum(dlog);
+      if constexpr (Z::NW > 1) {
+        sync();
+        if (lane == 0) sa[0][tid / 32] = dlog;
+        sync();
+        dlog = 0.f;
+        for (int i = 0; i < Z::NW; ++i) dlog += sa[0][i];
+      }
+      if (tid == 0) p.dlog[bh * p.nseg + seg] = dlog;
+    }
   }
-  if (i < mine)
-    for (int t = len; t < a.T; ++t)
-      (row_ptr<T>(is_row ? a.gk : a.gv, b, t, g))[i] = from_f<T>(0.f);
+  if constexpr (OUT) {  // rows past the length
+    // a unit is a query head (o, dq) or a key head (dk, dv): hu is the output's own head
+    for (int t = begin + len; t < stop; ++t)
+      for (int i = tid; i < p.f; i += Z::NT) row_ptr<float>(p.o, b, t, hu)[i] = 0.f;
+  }
 }
 
-__global__ void dlog_kernel(const double* part, float* out, int n, int H) {
+// In place: what each segment leaves alone -> the state (and M) before each
+// segment, or (REV) the adjoint after each.
+template <bool REV, bool LOG>
+__global__ void __launch_bounds__(256) scan_kernel(const Args p, float* seg, float* segm, const float* first) {
+  const int64_t elems = (int64_t)p.e * p.f, bh = blockIdx.y;
+  const int b = (int)(bh / p.H), h = (int)(bh % p.H);
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= elems) return;
+  const int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+  const float g2 = log2_decay(p.log_decay, h);
+  float s = first ? first[bh * elems + i] : 0.f, m = 0.f;
+  for (int k = 0; k < p.nseg; ++k) {
+    const int q = REV ? p.nseg - 1 - k : k;
+    const int64_t at = (bh * p.nseg + q) * elems + i;
+    const int n = min(max(len - q * p.seg_len, 0), p.seg_len);
+    const float w = exp2f(g2 * (float)n), own = seg[at];
+    seg[at] = s;
+    if constexpr (LOG) {
+      const float own_m = segm[at];
+      segm[at] = m;
+      m = fmaf(w, fmaf((float)n, s, m), own_m);
+    }
+    s = fmaf(w, s, own);
+  }
+}
+
+__global__ void __launch_bounds__(128) dlog_kernel(const float* part, float* out, int B, int H, int nseg) {
   __shared__ double red[4];
   const int h = blockIdx.x;
   double s = 0;
-  for (int b = threadIdx.x; b < n; b += blockDim.x) s += part[(size_t)b * H + h];
-  s = block_sum(s, red);
-  if (threadIdx.x == 0) out[h] = (float)s;
+  for (int64_t i = threadIdx.x; i < (int64_t)B * nseg; i += 128)
+    s += part[((i / nseg) * H + h) * nseg + i % nseg];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) out[h] = (float)(red[0] + red[1] + red[2] + red[3]);
+}
+
+template <bool REV, bool LOG, bool OUT>
+int run(Args p, const TmpcLinAttnDims* d, cudaStream_t st) {
+  by_size(d, [&](auto dd) {
+    constexpr int D = decltype(dd)::value;
+    using Z = Shape<D>;
+    p.units = (int64_t)d->B * (p.H / p.rep) * p.nseg;
+    pass_kernel<D, REV, LOG, OUT><<<(unsigned)((p.units + Z::UNITS - 1) / Z::UNITS), Z::BLOCK, 0, st>>>(p);
+  });
+  return (int)cudaPeekAtLastError();
+}
+
+// One pass; a long sequence in segments: each one's own state first, then the
+// states before them, then the pass over all segments side by side.
+template <bool REV, bool LOG>
+int pass(Args p, const TmpcLinAttnDims* d, float* seg, float* segm, const float* first, cudaStream_t st) {
+  if (p.nseg > 1) {
+    p.seg_state = seg, p.seg_m = segm;
+    Args own = p;
+    own.rep = 1;
+    int rc = run<REV, LOG, false>(own, d, st);
+    if (rc) return rc;
+    const int elems = p.e * p.f;
+    scan_kernel<REV, LOG><<<dim3((elems + 255) / 256, (unsigned)(d->B * p.H)), 256, 0, st>>>(p, seg, segm, first);
+  }
+  p.state_in = first;
+  return run<REV, LOG, true>(p, d, st);
+}
+
+// States that fit the device at once, by the registers.
+inline int64_t resident(const TmpcLinAttnDims* d) {
+  const int m = std::max(d->dk, d->dv);
+  return (int64_t)sm_count() * (m <= 32 ? 8 : m <= 64 ? 2 : 1);
+}
+
+inline Args base_args(const LinAttnArgs& a, const TmpcLinAttnDims* d, int64_t heads) {
+  LinAttnArgs z{};
+  z.T = d->T;
+  set_segments(z, (int64_t)d->B * heads, resident(d));
+  Args p{};
+  p.log_decay = a.log_decay, p.lengths = a.lengths;
+  p.T = d->T, p.H = d->H, p.G = d->G, p.rep = 1;
+  p.nseg = z.nseg, p.seg_len = z.seg_len;
+  p.a_scale = p.b_scale = 1.f;
+  return p;
+}
+
+inline size_t seg_floats(const TmpcLinAttnDims* d, int64_t heads) {
+  const Args p = base_args(LinAttnArgs{}, d, heads);
+  return p.nseg > 1 ? (size_t)d->B * d->H * p.nseg * d->dk * d->dv : 0;
 }
 
 }  // namespace rec
 
 template <>
-size_t LinAttn<float>::forward_ws(const TmpcLinAttnDims*) {
-  return 0;
+size_t LinAttn<float>::forward_ws(const TmpcLinAttnDims* d) {
+  return rec::seg_floats(d, d->H) * 4;
 }
 
 template <>
-int LinAttn<float>::forward(LinAttnArgs a, const TmpcLinAttnDims* d, char*, cudaStream_t st) {
-  by_size(d, [&](auto dd) {
-    constexpr int D = decltype(dd)::value;
-    rec::fwd_kernel<float, D><<<dim3(a.B, a.H), rec::kCols, 0, st>>>(a);
-  });
-  return (int)cudaPeekAtLastError();
+int LinAttn<float>::forward(LinAttnArgs a, const TmpcLinAttnDims* d, char* ws, cudaStream_t st) {
+  rec::Args p = rec::base_args(a, d, d->H);
+  p.a = a.q, p.b = a.k, p.c = a.v, p.o = a.o;
+  p.b_key = p.c_key = true;
+  p.e = d->dk, p.f = d->dv, p.si = d->dv, p.sj = 1;
+  p.state_out = a.state_out;
+  p.a_scale = a.scale;
+  p.vec = rows_aligned(a.q, d->dk, 4) && rows_aligned(a.k, d->dk, 4) && rows_aligned(a.v, d->dv, 4) &&
+          rows_aligned(a.o, d->dv, 4);
+  return rec::pass<false, false>(p, d, reinterpret_cast<float*>(ws), nullptr, a.state_in, st);
 }
 
 template <>
 size_t LinAttn<float>::backward_ws(const TmpcLinAttnDims* d) {
-  return (size_t)2 * d->B * d->H * sizeof(double) +
-         (d->H > d->G ? (size_t)d->B * d->T * d->G * (d->dk + d->dv) * sizeof(float) : 0);
+  const rec::Args p = rec::base_args(LinAttnArgs{}, d, d->G);
+  return (rec::seg_floats(d, d->G) * 2 + (size_t)d->B * d->H * p.nseg) * 4;
 }
 
 template <>
 int LinAttn<float>::backward(LinAttnArgs a, const TmpcLinAttnDims* d, float* dlog_decay, char* ws, cudaStream_t st) {
-  a.dlog = reinterpret_cast<float*>(ws);
-  a.acc = reinterpret_cast<float*>(ws + (size_t)2 * d->B * d->H * sizeof(double));
-  by_size(d, [&](auto dd) {
-    constexpr int D = decltype(dd)::value;
-    rec::dq_kernel<float, D><<<dim3(a.B, a.H), rec::kCols, 0, st>>>(a);
-    rec::dkv_kernel<float, D><<<dim3(a.B, a.G), 2 * rec::kCols, 0, st>>>(a);
-  });
-  if (dlog_decay)
-    rec::dlog_kernel<<<a.H, 128, 0, st>>>(reinterpret_cast<double*>(a.dlog), dlog_decay, 2 * a.B, a.H);
+  float* seg = reinterpret_cast<float*>(ws);
+  float* segm = seg + rec::seg_floats(d, d->G);
+  float* part = segm + rec::seg_floats(d, d->G);
+  rec::Args p = rec::base_args(a, d, d->G);
+  p.vec = rows_aligned(a.q, d->dk, 4) && rows_aligned(a.k, d->dk, 4) && rows_aligned(a.v, d->dv, 4) &&
+          rows_aligned(a.o, d->dv, 4) && rows_aligned(a.gq, d->dk, 4) && rows_aligned(a.gk, d->dk, 4) &&
+          rows_aligned(a.gv, d->dv, 4);
+  rec::Args q = p;  // dq
+  q.a = a.o, q.b = a.v, q.c = a.k, q.o = a.gq, q.x = a.q;
+  q.b_key = q.c_key = true;
+  q.e = d->dv, q.f = d->dk, q.si = 1, q.sj = d->dv;
+  q.a_scale = a.scale;
+  q.dstate_out = a.dstate_out, q.dlog = part;
+  int rc = dlog_decay ? rec::pass<false, true>(q, d, seg, segm, a.state_in, st)
+                      : rec::pass<false, false>(q, d, seg, nullptr, a.state_in, st);
+  if (rc) return rc;
+  p.rep = d->H / d->G;
+  p.a_key = true;
+  p.b_scale = a.scale;
+  rec::Args v = p;  // dv
+  v.a = a.k, v.b = a.q, v.c = a.o, v.o = a.gv;
+  v.e = d->dk, v.f = d->dv, v.si = d->dv, v.sj = 1;
+  v.state_out = a.dstate_in;
+  rc = rec::pass<true, false>(v, d, seg, nullptr, a.dstate_out, st);
+  if (rc) return rc;
+  p.a = a.v, p.b = a.o, p.c = a.q, p.o = a.gk;  // dk
+  p.e = d->dv, p.f = d->dk, p.si = 1, p.sj = d->dv;
+  rc = rec::pass<true, false>(p, d, seg, nullptr, a.dstate_out, st);
+  if (rc) return rc;
+  if (dlog_decay) rec::dlog_kernel<<<d->H, 128, 0, st>>>(part, dlog_decay, d->B, d->H, p.nseg);
   return (int)cudaPeekAtLastError();
 }
 

@@ -1,0 +1,118 @@
+"""History encoder: a small sequence model that turns an environment's history
+(measurements, states, controls) into parameters of its MPC problem, e.g. the
+reference trajectory.  Built on the operators of ``turbompc_b200.sequence``:
+every layer is a residual block of linear attention with a learned decay per
+head, then one of a gated feed-forward, each after a root-mean-square norm.
+
+The same weights run in two forms: ``forward`` over whole histories (training,
+or catching up on a log), and ``step`` for one token per environment and control
+tick, which keeps a state of constant size per layer and environment and
+updates it in place.
+"""
+from __future__ import annotations
+
+import math
+from typing import List, Optional, Tuple
+
+import torch
+import torch.nn.functional as F
+from torch import nn
+
+from . import sequence
+
+State = List[torch.Tensor]  # one (B, heads, head_dim, head_dim) float32 tensor per layer
+
+
+class _Layer(nn.Module):
+    def __init__(self, d: int, heads: int, kv_heads: int, head_dim: int, hidden: int, activation: str, **kw):
+        super().__init__()
+        self.heads, self.kv_heads, self.head_dim, self.activation = heads, kv_heads, head_dim, activation
+        self.norm_attention = nn.Parameter(torch.ones(d, **kw))
+        self.norm_gated = nn.Parameter(torch.ones(d, **kw))
+        w = lambda rows, cols: nn.Parameter(torch.randn(rows, cols, **kw) * cols ** -0.5)
+        self.w_qkv = w((heads + 2 * kv_heads) * head_dim, d)
+        self.w_out = w(d, heads * head_dim)
+        self.w_gate, self.w_up = w(hidden, d), w(hidden, d)
+        self.w_down = w(d, hidden)
+        # decays 1 - 2^-i, i over 2..7: memories of 4 to 128 tokens; log_decay = -exp(log_rate)
+        i = 2.0 + 5.0 * torch.arange(heads, dtype=torch.float64) / max(heads - 1, 1)
+        self.log_rate = nn.Parameter(torch.log(-torch.log1p(-torch.exp2(-i))).float().to(kw.get("device")))
+
+    def log_decay(self) -> torch.Tensor:
+        return -torch.exp(self.log_rate)
+
+    def qkv(self, y: torch.Tensor):
+        """Views of one projection, (..., heads, head_dim) each."""
+        H, G, D = self.heads, self.kv_heads, self.head_dim
+        p = F.linear(y, self.w_qkv).unflatten(-1, (H + 2 * G, D))
+        return p[..., :H, :], p[..., H:H + G, :], p[..., H + G:, :]
+
+    def after_attention(self, o: torch.Tensor, r: torch.Tensor):
+        y, r = sequence.add_rms_norm(F.linear(o.flatten(-2), self.w_out), r, self.norm_gated)
+        return F.linear(sequence.gated_linear(y, self.w_gate, self.w_up, self.activation), self.w_down), r
+
+
+class HistoryEncoder(nn.Module):
+    """``n_in`` numbers per token in, ``n_out`` out.  ``forward`` takes tokens
+    (B, T, n_in) with optional int32 ``lengths`` (B,) and ``state`` and returns
+    (outputs (B, T, n_out), state after the last token); ``step`` takes one
+    token (B, n_in) and a state, updates the state in place and returns (B, n_out).
+    Weights, tokens and outputs are float32 or bfloat16 CUDA tensors."""
+
+    def __init__(self, n_in: int, n_out: int, d_model: int = 128, heads: int = 4, kv_heads: Optional[int] = None,
+                 head_dim: int = 32, hidden: Optional[int] = None, layers: int = 2, activation: str = "silu",
+                 dtype: torch.dtype = torch.float32, device="cuda"):
+        super().__init__()
+        kv_heads = heads if kv_heads is None else kv_heads
+        if heads % kv_heads:
+            raise ValueError(f"{heads} heads do not divide into {kv_heads} key / value heads")
+        hidden = (8 * d_model) // 3 if hidden is None else hidden
+        kw = dict(dtype=dtype, device=device)
+        self.n_in, self.n_out = n_in, n_out
+        self.w_in = nn.Parameter(torch.randn(d_model, n_in, **kw) * n_in ** -0.5)
+        self.layers = nn.ModuleList(_Layer(d_model, heads, kv_heads, head_dim, hidden, activation, **kw)
+                                    for _ in range(layers))
+        self.norm_out = nn.Parameter(torch.ones(d_model, **kw))
+        self.w_out = nn.Parameter(torch.randn(n_out, d_model, **kw) / math.sqrt(d_model))
+        self.b_out = nn.Parameter(torch.zeros(n_out, **kw))
+
+    def initial_state(self, batch: int) -> State:
+        return [torch.zeros(batch, layer.heads, layer.head_dim, layer.head_dim, dtype=torch.float32,
+                            device=self.w_in.device) for layer in self.layers]
+
+    def forward(self, tokens: torch.Tensor, lengths: Optional[torch.Tensor] = None,
+                state: Optional[State] = None) -> Tuple[torch.Tensor, State]:
+        if tokens.dim() != 3 or tokens.shape[-1] != self.n_in:
+            raise ValueError(f"tokens must be (B, T, {self.n_in}), got shape {tuple(tokens.shape)}")
+        x, r = F.linear(tokens, self.w_in), None
+        out: State = []
+        for i, layer in enumerate(self.layers):
+            y, r = sequence.add_rms_norm(x, r, layer.norm_attention)
+            q, k, v = layer.qkv(y)
+            o, s = sequence.linear_attention(q, k, v, layer.log_decay(), lengths=lengths, return_state=True,
+                                             initial_state=None if state is None else state[i])
+            out.append(s)
+            x, r = layer.after_attention(o, r)
+        y, _ = sequence.add_rms_norm(x, r, self.norm_out)
+        return F.linear(y, self.w_out, self.b_out), out
+
+    @torch.no_grad()
+    def step(self, token: torch.Tensor, state: State) -> torch.Tensor:
+        if token.dim() != 2 or token.shape[-1] != self.n_in:
+            raise ValueError(f"token must be (B, {self.n_in}), got shape {tuple(token.shape)}")
+        x, r = F.linear(token, self.w_in), None
+        for layer, s in zip(self.layers, state):
+            y, r = sequence.add_rms_norm(x, r, layer.norm_attention)
+            q, k, v = layer.qkv(y)
+            o = sequence.linear_attention_step(q, k, v, layer.log_decay(), s)
+            x, r = layer.after_attention(o, r)
+        y, _ = sequence.add_rms_norm(x, r, self.norm_out)
+        return F.linear(y, self.w_out, self.b_out)
+
+
+def last_outputs(outputs: torch.Tensor, lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The outputs (B, n_out) at every sequence's last token (its first, where the length is 0)."""
+    if lengths is None:
+        return outputs[:, -1]
+    index = (lengths.long() - 1).clamp(0, outputs.shape[1] - 1)
+    return outputs.gather(1, index[:, None, None].expand(-1, 1, outputs.shape[-1]))[:, 0]

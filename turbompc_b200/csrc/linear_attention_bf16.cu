@@ -82,16 +82,21 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-template <int D>
+// A block's state: E rows (the size summed over in a read-out) x F columns (of
+// the output).
+template <int E, int F>
 struct Shape {
-  static constexpr int NW = D == 128 ? 8 : 4;         // warps: 4 row groups of 16 tokens x column groups
+  static constexpr int NW = E == 128 ? 8 : 4;         // warps: 4 row groups of 16 tokens x column groups
   static constexpr int NT = NW * 32;
-  static constexpr int OC = D == 128 ? 64 : D;        // output columns of a warp
-  static constexpr int SC = D == 32 ? 16 : D;         // state columns of a warp (16 rows)
-  static constexpr int TILE = C * D;                  // elements
-  static constexpr int kBlocks = D == 32 ? 5 : D == 64 ? 3 : 1;     // blocks per SM that the registers allow
-  static constexpr int kBlocksDkv = D == 32 ? 4 : D == 64 ? 3 : 1;
-  static constexpr int STATE = D * D;
+  static constexpr int OC = F / (NW / 4);             // output columns of a warp
+  static constexpr int SC = E == 32 ? F / 2 : F;      // state columns of a warp (16 rows)
+  static constexpr int STATE = E * F;
+  // Blocks per SM that the registers allow; with one, the next chunk is fetched
+  // while this one is computed, with several they cover for one another (64 x
+  // 64, 285 against 274 us for 1024 x 301 tokens of 8 heads).
+  static constexpr int kBlocks = F == 128 ? 1 : E == 128 ? 2 : E == 64 ? 4 : 5;
+  static constexpr int kBuf = kBlocks == 1 ? 2 : 1;
+  static constexpr int kBlocksDkv = E == 128 ? 1 : E == 64 ? 3 : 4;
 };
 
 // Element (row, col) of a tile of D-wide rows: the 16-byte units of a row are
@@ -103,40 +108,33 @@ __device__ __forceinline__ int at(int row, int col) {
   return row * D + (((col >> 3) ^ x) << 3) + (col & 7);
 }
 
-// One head's n tokens from t0 on into a C x D tile, the rest zero.  A thread
-// has one 16-byte column and every kRows-th row.
-template <int D>
-struct Loader {
-  using Z = Shape<D>;
-  static constexpr int UPR = D / 8, kRows = Z::NT / UPR;  // 16-byte units per row, rows per pass
-  const bf16* base;  // the chunk's first row
-  int64_t token;
-  int d;
-  bool vec;
-  __device__ __forceinline__ Loader(const TmpcSeqView& w, int b, int64_t t0, int h, int d_, bool vec_)
-      : base(row_ptr<bf16>(w, b, t0, h)), token(w.token), d(d_), vec(vec_) {}
-  __device__ __forceinline__ void load(bf16* s, int n) const {
-    if (vec) {
-      const int i = threadIdx.x % UPR * 8, r0 = threadIdx.x / UPR;
-      const bf16* p = base + r0 * token + i;
-      const int64_t step = kRows * token;
-      static_assert(kRows % 8 == 0, "a thread's rows share their permutation");
-      s += at<D>(r0, i);
-      const int m = i < d ? n : 0;
+// Columns c0 .. c0 + d - 1 of one head's n tokens from t0 on into a C x D tile,
+// the rest zero.  A thread has one 16-byte column and every kRows-th row.
+template <int D, int NT>
+__device__ __forceinline__ void load_tile(bf16* s, const TmpcSeqView& w, int b, int64_t t0, int n, int h, int c0, int d,
+                                          bool vec) {
+  constexpr int UPR = D / 8, kRows = NT / UPR;  // 16-byte units per row, rows per pass
+  static_assert(kRows % 8 == 0, "a thread's rows share their permutation");
+  const bf16* base = row_ptr<bf16>(w, b, t0, h) + c0;  // the tile's first row
+  if (vec) {
+    const int i = threadIdx.x % UPR * 8, r0 = threadIdx.x / UPR;
+    const bf16* p = base + r0 * w.token + i;
+    const int64_t step = kRows * w.token;
+    s += at<D>(r0, i);
+    const int m = i < d ? n : 0;
 #pragma unroll
-      for (int r = 0; r < C; r += kRows) {
-        const bool on = r0 + r < m;
-        cp16(s + r * D, on ? p : base, on);
-        p += step;
-      }
-    } else {
-      for (int u = threadIdx.x; u < C * D; u += Z::NT) {
-        const int t = u / D, i = u % D;
-        s[at<D>(t, i)] = (t < n && i < d) ? base[t * token + i] : __float2bfloat16_rn(0.f);
-      }
+    for (int r = 0; r < C; r += kRows) {
+      const bool on = r0 + r < m;
+      if (C % kRows == 0 || r0 + r < C) cp16(s + r * D, on ? p : base, on);
+      p += step;
+    }
+  } else {
+    for (int u = threadIdx.x; u < C * D; u += NT) {
+      const int t = u / D, i = u % D;
+      s[at<D>(t, i)] = (t < n && i < d) ? base[t * w.token + i] : __float2bfloat16_rn(0.f);
     }
   }
-};
+}
 
 // Fragment addresses: A (rows m, K k) of a row-major [m][k] tile; A of a tile
 // stored [k][m]; B (two 8-wide column tiles) of a tile stored [n][k], of one
@@ -164,26 +162,26 @@ __device__ __forceinline__ const bf16* frag_bk(const bf16* s, int n0, int k0) {
 
 // The warp's 16 x SC part of the state, float registers: acc[j] is columns
 // col0 + 8 j .. + 7.
-template <int D>
+template <int E, int F>
 struct State {
-  using Z = Shape<D>;
+  using Z = Shape<E, F>;
   float s[Z::SC / 8][4];
   int row0, col0;
   __device__ __forceinline__ State() {
     const int w = threadIdx.x >> 5;
-    row0 = D == 32 ? (w & 1) * 16 : w * 16;
-    col0 = D == 32 ? (w >> 1) * 16 : 0;
+    row0 = E == 32 ? (w & 1) * 16 : w * 16;
+    col0 = E == 32 ? (w >> 1) * Z::SC : 0;
   }
-  template <typename F>
-  __device__ __forceinline__ void each(F&& f) {  // f(row, col, value&)
+  template <typename Fn>
+  __device__ __forceinline__ void each(Fn&& f) {  // f(row, col, value&)
     const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
 #pragma unroll
     for (int j = 0; j < Z::SC / 8; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) f(row0 + g + (e >> 1) * 8, col0 + j * 8 + 2 * t + (e & 1), s[j][e]);
   }
-  template <typename F>
-  __device__ __forceinline__ void pairs(F&& f) {  // f(row, col, two values)
+  template <typename Fn>
+  __device__ __forceinline__ void pairs(Fn&& f) {  // f(row, col, two values)
     const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
 #pragma unroll
     for (int j = 0; j < Z::SC / 8; ++j)
@@ -194,23 +192,23 @@ struct State {
   // rows x cols of a float array, element (i, j) at p[i si + j sj]; zero elsewhere
   __device__ __forceinline__ void load(const float* p, int rows, int cols, int si, int sj) {
     if (!p) each([&](int, int, float& v) { v = 0.f; });
-    else if (rows == D && cols == D && sj == 1 && aligned8(p)) pairs([&](int i, int j, float* v) {
+    else if (rows == E && cols == F && sj == 1 && aligned8(p)) pairs([&](int i, int j, float* v) {
       const float2 x = *reinterpret_cast<const float2*>(p + i * si + j);
       v[0] = x.x, v[1] = x.y;
     });
-    else if (rows == D && cols == D) each([&](int i, int j, float& v) { v = p[i * si + j * sj]; });
+    else if (rows == E && cols == F) each([&](int i, int j, float& v) { v = p[i * si + j * sj]; });
     else each([&](int i, int j, float& v) { v = i < rows && j < cols ? p[i * si + j * sj] : 0.f; });
   }
   __device__ __forceinline__ void store(float* p, int rows, int cols, int si, int sj) {
-    if (rows == D && cols == D && sj == 1 && aligned8(p))
+    if (rows == E && cols == F && sj == 1 && aligned8(p))
       pairs([&](int i, int j, float* v) { *reinterpret_cast<float2*>(p + i * si + j) = make_float2(v[0], v[1]); });
-    else if (rows == D && cols == D) each([&](int i, int j, float& v) { p[i * si + j * sj] = v; });
+    else if (rows == E && cols == F) each([&](int i, int j, float& v) { p[i * si + j * sj] = v; });
     else
       each([&](int i, int j, float& v) {
         if (i < rows && j < cols) p[i * si + j * sj] = v;
       });
   }
-  // as N bfloat16 terms, one D x D tile each
+  // as N bfloat16 terms, one E x F tile each
   template <int N>
   __device__ __forceinline__ void publish(bf16* out) {
     const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
@@ -220,7 +218,7 @@ struct State {
       for (int r = 0; r < 2; ++r) {
         uint32_t x[N];
         split(s[j][2 * r], s[j][2 * r + 1], x);
-        const int o = at<D>(row0 + g + r * 8, col0 + j * 8) + 2 * t;
+        const int o = at<F>(row0 + g + r * 8, col0 + j * 8) + 2 * t;
 #pragma unroll
         for (int i = 0; i < N; ++i) *reinterpret_cast<uint32_t*>(out + i * Z::STATE + o) = x[i];
       }
@@ -238,7 +236,7 @@ struct State {
 #pragma unroll 1
     for (int k = 0; k < kt; ++k) {
       uint32_t f[4], x[N][4];
-      ldsm_t(f, frag_at<D>(a, row0, k * 16));
+      ldsm_t(f, frag_at<E>(a, row0, k * 16));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int tok = k * 16 + 2 * t + (i >> 1) * 8;
@@ -251,7 +249,7 @@ struct State {
 #pragma unroll
       for (int j = 0; j < Z::SC / 8; j += 2) {
         uint32_t r[4];
-        ldsm_t(r, frag_bk<D>(b, col0 + j * 8, k * 16));
+        ldsm_t(r, frag_bk<F>(b, col0 + j * 8, k * 16));
 #pragma unroll
         for (int m = 0; m < N; ++m) {
           mma(s[j], x[m], r[0], r[1]);
@@ -262,21 +260,21 @@ struct State {
   }
 };
 
-// The outputs' warp tile (16 tokens x OC columns) to global rows, through the
-// warp's rows of a tile nobody reads any more.
-template <int D>
-__device__ __forceinline__ void store_rows(const float (&o)[Shape<D>::OC / 8][4], bf16* stg, const TmpcSeqView& w, int b,
-                                           int t0, int n, int h, int d, bool vec) {
-  using Z = Shape<D>;
+// The outputs' warp tile (16 tokens x OC columns) to columns c0 .. c0 + d - 1 of
+// global rows, through the warp's rows of an E-wide tile nobody reads any more.
+template <int E, int F>
+__device__ __forceinline__ void store_rows(const float (&o)[Shape<E, F>::OC / 8][4], bf16* stg, const TmpcSeqView& w,
+                                           int b, int64_t t0, int n, int h, int c0, int d, bool vec) {
+  using Z = Shape<E, F>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int row0 = (warp & 3) * 16, col0 = (warp >> 2) * Z::OC;
 #pragma unroll
   for (int j = 0; j < Z::OC / 8; ++j) {
-    *reinterpret_cast<uint32_t*>(stg + at<D>(row0 + g, col0 + j * 8) + 2 * t) = pack2(o[j][0], o[j][1]);
-    *reinterpret_cast<uint32_t*>(stg + at<D>(row0 + g + 8, col0 + j * 8) + 2 * t) = pack2(o[j][2], o[j][3]);
+    *reinterpret_cast<uint32_t*>(stg + at<E>(row0 + g, col0 + j * 8) + 2 * t) = pack2(o[j][0], o[j][1]);
+    *reinterpret_cast<uint32_t*>(stg + at<E>(row0 + g + 8, col0 + j * 8) + 2 * t) = pack2(o[j][2], o[j][3]);
   }
   __syncwarp();
-  bf16* base = row_ptr<bf16>(w, b, t0, h);
+  bf16* base = row_ptr<bf16>(w, b, t0, h) + c0;
   if (vec) {
     constexpr int UPR = Z::OC / 8, kRows = 32 / UPR;
     const int r0 = row0 + lane / UPR, i = col0 + lane % UPR * 8, m = i < d ? n : 0;
@@ -284,23 +282,24 @@ __device__ __forceinline__ void store_rows(const float (&o)[Shape<D>::OC / 8][4]
     const int64_t step = kRows * w.token;
 #pragma unroll
     for (int r = 0; r < 16; r += kRows) {
-      if (r0 + r < m) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(stg + at<D>(r0 + r, i));
+      if (r0 + r < m) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(stg + at<E>(r0 + r, i));
       p += step;
     }
   } else {
     for (int u = lane; u < 16 * Z::OC; u += 32) {
       const int r = row0 + u / Z::OC, i = col0 + u % Z::OC;
-      if (r < n && i < d) base[r * w.token + i] = stg[at<D>(r, i)];
+      if (r < n && i < d) base[r * w.token + i] = stg[at<E>(r, i)];
     }
   }
 }
 
-// Rows t0 .. t1 - 1 of one head set to zero by the whole block.
-__device__ __forceinline__ void zero_rows(const TmpcSeqView& w, int b, int64_t t0, int64_t t1, int h, int d, bool vec) {
+// Columns c0 .. c0 + d - 1 of rows t0 .. t1 - 1 of one head set to zero by the block.
+__device__ __forceinline__ void zero_rows(const TmpcSeqView& w, int b, int64_t t0, int64_t t1, int h, int c0, int d,
+                                          bool vec) {
   if (t0 >= t1) return;
   const int upr = vec ? d / 8 : d, rows = blockDim.x / upr, r0 = threadIdx.x / upr;  // d <= 128 <= the block
   if (r0 >= rows) return;
-  bf16* p = row_ptr<bf16>(w, b, t0 + r0, h) + (threadIdx.x - r0 * upr) * (vec ? 8 : 1);
+  bf16* p = row_ptr<bf16>(w, b, t0 + r0, h) + c0 + (threadIdx.x - r0 * upr) * (vec ? 8 : 1);
   const int64_t step = rows * w.token;
   for (int64_t t = t0 + r0; t < t1; t += rows, p += step) {
     if (vec) *reinterpret_cast<uint4*>(p) = make_uint4(0, 0, 0, 0);
@@ -316,10 +315,10 @@ struct FwdArgs {
   const float* state_in;   // [B][H] x (e x f), element (i, j) at i si + j sj
   float* state_out;
   const float* seg_state;  // [B][H][nseg], same element order
-  float* part;             // dq only: [B][H][nseg * seg_len / C][2]: sum q . dq, sum (t + 1) q . dq
+  float* part;             // kDqLog: [B][H][splits][nseg * seg_len / C][2]: sum q . dq, sum (t + 1) q . dq
   int T, H, G, e, f;       // key and value sizes of this pass
   int si, sj;
-  int nseg, seg_len;
+  int nseg, seg_len, splits;
   bool vec;
   float scale;
 };
@@ -328,25 +327,27 @@ struct FwdArgs {
 // with the state are taken to float accuracy.
 enum Pass { kOut = 0, kDq = 1, kDqLog = 2 };
 
-template <int D, int PASS>
+template <int E, int F, int PASS>
 constexpr size_t fwd_smem() {
-  using Z = Shape<D>;
-  return (size_t)(2 * 3 * Z::TILE + (PASS == kDqLog ? 3 : 2) * Z::STATE) * 2 + (C + 1 + 16) * 4;
+  return (size_t)(Shape<E, F>::kBuf * C * (2 * E + F) + (PASS == kDqLog ? 3 : 2) * Shape<E, F>::STATE) * 2 + (C + 1 + 16) * 4;
 }
 
-template <int D, int PASS>
-__global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocks) fwd_kernel(const FwdArgs a) {
-  using Z = Shape<D>;
+template <int E, int F, int PASS>
+__global__ void __launch_bounds__(Shape<E, F>::NT, Shape<E, F>::kBlocks) fwd_kernel(const FwdArgs a) {
+  using Z = Shape<E, F>;
   constexpr bool DQ = PASS == kDqLog;
   constexpr int NS = DQ ? 3 : 2;  // terms of the state in a product
   extern __shared__ __align__(16) char raw[];
+  constexpr int kTiles = C * (2 * E + F);
   bf16* tiles = reinterpret_cast<bf16*>(raw);
-  bf16* st = tiles + 2 * 3 * Z::TILE;
+  bf16* st = tiles + Z::kBuf * kTiles;
   float* pw = reinterpret_cast<float*>(st + NS * Z::STATE);  // d^i
   float* red = pw + C + 1;
 
-  const int h = blockIdx.x % a.H;
-  const int seg = (blockIdx.x / a.H) % a.nseg, b = blockIdx.x / a.H / a.nseg;
+  const int split = blockIdx.x % a.splits, c0 = split * F, fl = min(F, a.f - c0);
+  const unsigned unit = blockIdx.x / a.splits;
+  const int h = unit % a.H;
+  const int seg = (unit / a.H) % a.nseg, b = unit / a.H / a.nseg;
   const int g = h / (a.H / a.G);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gr = lane >> 2, tq = lane & 3;
   const int row0 = (warp & 3) * 16, col0 = (warp >> 2) * Z::OC;
@@ -357,48 +358,50 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocks) fwd_kernel(co
   for (int i = threadIdx.x; i <= C; i += Z::NT) pw[i] = exp2f(g2 * (float)i);
 
   const int64_t bh = (int64_t)b * a.H + h, elems = (int64_t)a.e * a.f;
-  State<D> S;
+  State<E, F> S;
   const float* s0 = a.nseg > 1 ? a.seg_state + (bh * a.nseg + seg) * elems : a.state_in ? a.state_in + bh * elems : nullptr;
-  S.load(s0, a.e, a.f, a.si, a.sj);
+  S.load(s0 ? s0 + c0 * a.sj : nullptr, a.e, fl, a.si, a.sj);
   S.template publish<NS>(st);
 
-  auto load = [&](int i) {
-    bf16* buf = tiles + (i & 1) * 3 * Z::TILE;
-    const int t0 = begin + i * C, n = min(C, len - i * C);
-    Loader<D>(a.q, b, t0, h, a.e, a.vec).load(buf, n);
-    Loader<D>(a.k, b, t0, g, a.e, a.vec).load(buf + Z::TILE, n);
-    Loader<D>(a.v, b, t0, g, a.f, a.vec).load(buf + 2 * Z::TILE, n);
-  };
   const int chunks = (len + C - 1) / C;
-  if (chunks > 0) load(0);
-  cp_commit();
   bool state_on = s0 != nullptr;
-  for (int i = 0; i < chunks; ++i) {
-    if (i + 1 < chunks) load(i + 1);
-    cp_commit();
-    cp_wait<1>();
-    __syncthreads();
-    bf16* sq = tiles + (i & 1) * 3 * Z::TILE;
-    const bf16 *sk = sq + Z::TILE, *sv = sk + Z::TILE;
+  auto load = [&](int i) {
+    bf16* to = tiles + (Z::kBuf == 2 ? i & 1 : 0) * kTiles;
+    const int64_t t0 = begin + i * C;
     const int n = min(C, len - i * C);
+    load_tile<E, Z::NT>(to, a.q, b, t0, n, h, 0, a.e, a.vec);
+    load_tile<E, Z::NT>(to + C * E, a.k, b, t0, n, g, 0, a.e, a.vec);
+    load_tile<F, Z::NT>(to + 2 * C * E, a.v, b, t0, n, g, c0, fl, a.vec);
+  };
+  if (Z::kBuf == 2 && chunks > 0) load(0);
+  cp_commit();
+  for (int i = 0; i < chunks; ++i) {
+    if (i + Z::kBuf - 1 < chunks) load(i + Z::kBuf - 1);
+    cp_commit();
+    cp_wait<Z::kBuf - 1>();
+    __syncthreads();
+    const int64_t t0 = begin + i * C;
+    const int n = min(C, len - i * C);
+    bf16* sq = tiles + (Z::kBuf == 2 ? i & 1 : 0) * kTiles;
+    const bf16 *sk = sq + C * E, *sv = sk + C * E;
     if (row0 < n) {
-      uint32_t q[D / 16][4];
+      uint32_t q[E / 16][4];
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) ldsm(q[k], frag_a<D>(sq, row0, k * 16));
+      for (int k = 0; k < E / 16; ++k) ldsm(q[k], frag_a<E>(sq, row0, k * 16));
       uint32_t x[DQ ? Z::OC / 4 : 1];  // the queries in the layout of o, on their way during the products
       if constexpr (DQ) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const int row = row0 + gr + r * 8;
-          const bf16* p = row_ptr<bf16>(a.x, b, begin + i * C + row, h) + col0 + 2 * tq;
+          const bf16* p = row_ptr<bf16>(a.x, b, t0 + row, h) + c0 + col0 + 2 * tq;
 #pragma unroll
           for (int j = 0; j < Z::OC / 8; ++j) {
             const int c = col0 + j * 8 + 2 * tq;
             uint32_t v = 0;
-            if (row < n && c < a.f) {
+            if (row < n && c < fl) {
               if (a.vec) v = *reinterpret_cast<const uint32_t*>(p + j * 8);
               else v = (uint32_t)__bfloat16_as_ushort(p[j * 8]) |
-                       (c + 1 < a.f ? (uint32_t)__bfloat16_as_ushort(p[j * 8 + 1]) << 16 : 0u);
+                       (c + 1 < fl ? (uint32_t)__bfloat16_as_ushort(p[j * 8 + 1]) << 16 : 0u);
             }
             x[2 * j + r] = v;
           }
@@ -411,13 +414,13 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocks) fwd_kernel(co
         for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
       if (state_on) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
+        for (int k = 0; k < E / 16; ++k)
 #pragma unroll
           for (int j = 0; j < Z::OC / 8; j += 2)
 #pragma unroll
             for (int m = 0; m < NS; ++m) {
               uint32_t r[4];
-              ldsm_t(r, frag_bk<D>(st + m * Z::STATE, col0 + j * 8, k * 16));
+              ldsm_t(r, frag_bk<F>(st + m * Z::STATE, col0 + j * 8, k * 16));
               mma(o[j], q[k], r[0], r[1]);
               mma(o[j + 1], q[k], r[2], r[3]);
             }
@@ -443,9 +446,9 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocks) fwd_kernel(co
       for (int kt = 0; kt <= (warp & 3); ++kt) {
         float s[2][4] = {};
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
+        for (int k = 0; k < E / 16; ++k) {
           uint32_t r[4];
-          ldsm(r, frag_bn<D>(sk, kt * 16, k * 16));
+          ldsm(r, frag_bn<E>(sk, kt * 16, k * 16));
           mma(s[0], q[k], r[0], r[1]);
           mma(s[1], q[k], r[2], r[3]);
         }
@@ -463,7 +466,7 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocks) fwd_kernel(co
 #pragma unroll
         for (int j = 0; j < Z::OC / 8; j += 2) {
           uint32_t r[4];
-          ldsm_t(r, frag_bk<D>(sv, col0 + j * 8, kt * 16));
+          ldsm_t(r, frag_bk<F>(sv, col0 + j * 8, kt * 16));
           mma(o[j], p, r[0], r[1]);
           mma(o[j + 1], p, r[2], r[3]);
         }
@@ -472,10 +475,10 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocks) fwd_kernel(co
       for (int j = 0; j < Z::OC / 8; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[j][e] *= a.scale;
-      // the queries' rows of this warp (of both column halves at D = 128) are free now
+      // the queries' rows of this warp (of both column halves at E = 128) are free now
       if constexpr (Z::NW == 8) asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
       else __syncwarp();
-      store_rows<D>(o, sq, a.o, b, begin + i * C, n, h, a.f, a.vec);
+      store_rows<E, F>(o, sq, a.o, b, t0, n, h, c0, fl, a.vec);
     } else if (DQ && lane == 0) {
       red[warp] = 0.f, red[8 + warp] = 0.f;
     }
@@ -489,38 +492,42 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocks) fwd_kernel(co
       if (threadIdx.x < 2) {
         float r = 0.f;
         for (int w = 0; w < Z::NW; ++w) r += red[threadIdx.x * 8 + w];
-        a.part[((bh * a.nseg + seg) * (a.seg_len / C) + i) * 2 + threadIdx.x] = r * a.scale;
+        a.part[(((bh * a.splits + split) * a.nseg + seg) * (a.seg_len / C) + i) * 2 + threadIdx.x] = r * a.scale;
       }
     }
   }
-  cp_wait<0>();
-  zero_rows(a.o, b, begin + len, stop, h, a.f, a.vec);
-  if (a.state_out && seg == a.nseg - 1) S.store(a.state_out + bh * elems, a.e, a.f, a.si, a.sj);
+  zero_rows(a.o, b, begin + len, stop, h, c0, fl, a.vec);
+  if (a.state_out && seg == a.nseg - 1) S.store(a.state_out + bh * elems + c0 * a.sj, a.e, fl, a.si, a.sj);
 }
 
 // The state that a segment's tokens alone leave (REV false: sum d^(n-1-s) k v^T;
 // REV true: scale sum d^(t+1) q do^T, the adjoint they send back).
-template <int D, bool REV>
-__global__ void __launch_bounds__(Shape<D>::NT) segment_kernel(const LinAttnArgs a, float* out) {
-  using Z = Shape<D>;
+template <int E, int F, bool REV>
+__global__ void __launch_bounds__(Shape<E, F>::NT, Shape<E, F>::kBlocks) segment_kernel(const LinAttnArgs a, int splits,
+                                                                                       float* out) {
+  using Z = Shape<E, F>;
+  constexpr int kTiles = C * (E + F);
   extern __shared__ __align__(16) char raw[];
   bf16* tiles = reinterpret_cast<bf16*>(raw);
-  float* pw = reinterpret_cast<float*>(tiles + 4 * Z::TILE);
-  const int h = blockIdx.x % a.H;
-  const int seg = (blockIdx.x / a.H) % a.nseg, b = blockIdx.x / a.H / a.nseg;
+  float* pw = reinterpret_cast<float*>(tiles + 2 * kTiles);
+  const int c0 = blockIdx.x % splits * F, fl = min(F, a.dv - c0);
+  const unsigned unit = blockIdx.x / splits;
+  const int h = unit % a.H;
+  const int seg = (unit / a.H) % a.nseg, b = unit / a.H / a.nseg;
   const int g = h / (a.H / a.G);
   const int begin = seg * a.seg_len, stop = min(begin + a.seg_len, a.T);
   const int len = min(max(seq_len(a, b) - begin, 0), stop - begin);
   const float g2 = log2_decay(a.log_decay, h);
   for (int i = threadIdx.x; i <= C; i += Z::NT) pw[i] = exp2f(g2 * (float)i);
-  State<D> S;
+  State<E, F> S;
   S.load(nullptr, 0, 0, 0, 0);
   const int chunks = (len + C - 1) / C;
   auto load = [&](int i) {
-    bf16* buf = tiles + (i & 1) * 2 * Z::TILE;
-    const int c = REV ? chunks - 1 - i : i, t0 = begin + c * C, n = min(C, len - c * C);
-    Loader<D>(REV ? a.q : a.k, b, t0, REV ? h : g, a.dk, a.vec).load(buf, n);
-    Loader<D>(REV ? a.o : a.v, b, t0, REV ? h : g, a.dv, a.vec).load(buf + Z::TILE, n);
+    bf16* buf = tiles + (i & 1) * kTiles;
+    const int c = REV ? chunks - 1 - i : i, n = min(C, len - c * C);
+    const int64_t t0 = begin + c * C;
+    load_tile<E, Z::NT>(buf, REV ? a.q : a.k, b, t0, n, REV ? h : g, 0, a.dk, a.vec);
+    load_tile<F, Z::NT>(buf + C * E, REV ? a.o : a.v, b, t0, n, REV ? h : g, c0, fl, a.vec);
   };
   if (chunks > 0) load(0);
   cp_commit();
@@ -529,13 +536,14 @@ __global__ void __launch_bounds__(Shape<D>::NT) segment_kernel(const LinAttnArgs
     cp_commit();
     cp_wait<1>();
     __syncthreads();
-    const bf16* ta = tiles + (i & 1) * 2 * Z::TILE;
+    const bf16* ta = tiles + (i & 1) * kTiles;
     const int c = REV ? chunks - 1 - i : i, n = min(C, len - c * C);
-    S.template update<3>(ta, ta + Z::TILE, pw[n], n, [&](int t) { return REV ? pw[min(t + 1, C)] * a.scale : pw[max(n - 1 - t, 0)]; });
+    S.template update<3>(ta, ta + C * E, pw[n], n,
+                         [&](int t) { return REV ? pw[min(t + 1, C)] * a.scale : pw[max(n - 1 - t, 0)]; });
     __syncthreads();
   }
   cp_wait<0>();
-  S.store(out + (((int64_t)b * a.H + h) * a.nseg + seg) * a.dk * a.dv, a.dk, a.dv, a.dv, 1);
+  S.store(out + (((int64_t)b * a.H + h) * a.nseg + seg) * a.dk * a.dv + c0, a.dk, fl, a.dv, 1);
 }
 
 // In place: what each segment leaves alone -> the state before each segment
@@ -570,19 +578,19 @@ struct DkvArgs {
 // LOG: with dlog d or dstate_in, so the adjoint state's products to float accuracy.
 template <int D, bool LOG>
 constexpr size_t dkv_smem() {
-  using Z = Shape<D>;
-  return (size_t)(4 * Z::TILE + (LOG ? 3 : 1) * Z::STATE) * 2 + (C + 1 + 24) * 4;
+  using Z = Shape<D, D>;
+  return (size_t)(4 * C * D + (LOG ? 3 : 1) * Z::STATE) * 2 + (C + 1 + 24) * 4;
 }
 
 template <int D, bool LOG>
-__global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocksDkv) dkv_kernel(const DkvArgs args) {
-  using Z = Shape<D>;
+__global__ void __launch_bounds__(Shape<D, D>::NT, Shape<D, D>::kBlocksDkv) dkv_kernel(const DkvArgs args) {
+  using Z = Shape<D, D>;
   constexpr int NS = LOG ? 3 : 1;  // terms of the adjoint state in dk's product; dv's takes the first
   const LinAttnArgs& a = args.a;
   extern __shared__ __align__(16) char raw[];
   bf16* sq = reinterpret_cast<bf16*>(raw);
-  bf16 *sk = sq + Z::TILE, *sv = sk + Z::TILE, *sdo = sv + Z::TILE;
-  bf16* st = sdo + Z::TILE;
+  bf16 *sk = sq + C * D, *sv = sk + C * D, *sdo = sv + C * D;
+  bf16* st = sdo + C * D;
   float* pw = reinterpret_cast<float*>(st + NS * Z::STATE);
   float* red = pw + C + 1;
 
@@ -602,7 +610,7 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocksDkv) dkv_kernel
     const float g2 = log2_decay(a.log_decay, h);
     __syncthreads();
     for (int i = threadIdx.x; i <= C; i += Z::NT) pw[i] = exp2f(g2 * (float)i);
-    State<D> R;
+    State<D, D> R;
     const float* r0 = a.nseg > 1 ? a.seg_dstate + (bh * a.nseg + seg) * elems
                                  : a.dstate_out ? a.dstate_out + bh * elems : nullptr;
     R.load(r0, a.dk, a.dv, a.dv, 1);
@@ -610,10 +618,10 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocksDkv) dkv_kernel
     bool state_on = r0 != nullptr;
     for (int i = chunks - 1; i >= 0; --i) {
       const int t0 = begin + i * C, n = min(C, len - i * C);
-      Loader<D>(a.q, b, t0, h, a.dk, a.vec).load(sq, n);
-      Loader<D>(a.k, b, t0, g, a.dk, a.vec).load(sk, n);
-      Loader<D>(a.v, b, t0, g, a.dv, a.vec).load(sv, n);
-      Loader<D>(a.o, b, t0, h, a.dv, a.vec).load(sdo, n);
+      load_tile<D, Z::NT>(sq, a.q, b, t0, n, h, 0, a.dk, a.vec);
+      load_tile<D, Z::NT>(sk, a.k, b, t0, n, g, 0, a.dk, a.vec);
+      load_tile<D, Z::NT>(sv, a.v, b, t0, n, g, 0, a.dv, a.vec);
+      load_tile<D, Z::NT>(sdo, a.o, b, t0, n, h, 0, a.dv, a.vec);
       cp_commit();
       cp_wait<0>();
       __syncthreads();
@@ -739,8 +747,8 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocksDkv) dkv_kernel
           }
         }
         if (r + 1 == rep) {
-          store_rows<D>(dk, sk, a.gk, b, t0, n, g, a.dk, a.vec);
-          store_rows<D>(dv, sv, a.gv, b, t0, n, g, a.dv, a.vec);
+          store_rows<D, D>(dk, sk, a.gk, b, t0, n, g, 0, a.dk, a.vec);
+          store_rows<D, D>(dv, sv, a.gv, b, t0, n, g, 0, a.dv, a.vec);
         }
       }
       __syncthreads();
@@ -764,13 +772,13 @@ __global__ void __launch_bounds__(Shape<D>::NT, Shape<D>::kBlocksDkv) dkv_kernel
       if (a.dstate_in) R.store(a.dstate_in + bh * elems, a.dk, a.dv, a.dv, 1);
     }
   }
-  zero_rows(a.gk, b, begin + len, stop, g, a.dk, a.vec);
-  zero_rows(a.gv, b, begin + len, stop, g, a.dv, a.vec);
+  zero_rows(a.gk, b, begin + len, stop, g, 0, a.dk, a.vec);
+  zero_rows(a.gv, b, begin + len, stop, g, 0, a.dv, a.vec);
 }
 
 // dlog d per (sequence, head) from the chunks' shares, then the sum over the batch.
-__global__ void __launch_bounds__(256) dlog_kernel(const LinAttnArgs a, const float* pq, const float* pk,
-                                                  const float* edge, float* out) {
+__global__ void __launch_bounds__(256) dlog_kernel(const LinAttnArgs a, int splits, const float* pq,
+                                                  const float* pk, const float* edge, float* out) {
   __shared__ double red[8];
   const int h = blockIdx.x;
   const float g2 = log2_decay(a.log_decay, h);
@@ -782,9 +790,14 @@ __global__ void __launch_bounds__(256) dlog_kernel(const LinAttnArgs a, const fl
     double e = edge[bh];
     for (int i = 0; i * C < len; ++i) {
       const int n = min(C, len - i * C);
-      const float *q = pq + (bh * all_chunks + i) * 2, *k = pk + (bh * all_chunks + i) * 3;
-      const double x = g2 * (float)n < -20.f ? 0.0 : e - (double)q[0];
-      sum += (double)k[0] + (double)q[1] + (double)k[2] + n * x;
+      const float* k = pk + (bh * all_chunks + i) * 3;
+      double q0 = 0, q1 = 0;
+      for (int p = 0; p < splits; ++p) {
+        const float* q = pq + ((bh * splits + p) * all_chunks + i) * 2;
+        q0 += q[0], q1 += q[1];
+      }
+      const double x = g2 * (float)n < -20.f ? 0.0 : e - q0;
+      sum += (double)k[0] + q1 + (double)k[2] + n * x;
       e = x + (double)k[1];
     }
   }
@@ -798,7 +811,32 @@ __global__ void __launch_bounds__(256) dlog_kernel(const LinAttnArgs a, const fl
   }
 }
 
-inline int64_t resident_blocks(const TmpcLinAttnDims* d) {
+// Blocks per head of an e x f pass.
+inline int splits_of(int e, int f) { return e <= 64 && f > 64 ? 2 : 1; }
+
+// Calls f with the compiled state of an e x f pass (E >= F), and the blocks per head.
+template <typename Fn>
+void by_shape(int e, int f, Fn&& fn) {
+  using I32 = std::integral_constant<int, 32>;
+  using I64 = std::integral_constant<int, 64>;
+  using I128 = std::integral_constant<int, 128>;
+  // Two blocks of 64 columns: 453 us where one of 128 takes 374 (32749 tokens,
+  // 16 heads of 128 x 128): each of the two splits the keys' terms again.
+  if (e > 64) {
+    if (f <= 32) fn(I128{}, I32{}, 1);
+    else if (f <= 64) fn(I128{}, I64{}, 1);
+    else fn(I128{}, I128{}, 1);
+  } else if (f > 32) {
+    fn(I64{}, I64{}, splits_of(e, f));
+  } else if (e > 32) {
+    fn(I64{}, I32{}, 1);
+  } else {
+    fn(I32{}, I32{}, 1);
+  }
+}
+
+// Heads that fit the device at once (of the widest pass).
+inline int64_t resident_heads(const TmpcLinAttnDims* d) {
   const int m = std::max(d->dk, d->dv);
   return (int64_t)sm_count() * (m <= 64 ? 2 : 1);
 }
@@ -808,12 +846,13 @@ inline int64_t resident_blocks(const TmpcLinAttnDims* d) {
 template <bool REV>
 int run_segments(const LinAttnArgs& a, const TmpcLinAttnDims* d, float* seg, const float* first, cudaStream_t st) {
   int rc = 0;
-  by_size(d, [&](auto dd) {
-    constexpr int D = decltype(dd)::value;
-    const size_t smem = (size_t)4 * Shape<D>::TILE * 2 + (C + 1) * 4;
-    rc = allow_smem<segment_kernel<D, REV>>((int)smem);
+  by_shape(d->dk, d->dv, [&](auto ee, auto ff, int splits) {
+    constexpr int E = decltype(ee)::value, F = decltype(ff)::value;
+    constexpr int smem = 2 * C * (E + F) * 2 + (C + 1) * 4;
+    rc = allow_smem<segment_kernel<E, F, REV>>(smem);
     if (!rc)
-      segment_kernel<D, REV><<<(unsigned)((int64_t)a.B * a.nseg * a.H), Shape<D>::NT, smem, st>>>(a, seg);
+      segment_kernel<E, F, REV><<<(unsigned)((int64_t)a.B * a.nseg * a.H * splits), Shape<E, F>::NT, smem, st>>>(
+          a, splits, seg);
   });
   if (rc) return rc;
   scan_kernel<REV><<<dim3((unsigned)((a.dk * a.dv + 255) / 256), (unsigned)(a.B * a.H)), 256, 0, st>>>(a, seg, first);
@@ -821,13 +860,15 @@ int run_segments(const LinAttnArgs& a, const TmpcLinAttnDims* d, float* seg, con
 }
 
 template <int PASS>
-int run_fwd(const FwdArgs& f, const LinAttnArgs& a, const TmpcLinAttnDims* d, cudaStream_t st) {
+int run_fwd(FwdArgs f, int B, cudaStream_t st) {
   int rc = 0;
-  by_size(d, [&](auto dd) {
-    constexpr int D = decltype(dd)::value;
-    rc = allow_smem<fwd_kernel<D, PASS>>((int)fwd_smem<D, PASS>());
+  by_shape(f.e, f.f, [&](auto ee, auto ff, int splits) {
+    constexpr int E = decltype(ee)::value, F = decltype(ff)::value;
+    constexpr int smem = (int)fwd_smem<E, F, PASS>();
+    f.splits = splits;
+    rc = allow_smem<fwd_kernel<E, F, PASS>>(smem);
     if (!rc)
-      fwd_kernel<D, PASS><<<(unsigned)((int64_t)a.B * a.nseg * a.H), Shape<D>::NT, fwd_smem<D, PASS>(), st>>>(f);
+      fwd_kernel<E, F, PASS><<<(unsigned)((int64_t)B * f.nseg * f.H * splits), Shape<E, F>::NT, smem, st>>>(f);
   });
   return rc ? rc : (int)cudaPeekAtLastError();
 }
@@ -849,7 +890,7 @@ inline BackwardPlan backward_plan(const LinAttnArgs& a, const TmpcLinAttnDims* d
     p.seg_state = take(bh * a.nseg * elems);
     p.seg_dstate = take(bh * a.nseg * elems);
   }
-  p.pq = take(bh * chunks * 2);
+  p.pq = take(bh * splits_of(d->dv, d->dk) * chunks * 2);
   p.pk = take(bh * chunks * 3);
   p.edge = take(bh);
   size_t chunk_floats = 0;
@@ -862,7 +903,7 @@ inline BackwardPlan backward_plan(const LinAttnArgs& a, const TmpcLinAttnDims* d
 inline LinAttnArgs sized(const TmpcLinAttnDims* d, int64_t heads) {
   LinAttnArgs a{};
   a.B = d->B, a.T = d->T, a.H = d->H, a.G = d->G, a.dk = d->dk, a.dv = d->dv;
-  set_segments(a, (int64_t)d->B * heads, resident_blocks(d));
+  set_segments(a, (int64_t)d->B * heads, resident_heads(d));
   return a;
 }
 
@@ -886,8 +927,8 @@ int LinAttn<bf16>::forward(LinAttnArgs a, const TmpcLinAttnDims* d, char* ws, cu
     if (rc) return rc;
   }
   const la::FwdArgs f{a.q, a.k, a.v, a.o, a.o, a.log_decay, a.lengths, a.state_in, a.state_out, seg, nullptr,
-                      a.T, a.H, a.G, a.dk, a.dv, a.dv, 1, a.nseg, a.seg_len, a.vec, a.scale};
-  return la::run_fwd<la::kOut>(f, a, d, st);
+                      a.T, a.H, a.G, a.dk, a.dv, a.dv, 1, a.nseg, a.seg_len, 1, a.vec, a.scale};
+  return la::run_fwd<la::kOut>(f, d->B, st);
 }
 
 template <>
@@ -914,8 +955,8 @@ int LinAttn<bf16>::backward(LinAttnArgs a, const TmpcLinAttnDims* d, float* dlog
   a.acc = at(p.acc);
   // dq: the forward sum over (do, v, k) with the transposed state
   const la::FwdArgs f{a.o, a.v, a.k, a.gq, a.q, a.log_decay, a.lengths, a.state_in, nullptr, a.seg_state, at(p.pq),
-                      a.T, a.H, a.G, a.dv, a.dk, 1, a.dv, a.nseg, a.seg_len, a.vec, a.scale};
-  int rc = dlog_decay ? la::run_fwd<la::kDqLog>(f, a, d, st) : la::run_fwd<la::kDq>(f, a, d, st);
+                      a.T, a.H, a.G, a.dv, a.dk, 1, a.dv, a.nseg, a.seg_len, 1, a.vec, a.scale};
+  int rc = dlog_decay ? la::run_fwd<la::kDqLog>(f, d->B, st) : la::run_fwd<la::kDq>(f, d->B, st);
   if (rc) return rc;
   const la::DkvArgs k{a, at(p.pk), dlog_decay ? at(p.edge) : nullptr};
   by_size(d, [&](auto dd) {
@@ -924,14 +965,14 @@ int LinAttn<bf16>::backward(LinAttnArgs a, const TmpcLinAttnDims* d, float* dlog
       constexpr bool LOG = decltype(log)::value;
       rc = allow_smem<la::dkv_kernel<D, LOG>>((int)la::dkv_smem<D, LOG>());
       if (!rc)
-        la::dkv_kernel<D, LOG><<<(unsigned)((int64_t)a.B * a.nseg * a.G), la::Shape<D>::NT, la::dkv_smem<D, LOG>(),
+        la::dkv_kernel<D, LOG><<<(unsigned)((int64_t)a.B * a.nseg * a.G), la::Shape<D, D>::NT, la::dkv_smem<D, LOG>(),
                                  st>>>(k);
     };
     if (dlog_decay || a.dstate_in) run(std::true_type{});
     else run(std::false_type{});
   });
   if (rc) return rc;
-  if (dlog_decay) la::dlog_kernel<<<a.H, 256, 0, st>>>(a, at(p.pq), at(p.pk), at(p.edge), dlog_decay);
+  if (dlog_decay) la::dlog_kernel<<<a.H, 256, 0, st>>>(a, la::splits_of(d->dv, d->dk), at(p.pq), at(p.pk), at(p.edge), dlog_decay);
   return (int)cudaPeekAtLastError();
 }
 

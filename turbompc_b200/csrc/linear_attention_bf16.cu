@@ -908,20 +908,56 @@ inline LinAttnArgs sized(const TmpcLinAttnDims* d, int64_t heads) {
 }
 
 }  // namespace la
+}  // namespace seq
+}  // namespace tmpc
+
+#include "seq_attention_tc.cuh"
+
+namespace tmpc {
+namespace seq {
+namespace tc {
+
+// Wide heads over more tokens than half a chunk of 128.
+inline bool wanted(const TmpcLinAttnDims* d) { return std::max(d->dk, d->dv) > 64 && d->T > CT / 2; }
+
+inline LinAttnArgs sized(const TmpcLinAttnDims* d) {
+  LinAttnArgs a{};
+  a.T = d->T;
+  set_segments(a, (int64_t)d->B * d->H, sm_count(), CT);
+  return a;
+}
+
+}  // namespace tc
 
 template <>
 size_t LinAttn<bf16>::forward_ws(const TmpcLinAttnDims* d) {
-  const LinAttnArgs a = la::sized(d, d->H);
-  return a.nseg > 1 ? (size_t)d->B * d->H * a.nseg * d->dk * d->dv * 4 : 0;
+  int nseg = la::sized(d, d->H).nseg;
+  if (tc::wanted(d)) nseg = std::max(nseg, tc::sized(d).nseg);
+  return nseg > 1 ? (size_t)d->B * d->H * nseg * d->dk * d->dv * 4 : 0;
 }
 
 template <>
 int LinAttn<bf16>::forward(LinAttnArgs a, const TmpcLinAttnDims* d, char* ws, cudaStream_t st) {
-  const LinAttnArgs z = la::sized(d, d->H);
-  a.nseg = z.nseg, a.seg_len = z.seg_len;
   a.vec = rows_aligned(a.q, d->dk, 2) && rows_aligned(a.k, d->dk, 2) && rows_aligned(a.v, d->dv, 2) &&
           rows_aligned(a.o, d->dv, 2);
   float* seg = reinterpret_cast<float*>(ws);
+  tc::Maps maps;
+  if (tc::wanted(d) && a.vec && tc::view_map(&maps.q, a.q, d->dk, d->H, d->T, d->B) &&
+      tc::view_map(&maps.k, a.k, d->dk, d->G, d->T, d->B) && tc::view_map(&maps.v, a.v, d->dv, d->G, d->T, d->B)) {
+    const LinAttnArgs z = tc::sized(d);
+    a.nseg = z.nseg, a.seg_len = z.seg_len;
+    const tc::Args t{a.o, a.log_decay, a.lengths, a.state_in, a.state_out, seg, seg, a.T, a.H, a.G, a.dk, a.dv, a.dv, 1,
+                     a.nseg, a.seg_len, a.scale, 0};
+    if (a.nseg > 1) {
+      const int rc = tc::launch<true>(maps, t, d->B, st);
+      if (rc) return rc;
+      la::scan_kernel<false><<<dim3((unsigned)((a.dk * a.dv + 255) / 256), (unsigned)(a.B * a.H)), 256, 0, st>>>(
+          a, seg, a.state_in);
+    }
+    return tc::launch<false>(maps, t, d->B, st);
+  }
+  const LinAttnArgs z = la::sized(d, d->H);
+  a.nseg = z.nseg, a.seg_len = z.seg_len;
   if (a.nseg > 1) {
     const int rc = la::run_segments<false>(a, d, seg, a.state_in, st);
     if (rc) return rc;

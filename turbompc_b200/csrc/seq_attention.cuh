@@ -69,15 +69,15 @@ void by_size(const TmpcLinAttnDims* d, F&& f) {
   else f(std::integral_constant<int, 128>{});
 }
 
-// Segments of a call with `lanes` independent (sequence, head) pairs, of which
-// `resident` fit on the device at once: none while the pairs fill it; else
-// enough to fill it, each at least four chunks long.
-inline void set_segments(LinAttnArgs& a, int64_t lanes, int64_t resident) {
-  const int64_t chunks = ((int64_t)a.T + kChunk - 1) / kChunk;
+// Segments, in whole chunks, of a call with `lanes` independent (sequence, head)
+// pairs, of which `resident` fit on the device at once: none while the pairs
+// fill half of it; else enough to fill it, each at least four chunks long.
+inline void set_segments(LinAttnArgs& a, int64_t lanes, int64_t resident, int chunk = kChunk) {
+  const int64_t chunks = ((int64_t)a.T + chunk - 1) / chunk;
   int64_t n = lanes > 0 && lanes * 2 <= resident ? resident / lanes : 1;
   n = std::max<int64_t>(1, std::min<int64_t>(n, chunks / 4));
   const int64_t per = (chunks + n - 1) / n;
-  a.seg_len = (int)(std::max<int64_t>(per, 1) * kChunk);
+  a.seg_len = (int)(std::max<int64_t>(per, 1) * chunk);
   a.nseg = (int)std::max<int64_t>(1, (chunks + per - 1) / std::max<int64_t>(per, 1));
 }
 

@@ -1,0 +1,419 @@
+// Linear attention for wide heads (more than 64 elements on a side), bfloat16:
+// the forward pass on the tensor cores' asynchronous path (tcgen05), in chunks
+// of 128 tokens.  Included by linear_attention_bf16.cu.
+//
+// Per chunk, with S the float state before it, held in the workers' registers:
+//     SC = Q K^T                               128 x 128 scores
+//     IN = Q S          S in two bfloat16 terms
+//     OT = P V          P = the masked, decayed scores, one bfloat16, kept in TMEM
+//     DL = K'^T V       K' = d^(n-1-s) k_s in three bfloat16 terms
+//     o = scale (d^(t+1) IN + OT),   S <- d^n S + DL
+// Each product has its own 128 columns of TMEM.  Warp 16 loads Q, K and V by TMA,
+// warp 17 issues the products, warps 0 .. 15 do everything between them: a
+// thread owns one TMEM lane (a token, or a row of S) and 32 columns.  K' goes
+// through two buffers of 32 tokens, so that forming a part and multiplying the
+// one before overlap.  With the matrix instructions issued from registers the
+// same work is bound by them and by the operands' loads from shared memory (64
+// tokens of a 128 x 128 head: 12 thousand cycles per SM).
+//
+// Every wait is bounded, as in seq_gemm.cuh: a wait that runs out sets the
+// block's abort flag, what is in flight is drained, TMEM is freed, and outputs
+// not computed are NaN.
+#pragma once
+
+#include "seq_gemm.cuh"
+
+namespace tmpc {
+namespace seq {
+namespace tc {
+
+constexpr int CT = 128;            // tokens per chunk
+constexpr int kWorkers = 16;       // warps
+constexpr int kThreads = (kWorkers + 2) * 32;
+constexpr int kTile = CT * 128 * 2;  // bytes of a 128 x 128 bfloat16 tile: two boxes of 64 columns
+constexpr int kPart = 32;          // tokens of a part of K'
+constexpr int kPartBytes = kPart * 128 * 2;
+
+// Shared memory: Q, K, V, S in two terms, K' parts (two buffers of three terms).
+constexpr int kQ = 0, kK = kTile, kV = 2 * kTile, kS = 3 * kTile, kKp = 5 * kTile;
+constexpr int kBars = kKp + 2 * 3 * kPartBytes;
+constexpr int kSmem = kBars + 1024 + 1024;  // barriers and powers of d; alignment
+static_assert(kSmem <= 227 * 1024, "");
+
+struct Bars {
+  uint64_t qk_full, v_full, sc_done, in_done, ot_done, dl_done, p_ready, s_ready, o_read, k_free, kp_ready[2], kp_free[2],
+      done;
+  uint32_t tmem;
+  int abort_flag;
+  float pw[CT + 1];
+};
+
+struct Args {
+  TmpcSeqView o;
+  const float* log_decay;
+  const int32_t* lengths;
+  const float* state_in;   // element (i, j) of a head's state at i si + j sj
+  float* state_out;
+  const float* seg_state;  // [B][H][nseg]
+  float* seg_out;          // state only: where to leave a segment's own state
+  int T, H, G, e, f, si, sj, nseg, seg_len;
+  float scale;
+  uint32_t polls;
+};
+
+struct Maps {
+  CUtensorMap q, k, v;
+};
+
+__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {  // 128-byte swizzle
+  return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+__device__ __forceinline__ void mma_tmem_a(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
+      : "memory");
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// 16-byte unit u (0 .. 15, 8 elements each) of row r of a tile whose 64-wide boxes have `rows` rows.
+__device__ __forceinline__ int unit_at(int r, int u, int rows) {
+  return (u >> 3) * rows * 128 + r * 128 + (((u & 7) ^ (r & 7)) << 4);
+}
+
+template <bool STATE_ONLY>
+__global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Maps maps, const Args a) {
+  using gemm::fence_after;
+  using gemm::fence_before;
+  using gemm::mbar_arrive;
+  using gemm::mma_commit;
+  using gemm::mma_f16;
+  using gemm::tmem_ld16;
+  using gemm::tmem_wait_ld;
+  extern __shared__ char raw[];
+  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  Bars& bar = *reinterpret_cast<Bars*>(smem + kBars);
+  volatile int* abort_flag = &bar.abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  const int h = blockIdx.x % a.H, seg = blockIdx.x / a.H % a.nseg, b = blockIdx.x / a.H / a.nseg;
+  const int g = h / (a.H / a.G);
+  int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+  const int begin = seg * a.seg_len, stop = min(begin + a.seg_len, a.T);
+  len = min(max(len - begin, 0), stop - begin);
+  const int chunks = (len + CT - 1) / CT;
+  const float g2 = log2_decay(a.log_decay, h);
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bar.qk_full, 1), mbar_init(&bar.v_full, 1);
+    mbar_init(&bar.sc_done, 1), mbar_init(&bar.in_done, 1), mbar_init(&bar.ot_done, 1), mbar_init(&bar.dl_done, 1);
+    mbar_init(&bar.p_ready, kWorkers), mbar_init(&bar.s_ready, kWorkers), mbar_init(&bar.o_read, kWorkers);
+    mbar_init(&bar.k_free, kWorkers), mbar_init(&bar.done, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&bar.kp_ready[i], kWorkers), mbar_init(&bar.kp_free[i], 1);
+    bar.abort_flag = 0;
+  }
+  for (int i = threadIdx.x; i <= CT; i += kThreads) bar.pw[i] = exp2f(g2 * (float)i);
+  if (warp == kWorkers) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar.tmem)), "n"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = bar.tmem;
+  const uint32_t tSC = tmem, tIN = tmem + 128, tOT = tmem + 256, tDL = tmem + 384;
+  bool ok = true;
+  auto wait = [&](uint64_t* w, uint32_t parity) {
+    if (ok) ok = gemm::wait(w, parity, a.polls, abort_flag);
+    return ok;
+  };
+
+  if (warp == kWorkers && lane == 0) {  // loads
+    int i = 0;
+    for (; i < chunks; ++i) {
+      const int t0 = begin + i * CT;
+      // K is free when its last part of K' is formed (and the scores are done, which p_ready of the same chunk waits
+      // for); Q when the read-out of the state is done; V when the state's update is.
+      if (i > 0 && !wait(&bar.k_free, (i - 1) & 1)) break;
+      if (!STATE_ONLY && i > 0 && !wait(&bar.in_done, (i - 1) & 1)) break;
+      mbar_expect_tx(&bar.qk_full, (STATE_ONLY ? 1 : 2) * kTile);
+      for (int x = 0; x < 2; ++x) {
+        if (!STATE_ONLY) tma_load_4d(smem + kQ + x * (kTile / 2), &maps.q, x * 64, h, t0, b, &bar.qk_full);
+        tma_load_4d(smem + kK + x * (kTile / 2), &maps.k, x * 64, g, t0, b, &bar.qk_full);
+      }
+      if (i > 0 && !wait(&bar.dl_done, (i - 1) & 1)) {
+        mbar_wait_bounded(&bar.qk_full, i & 1, kTransferDrainPolls);
+        break;
+      }
+      mbar_expect_tx(&bar.v_full, kTile);
+      for (int x = 0; x < 2; ++x) tma_load_4d(smem + kV + x * (kTile / 2), &maps.v, x * 64, g, t0, b, &bar.v_full);
+    }
+    if (chunks > 0 && i > 0) {  // nothing may land after the block has left
+      mbar_wait_bounded(&bar.qk_full, (i - 1) & 1, kTransferDrainPolls);
+      mbar_wait_bounded(&bar.v_full, (i - 1) & 1, kTransferDrainPolls);
+    }
+  } else if (warp == kWorkers + 1 && lane == 0) {  // products, 128 x 128, K 16 each
+    constexpr uint32_t kBase = 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(128 / 8) << 17 | (uint32_t)(128 / 16) << 24;
+    constexpr uint32_t kAmn = 1u << 15, kBmn = 1u << 16;
+    const uint32_t sq = smem_u32(smem + kQ), sk = smem_u32(smem + kK), sv = smem_u32(smem + kV),
+                   ss = smem_u32(smem + kS), skp = smem_u32(smem + kKp);
+    auto krow = [](int k) { return (k >> 2) * (kTile / 2) + (k & 3) * 32; };  // K-major tile: 4 steps per 64-wide box
+    for (int i = 0; i < chunks && ok; ++i) {
+      const uint32_t ph = i & 1;
+      if constexpr (!STATE_ONLY) {
+        if (!wait(&bar.qk_full, ph)) break;
+        fence_after();
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          mma_f16(tSC, desc(sq + krow(k), 16, 1024), desc(sk + krow(k), 16, 1024), kBase, k > 0);
+        mma_commit(&bar.sc_done);
+        if (!wait(&bar.s_ready, ph) || (i > 0 && !wait(&bar.o_read, (i - 1) & 1))) break;
+        fence_after();
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            mma_f16(tIN, desc(sq + krow(k), 16, 1024), desc(ss + m * kTile + k * 2048, kTile / 2, 1024), kBase | kBmn,
+                    m + k > 0);
+        mma_commit(&bar.in_done);
+        if (!wait(&bar.v_full, ph) || !wait(&bar.p_ready, ph)) break;
+        fence_after();
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          mma_tmem_a(tOT, tSC + k * 8, desc(sv + k * 2048, kTile / 2, 1024), kBase | kBmn, k > 0);
+        mma_commit(&bar.ot_done);
+      }
+      if (STATE_ONLY && !wait(&bar.v_full, ph)) break;
+      for (int j = 0; j < CT / kPart; ++j) {
+        if (!wait(&bar.kp_ready[j & 1], ((i * (CT / kPart) + j) >> 1) & 1)) break;
+        fence_after();
+        const uint32_t kp = skp + (j & 1) * 3 * kPartBytes;
+#pragma unroll
+        for (int m = 0; m < 3; ++m)
+#pragma unroll
+          for (int k = 0; k < kPart / 16; ++k)
+            mma_f16(tDL, desc(kp + m * kPartBytes + k * 2048, kPartBytes / 2, 1024),
+                    desc(sv + j * kPart * 128 + k * 2048, kTile / 2, 1024), kBase | kAmn | kBmn, j + m + k > 0);
+        mma_commit(&bar.kp_free[j & 1]);
+      }
+      if (ok) mma_commit(&bar.dl_done);
+    }
+    if (!ok) {  // TMEM may be freed only after the products in flight
+      mma_commit(&bar.done);
+      mbar_wait_bounded(&bar.done, 0, kTransferDrainPolls);
+    }
+  } else if (warp < kWorkers) {
+    const int quad = warp & 3, c0 = (warp >> 2) * 32;
+    const int row = quad * 32 + lane;  // token of the chunk, or row of the state
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    const float* pw = bar.pw;
+    const float nan = __int_as_float(0x7fffffff);
+    const int64_t bh = (int64_t)b * a.H + h, elems = (int64_t)a.e * a.f;
+    auto arrive = [&](uint64_t* w) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(w);
+    };
+    float S[32];
+    const float* s0 = STATE_ONLY ? nullptr
+                      : a.nseg > 1 ? a.seg_state + (bh * a.nseg + seg) * elems
+                      : a.state_in ? a.state_in + bh * elems : nullptr;
+#pragma unroll
+    for (int c = 0; c < 32; ++c)
+      S[c] = s0 && row < a.e && c0 + c < a.f ? s0[row * a.si + (c0 + c) * a.sj] : 0.f;
+    auto publish = [&] {  // S in two terms, rows of the state as rows of the tile
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        uint32_t t[2][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t x[2];
+          la::split(S[u * 8 + 2 * e], S[u * 8 + 2 * e + 1], x);
+          t[0][e] = x[0], t[1][e] = x[1];
+        }
+        const int o = unit_at(row, c0 / 8 + u, 128);
+        *reinterpret_cast<uint4*>(smem + kS + o) = make_uint4(t[0][0], t[0][1], t[0][2], t[0][3]);
+        *reinterpret_cast<uint4*>(smem + kS + kTile + o) = make_uint4(t[1][0], t[1][1], t[1][2], t[1][3]);
+      }
+      fence_async();
+      arrive(&bar.s_ready);
+    };
+    if (!STATE_ONLY && chunks > 0) publish();
+    for (int i = 0; i < chunks; ++i) {
+      const uint32_t ph = i & 1;
+      const int n = min(CT, len - i * CT);
+      if constexpr (!STATE_ONLY) {  // the scores become P, in their own columns of TMEM
+        wait(&bar.sc_done, ph);
+        fence_after();
+        float x[32];
+        tmem_ld16(tSC + lane_off + c0, *reinterpret_cast<float(*)[16]>(&x[0]));
+        tmem_ld16(tSC + lane_off + c0 + 16, *reinterpret_cast<float(*)[16]>(&x[16]));
+        tmem_wait_ld();
+        uint32_t p[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          const int l0 = row - (c0 + 2 * c), l1 = l0 - 1;
+          p[c] = la::pack2(l0 >= 0 ? x[2 * c] * pw[max(l0, 0)] : 0.f, l1 >= 0 ? x[2 * c + 1] * pw[max(l1, 0)] : 0.f);
+        }
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + quad) : "memory");  // the lanes' other columns have been read
+        tmem_st16(tSC + lane_off + c0 / 2, p);
+        fence_before();
+      } else {
+        wait(&bar.qk_full, ph);
+      }
+      if (!STATE_ONLY) wait(&bar.qk_full, ph);
+      wait(&bar.v_full, ph);
+      if (n < CT) {  // tokens past the end hold anything; 0 times anything must be 0
+        for (int u = threadIdx.x; u < (CT - n) * 16; u += kWorkers * 32)
+          *reinterpret_cast<uint4*>(smem + kV + unit_at(n + u / 16, u % 16, CT)) = make_uint4(0, 0, 0, 0);
+        fence_async();
+        asm volatile("bar.sync 5, 512;" ::: "memory");
+      }
+      if (!STATE_ONLY) arrive(&bar.p_ready);
+#pragma unroll 1
+      for (int j = 0; j < CT / kPart; ++j) {
+        const int use = i * (CT / kPart) + j;
+        if (use >= 2) wait(&bar.kp_free[j & 1], ((use >> 1) - 1) & 1);
+        const int r = threadIdx.x >> 4, u = threadIdx.x & 15, t = j * kPart + r;  // 32 tokens x 16 units
+        uint4 v = make_uint4(0, 0, 0, 0);
+        float w = 0.f;
+        if (t < n) {
+          v = *reinterpret_cast<const uint4*>(smem + kK + unit_at(t, u, CT));
+          w = pw[n - 1 - t];
+        }
+        const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+        uint32_t out[3][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f2 = la::unpack2(in[e]);
+          uint32_t x[3];
+          la::split(f2.x * w, f2.y * w, x);
+          out[0][e] = x[0], out[1][e] = x[1], out[2][e] = x[2];
+        }
+        char* dst = smem + kKp + (j & 1) * 3 * kPartBytes + unit_at(r, u, kPart);
+#pragma unroll
+        for (int m = 0; m < 3; ++m)
+          *reinterpret_cast<uint4*>(dst + m * kPartBytes) = make_uint4(out[m][0], out[m][1], out[m][2], out[m][3]);
+        fence_async();
+        arrive(&bar.kp_ready[j & 1]);
+      }
+      arrive(&bar.k_free);
+      wait(&bar.dl_done, ph);
+      fence_after();
+      {
+        const float keep = pw[n];
+#pragma unroll
+        for (int c = 0; c < 32; c += 16) {
+          float x[16];
+          tmem_ld16(tDL + lane_off + c0 + c, x);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) S[c + e] = fmaf(S[c + e], keep, x[e]);
+        }
+        fence_before();
+      }
+      if constexpr (!STATE_ONLY) {
+        wait(&bar.in_done, ph);
+        if (i + 1 < chunks) publish();
+        wait(&bar.ot_done, ph);
+        fence_after();
+        uint32_t out[16];
+        const float d = pw[row + 1] * a.scale;
+#pragma unroll
+        for (int c = 0; c < 32; c += 16) {
+          float x[16], y[16];
+          tmem_ld16(tIN + lane_off + c0 + c, x);
+          tmem_ld16(tOT + lane_off + c0 + c, y);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float v0 = fmaf(x[2 * e], d, y[2 * e] * a.scale), v1 = fmaf(x[2 * e + 1], d, y[2 * e + 1] * a.scale);
+            out[c / 2 + e] = ok ? la::pack2(v0, v1) : la::pack2(nan, nan);
+          }
+        }
+        fence_before();
+        arrive(&bar.o_read);
+        if (row < n) {
+          bf16* dst = row_ptr<bf16>(a.o, b, begin + (int64_t)i * CT + row, h) + c0;
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (c0 + u * 8 < a.f)
+              *reinterpret_cast<uint4*>(dst + u * 8) = make_uint4(out[4 * u], out[4 * u + 1], out[4 * u + 2], out[4 * u + 3]);
+        }
+      }
+    }
+    float* dst = STATE_ONLY ? a.seg_out + (bh * a.nseg + seg) * elems
+                 : a.state_out && seg == a.nseg - 1 ? a.state_out + bh * elems : nullptr;
+    if (dst && row < a.e) {
+#pragma unroll
+      for (int c = 0; c < 32; ++c)
+        if (c0 + c < a.f) dst[row * a.si + (c0 + c) * a.sj] = ok ? S[c] : nan;
+    }
+    if constexpr (!STATE_ONLY) {  // rows past the length
+      const int units = a.f / 8;
+      for (int64_t u = threadIdx.x; u < (int64_t)(stop - begin - len) * units; u += kWorkers * 32)
+        *reinterpret_cast<uint4*>(row_ptr<bf16>(a.o, b, begin + len + u / units, h) + u % units * 8) = make_uint4(0, 0, 0, 0);
+    }
+  }
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == kWorkers) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+  }
+}
+
+// A [batch][token][head][d] view as a map of boxes of 64 x 128 tokens.  Fails
+// (false) where TMA cannot read it: a stride of zero on an axis longer than one.
+inline bool view_map(CUtensorMap* m, const TmpcSeqView& v, int d, int heads, int T, int B) {
+  const gemm::EncodeFn fn = gemm::encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)T, (cuuint64_t)B};
+  const int64_t st[3] = {v.head, v.token, v.batch};
+  cuuint64_t strides[3];
+  for (int i = 0; i < 3; ++i) {
+    int64_t s = st[i] * 2;
+    if (dims[i + 1] == 1) s = (int64_t)((d + 7) / 8) * 16;  // never used
+    if (s <= 0 || s >= (int64_t)1 << 40) return false;
+    strides[i] = (cuuint64_t)s;
+  }
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)CT, 1}, es[4] = {1, 1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, v.ptr, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool STATE_ONLY>
+int launch(const Maps& maps, Args a, int B, cudaStream_t st) {
+  const int rc = allow_smem<kernel<STATE_ONLY>>(kSmem);
+  if (rc) return rc;
+  a.polls = transfer_poll_limit().load();
+  kernel<STATE_ONLY><<<(unsigned)((int64_t)B * a.nseg * a.H), kThreads, kSmem, st>>>(maps, a);
+  return (int)cudaPeekAtLastError();
+}
+
+}  // namespace tc
+}  // namespace seq
+}  // namespace tmpc

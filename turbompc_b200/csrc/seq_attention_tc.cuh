@@ -11,8 +11,11 @@
 // Each product has its own 128 columns of TMEM.  Warp 16 loads Q, K and V by TMA,
 // warp 17 issues the products, warps 0 .. 15 do everything between them: a
 // thread owns one TMEM lane (a token, or a row of S) and 32 columns.  K' goes
-// through two buffers of 32 tokens, so that forming a part and multiplying the
-// one before overlap.  With the matrix instructions issued from registers the
+// through two buffers of 32 tokens, and the workers' order (two parts of K', P,
+// the other two parts, the output, the state) leaves each product time to end
+// before its result is asked for; the next chunk is on its way into L2
+// meanwhile.  The first pass over a segment, which wants its state alone, has
+// the room to keep two chunks of K and V and two DL.  With the matrix instructions issued from registers the
 // same work is bound by them and by the operands' loads from shared memory (64
 // tokens of a 128 x 128 head: 12 thousand cycles per SM).
 //
@@ -36,17 +39,18 @@ constexpr int kPartBytes = kPart * 128 * 2;
 
 // Shared memory: Q, K, V, S in two terms, K' parts (two buffers of three terms).
 constexpr int kQ = 0, kK = kTile, kV = 2 * kTile, kS = 3 * kTile, kKp = 5 * kTile;
+// For the state alone: K, V of two chunks in the place of Q, K, V and S's first term.
 constexpr int kBars = kKp + 2 * 3 * kPartBytes;
-constexpr int kSmem = kBars + 1024 + 1024;  // barriers and powers of d; alignment
-static_assert(kSmem <= 227 * 1024, "");
 
 struct Bars {
-  uint64_t qk_full, v_full, sc_done, in_done, ot_done, dl_done, p_ready, s_ready, o_read, k_free, kp_ready[2], kp_free[2],
-      done;
+  uint64_t qk_full[2], v_full[2], k_free[2], dl_done[2], sc_done, in_done, ot_done, p_ready, s_ready, o_read, kp_ready[2],
+      kp_free[2], done;
   uint32_t tmem;
   int abort_flag;
-  float pw[CT + 1];
+  float pw[2 * CT + 1];  // d^(i - CT), 0 for i < CT (read, not used, past the diagonal)
 };
+constexpr int kSmem = kBars + (int)sizeof(Bars) + 1024;  // 1024: alignment
+static_assert(kSmem <= 227 * 1024, "");
 
 struct Args {
   TmpcSeqView o;
@@ -95,6 +99,12 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
+__device__ __forceinline__ void tma_prefetch_4d(const CUtensorMap* map, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global [%0, {%1, %2, %3, %4}];" ::"l"(map), "r"(x), "r"(y), "r"(z),
+               "r"(w)
+               : "memory");
+}
+
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // 16-byte unit u (0 .. 15, 8 elements each) of row r of a tile whose 64-wide boxes have `rows` rows.
@@ -125,15 +135,17 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
   const int chunks = (len + CT - 1) / CT;
   const float g2 = log2_decay(a.log_decay, h);
 
+  constexpr int NB = STATE_ONLY ? 2 : 1;  // chunks of K and V in shared memory
   if (threadIdx.x == 0) {
-    mbar_init(&bar.qk_full, 1), mbar_init(&bar.v_full, 1);
-    mbar_init(&bar.sc_done, 1), mbar_init(&bar.in_done, 1), mbar_init(&bar.ot_done, 1), mbar_init(&bar.dl_done, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar.qk_full[i], 1), mbar_init(&bar.v_full[i], 1), mbar_init(&bar.dl_done[i], 1);
+      mbar_init(&bar.k_free[i], kWorkers), mbar_init(&bar.kp_ready[i], kWorkers), mbar_init(&bar.kp_free[i], 1);
+    }
+    mbar_init(&bar.sc_done, 1), mbar_init(&bar.in_done, 1), mbar_init(&bar.ot_done, 1), mbar_init(&bar.done, 1);
     mbar_init(&bar.p_ready, kWorkers), mbar_init(&bar.s_ready, kWorkers), mbar_init(&bar.o_read, kWorkers);
-    mbar_init(&bar.k_free, kWorkers), mbar_init(&bar.done, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&bar.kp_ready[i], kWorkers), mbar_init(&bar.kp_free[i], 1);
     bar.abort_flag = 0;
   }
-  for (int i = threadIdx.x; i <= CT; i += kThreads) bar.pw[i] = exp2f(g2 * (float)i);
+  for (int i = threadIdx.x; i <= 2 * CT; i += kThreads) bar.pw[i] = i < CT ? 0.f : exp2f(g2 * (float)(i - CT));
   if (warp == kWorkers) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar.tmem)), "n"(512)
                  : "memory");
@@ -143,47 +155,60 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
   __syncthreads();
   fence_after();
   const uint32_t tmem = bar.tmem;
-  const uint32_t tSC = tmem, tIN = tmem + 128, tOT = tmem + 256, tDL = tmem + 384;
+  const uint32_t tSC = tmem, tIN = tmem + 128, tOT = tmem + 256, tDL = tmem + 384;  // and OT's for the second DL
+  auto k_tile = [&](int i) { return smem + (STATE_ONLY ? (i & 1) * 2 * kTile : kK); };
+  auto v_tile = [&](int i) { return smem + (STATE_ONLY ? (i & 1) * 2 * kTile + kTile : kV); };
+  auto dl_cols = [&](int i) { return tDL - (STATE_ONLY ? (i & 1) * 128 : 0); };
   bool ok = true;
   auto wait = [&](uint64_t* w, uint32_t parity) {
     if (ok) ok = gemm::wait(w, parity, a.polls, abort_flag);
     return ok;
   };
+  // chunk i's turn of a barrier per buffer
+  auto wait_buf = [&](uint64_t (&w)[2], int i) { return wait(&w[i % NB], (i / NB) & 1); };
 
   if (warp == kWorkers && lane == 0) {  // loads
-    int i = 0;
+    int i = 0, last_v = -1;
     for (; i < chunks; ++i) {
       const int t0 = begin + i * CT;
-      // K is free when its last part of K' is formed (and the scores are done, which p_ready of the same chunk waits
-      // for); Q when the read-out of the state is done; V when the state's update is.
-      if (i > 0 && !wait(&bar.k_free, (i - 1) & 1)) break;
+      // K is free when its last part of K' is formed (the scores are done by then); Q when the read-out of the state
+      // is done; V when the state's update is, the last product that reads it.
+      if (i >= NB && !wait_buf(bar.k_free, i - NB)) break;
       if (!STATE_ONLY && i > 0 && !wait(&bar.in_done, (i - 1) & 1)) break;
-      mbar_expect_tx(&bar.qk_full, (STATE_ONLY ? 1 : 2) * kTile);
+      uint64_t* full = &bar.qk_full[i % NB];
+      mbar_expect_tx(full, (STATE_ONLY ? 1 : 2) * kTile);
       for (int x = 0; x < 2; ++x) {
-        if (!STATE_ONLY) tma_load_4d(smem + kQ + x * (kTile / 2), &maps.q, x * 64, h, t0, b, &bar.qk_full);
-        tma_load_4d(smem + kK + x * (kTile / 2), &maps.k, x * 64, g, t0, b, &bar.qk_full);
+        if (!STATE_ONLY) tma_load_4d(smem + kQ + x * (kTile / 2), &maps.q, x * 64, h, t0, b, full);
+        tma_load_4d(k_tile(i) + x * (kTile / 2), &maps.k, x * 64, g, t0, b, full);
       }
-      if (i > 0 && !wait(&bar.dl_done, (i - 1) & 1)) {
-        mbar_wait_bounded(&bar.qk_full, i & 1, kTransferDrainPolls);
+      if (i >= NB && !wait_buf(bar.dl_done, i - NB)) {
+        ++i;
         break;
       }
-      mbar_expect_tx(&bar.v_full, kTile);
-      for (int x = 0; x < 2; ++x) tma_load_4d(smem + kV + x * (kTile / 2), &maps.v, x * 64, g, t0, b, &bar.v_full);
+      mbar_expect_tx(&bar.v_full[i % NB], kTile);
+      for (int x = 0; x < 2; ++x) tma_load_4d(v_tile(i) + x * (kTile / 2), &maps.v, x * 64, g, t0, b, &bar.v_full[i % NB]);
+      last_v = i;
+      if (i + 1 < chunks)
+        for (int x = 0; x < 2; ++x) {
+          if (!STATE_ONLY) tma_prefetch_4d(&maps.q, x * 64, h, t0 + CT, b);
+          tma_prefetch_4d(&maps.k, x * 64, g, t0 + CT, b);
+          tma_prefetch_4d(&maps.v, x * 64, g, t0 + CT, b);
+        }
     }
-    if (chunks > 0 && i > 0) {  // nothing may land after the block has left
-      mbar_wait_bounded(&bar.qk_full, (i - 1) & 1, kTransferDrainPolls);
-      mbar_wait_bounded(&bar.v_full, (i - 1) & 1, kTransferDrainPolls);
-    }
+    // nothing may land after the block has left
+    for (int k = max(i - NB, 0); k < i; ++k)
+      mbar_wait_bounded(&bar.qk_full[k % NB], (k / NB) & 1, kTransferDrainPolls);
+    for (int k = max(last_v + 1 - NB, 0); k <= last_v; ++k)
+      mbar_wait_bounded(&bar.v_full[k % NB], (k / NB) & 1, kTransferDrainPolls);
   } else if (warp == kWorkers + 1 && lane == 0) {  // products, 128 x 128, K 16 each
     constexpr uint32_t kBase = 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(128 / 8) << 17 | (uint32_t)(128 / 16) << 24;
     constexpr uint32_t kAmn = 1u << 15, kBmn = 1u << 16;
-    const uint32_t sq = smem_u32(smem + kQ), sk = smem_u32(smem + kK), sv = smem_u32(smem + kV),
-                   ss = smem_u32(smem + kS), skp = smem_u32(smem + kKp);
+    const uint32_t sq = smem_u32(smem + kQ), ss = smem_u32(smem + kS), skp = smem_u32(smem + kKp);
     auto krow = [](int k) { return (k >> 2) * (kTile / 2) + (k & 3) * 32; };  // K-major tile: 4 steps per 64-wide box
     for (int i = 0; i < chunks && ok; ++i) {
-      const uint32_t ph = i & 1;
+      const uint32_t ph = i & 1, sk = smem_u32(k_tile(i)), sv = smem_u32(v_tile(i));
       if constexpr (!STATE_ONLY) {
-        if (!wait(&bar.qk_full, ph)) break;
+        if (!wait_buf(bar.qk_full, i)) break;
         fence_after();
 #pragma unroll
         for (int k = 0; k < 8; ++k)
@@ -198,15 +223,17 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
             mma_f16(tIN, desc(sq + krow(k), 16, 1024), desc(ss + m * kTile + k * 2048, kTile / 2, 1024), kBase | kBmn,
                     m + k > 0);
         mma_commit(&bar.in_done);
-        if (!wait(&bar.v_full, ph) || !wait(&bar.p_ready, ph)) break;
-        fence_after();
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          mma_tmem_a(tOT, tSC + k * 8, desc(sv + k * 2048, kTile / 2, 1024), kBase | kBmn, k > 0);
-        mma_commit(&bar.ot_done);
       }
-      if (STATE_ONLY && !wait(&bar.v_full, ph)) break;
+      if (!wait_buf(bar.v_full, i)) break;
       for (int j = 0; j < CT / kPart; ++j) {
+        if (!STATE_ONLY && j == 2) {
+          if (!wait(&bar.p_ready, ph)) break;
+          fence_after();
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            mma_tmem_a(tOT, tSC + k * 8, desc(sv + k * 2048, kTile / 2, 1024), kBase | kBmn, k > 0);
+          mma_commit(&bar.ot_done);
+        }
         if (!wait(&bar.kp_ready[j & 1], ((i * (CT / kPart) + j) >> 1) & 1)) break;
         fence_after();
         const uint32_t kp = skp + (j & 1) * 3 * kPartBytes;
@@ -214,11 +241,11 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
         for (int m = 0; m < 3; ++m)
 #pragma unroll
           for (int k = 0; k < kPart / 16; ++k)
-            mma_f16(tDL, desc(kp + m * kPartBytes + k * 2048, kPartBytes / 2, 1024),
+            mma_f16(dl_cols(i), desc(kp + m * kPartBytes + k * 2048, kPartBytes / 2, 1024),
                     desc(sv + j * kPart * 128 + k * 2048, kTile / 2, 1024), kBase | kAmn | kBmn, j + m + k > 0);
         mma_commit(&bar.kp_free[j & 1]);
       }
-      if (ok) mma_commit(&bar.dl_done);
+      if (ok) mma_commit(&bar.dl_done[i % NB]);
     }
     if (!ok) {  // TMEM may be freed only after the products in flight
       mma_commit(&bar.done);
@@ -228,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
     const int quad = warp & 3, c0 = (warp >> 2) * 32;
     const int row = quad * 32 + lane;  // token of the chunk, or row of the state
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
-    const float* pw = bar.pw;
+    const float* pw = bar.pw + CT;
     const float nan = __int_as_float(0x7fffffff);
     const int64_t bh = (int64_t)b * a.H + h, elems = (int64_t)a.e * a.f;
     auto arrive = [&](uint64_t* w) {
@@ -260,82 +287,90 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
       arrive(&bar.s_ready);
     };
     if (!STATE_ONLY && chunks > 0) publish();
+    // part j of K' of chunk i, 32 tokens x 16 units: one unit per thread
+    auto part = [&](int i, int j, int n) {
+      const int use = i * (CT / kPart) + j;
+      if (use >= 2) wait(&bar.kp_free[j & 1], ((use >> 1) - 1) & 1);
+      const int r = threadIdx.x >> 4, u = threadIdx.x & 15, t = j * kPart + r;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      float w = 0.f;
+      if (t < n) {
+        v = *reinterpret_cast<const uint4*>(k_tile(i) + unit_at(t, u, CT));
+        w = pw[n - 1 - t];
+      }
+      const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+      uint32_t out[3][4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f2 = la::unpack2(in[e]);
+        uint32_t x[3];
+        la::split(f2.x * w, f2.y * w, x);
+        out[0][e] = x[0], out[1][e] = x[1], out[2][e] = x[2];
+      }
+      char* dst = smem + kKp + (j & 1) * 3 * kPartBytes + unit_at(r, u, kPart);
+#pragma unroll
+      for (int m = 0; m < 3; ++m)
+        *reinterpret_cast<uint4*>(dst + m * kPartBytes) = make_uint4(out[m][0], out[m][1], out[m][2], out[m][3]);
+      fence_async();
+      arrive(&bar.kp_ready[j & 1]);
+    };
+    // S <- d^n S + DL of chunk i
+    auto advance = [&](int i) {
+      wait_buf(bar.dl_done, i);
+      fence_after();
+      const float keep = pw[min(CT, len - i * CT)];
+#pragma unroll
+      for (int c = 0; c < 32; c += 16) {
+        float x[16];
+        tmem_ld16(dl_cols(i) + lane_off + c0 + c, x);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) S[c + e] = fmaf(S[c + e], keep, x[e]);
+      }
+      fence_before();
+    };
     for (int i = 0; i < chunks; ++i) {
       const uint32_t ph = i & 1;
       const int n = min(CT, len - i * CT);
+      wait_buf(bar.qk_full, i);
+      if (n < CT) {  // tokens past the end hold anything; 0 times anything must be 0
+        wait_buf(bar.v_full, i);
+        for (int u = threadIdx.x; u < (CT - n) * 16; u += kWorkers * 32)
+          *reinterpret_cast<uint4*>(v_tile(i) + unit_at(n + u / 16, u % 16, CT)) = make_uint4(0, 0, 0, 0);
+        fence_async();
+        asm volatile("bar.sync 5, 512;" ::: "memory");
+      }
+      part(i, 0, n);
+      part(i, 1, n);
       if constexpr (!STATE_ONLY) {  // the scores become P, in their own columns of TMEM
         wait(&bar.sc_done, ph);
         fence_after();
-        float x[32];
-        tmem_ld16(tSC + lane_off + c0, *reinterpret_cast<float(*)[16]>(&x[0]));
-        tmem_ld16(tSC + lane_off + c0 + 16, *reinterpret_cast<float(*)[16]>(&x[16]));
-        tmem_wait_ld();
+        const int lag = row - c0;
+        const float* w = pw + lag;
         uint32_t p[16];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const int l0 = row - (c0 + 2 * c), l1 = l0 - 1;
-          p[c] = la::pack2(l0 >= 0 ? x[2 * c] * pw[max(l0, 0)] : 0.f, l1 >= 0 ? x[2 * c + 1] * pw[max(l1, 0)] : 0.f);
+        for (int c = 0; c < 32; c += 16) {
+          float x[16];
+          tmem_ld16(tSC + lane_off + c0 + c, x);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int k = c + 2 * e;  // keys past the query's token, and past the end, are left out whatever they hold
+            p[k / 2] = la::pack2(lag >= k ? x[2 * e] * w[-k] : 0.f, lag >= k + 1 ? x[2 * e + 1] * w[-k - 1] : 0.f);
+          }
         }
         asm volatile("bar.sync %0, 128;" ::"r"(1 + quad) : "memory");  // the lanes' other columns have been read
         tmem_st16(tSC + lane_off + c0 / 2, p);
         fence_before();
+        arrive(&bar.p_ready);
+      }
+      part(i, 2, n);
+      part(i, 3, n);
+      arrive(&bar.k_free[i % NB]);
+      if constexpr (STATE_ONLY) {
+        if (i > 0) advance(i - 1);
       } else {
-        wait(&bar.qk_full, ph);
-      }
-      if (!STATE_ONLY) wait(&bar.qk_full, ph);
-      wait(&bar.v_full, ph);
-      if (n < CT) {  // tokens past the end hold anything; 0 times anything must be 0
-        for (int u = threadIdx.x; u < (CT - n) * 16; u += kWorkers * 32)
-          *reinterpret_cast<uint4*>(smem + kV + unit_at(n + u / 16, u % 16, CT)) = make_uint4(0, 0, 0, 0);
-        fence_async();
-        asm volatile("bar.sync 5, 512;" ::: "memory");
-      }
-      if (!STATE_ONLY) arrive(&bar.p_ready);
-#pragma unroll 1
-      for (int j = 0; j < CT / kPart; ++j) {
-        const int use = i * (CT / kPart) + j;
-        if (use >= 2) wait(&bar.kp_free[j & 1], ((use >> 1) - 1) & 1);
-        const int r = threadIdx.x >> 4, u = threadIdx.x & 15, t = j * kPart + r;  // 32 tokens x 16 units
-        uint4 v = make_uint4(0, 0, 0, 0);
-        float w = 0.f;
-        if (t < n) {
-          v = *reinterpret_cast<const uint4*>(smem + kK + unit_at(t, u, CT));
-          w = pw[n - 1 - t];
-        }
-        const uint32_t in[4] = {v.x, v.y, v.z, v.w};
-        uint32_t out[3][4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f2 = la::unpack2(in[e]);
-          uint32_t x[3];
-          la::split(f2.x * w, f2.y * w, x);
-          out[0][e] = x[0], out[1][e] = x[1], out[2][e] = x[2];
-        }
-        char* dst = smem + kKp + (j & 1) * 3 * kPartBytes + unit_at(r, u, kPart);
-#pragma unroll
-        for (int m = 0; m < 3; ++m)
-          *reinterpret_cast<uint4*>(dst + m * kPartBytes) = make_uint4(out[m][0], out[m][1], out[m][2], out[m][3]);
-        fence_async();
-        arrive(&bar.kp_ready[j & 1]);
-      }
-      arrive(&bar.k_free);
-      wait(&bar.dl_done, ph);
-      fence_after();
-      {
-        const float keep = pw[n];
-#pragma unroll
-        for (int c = 0; c < 32; c += 16) {
-          float x[16];
-          tmem_ld16(tDL + lane_off + c0 + c, x);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 16; ++e) S[c + e] = fmaf(S[c + e], keep, x[e]);
-        }
-        fence_before();
-      }
-      if constexpr (!STATE_ONLY) {
         wait(&bar.in_done, ph);
-        if (i + 1 < chunks) publish();
         wait(&bar.ot_done, ph);
         fence_after();
         uint32_t out[16];
@@ -361,8 +396,11 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
             if (c0 + u * 8 < a.f)
               *reinterpret_cast<uint4*>(dst + u * 8) = make_uint4(out[4 * u], out[4 * u + 1], out[4 * u + 2], out[4 * u + 3]);
         }
+        if (i + 1 < chunks || a.state_out) advance(i);
+        if (i + 1 < chunks) publish();  // the read-out of the old state has ended
       }
     }
+    if (STATE_ONLY && chunks > 0) advance(chunks - 1);
     float* dst = STATE_ONLY ? a.seg_out + (bh * a.nseg + seg) * elems
                  : a.state_out && seg == a.nseg - 1 ? a.state_out + bh * elems : nullptr;
     if (dst && row < a.e) {

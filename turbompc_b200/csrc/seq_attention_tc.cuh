@@ -76,8 +76,8 @@ __device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo, uint32_t s
 
 __device__ __forceinline__ void mma_tmem_a(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "{\n .reg .pred p, e;\n setp.ne.u32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
       "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
       : "memory");
 }
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   Bars& bar = *reinterpret_cast<Bars*>(smem + kBars);
   volatile int* abort_flag = &bar.abort_flag;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   const int h = blockIdx.x % a.H, seg = blockIdx.x / a.H % a.nseg, b = blockIdx.x / a.H / a.nseg;
   const int g = h / (a.H / a.G);
@@ -200,7 +200,11 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
       mbar_wait_bounded(&bar.qk_full[k % NB], (k / NB) & 1, kTransferDrainPolls);
     for (int k = max(last_v + 1 - NB, 0); k <= last_v; ++k)
       mbar_wait_bounded(&bar.v_full[k % NB], (k / NB) & 1, kTransferDrainPolls);
-  } else if (warp == kWorkers + 1 && lane == 0) {  // products, 128 x 128, K 16 each
+  } else if (warp == kWorkers + 1) {  // products, 128 x 128, K 16 each
+    auto wwait = [&](uint64_t* w, uint32_t parity) {
+      if (ok) ok = gemm::warp_wait(w, parity, a.polls, abort_flag);
+      return ok;
+    };
     constexpr uint32_t kBase = 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(128 / 8) << 17 | (uint32_t)(128 / 16) << 24;
     constexpr uint32_t kAmn = 1u << 15, kBmn = 1u << 16;
     const uint32_t sq = smem_u32(smem + kQ), ss = smem_u32(smem + kS), skp = smem_u32(smem + kKp);
@@ -208,13 +212,13 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
     for (int i = 0; i < chunks && ok; ++i) {
       const uint32_t ph = i & 1, sk = smem_u32(k_tile(i)), sv = smem_u32(v_tile(i));
       if constexpr (!STATE_ONLY) {
-        if (!wait_buf(bar.qk_full, i)) break;
+        if (!wwait(&bar.qk_full[i % NB], (i / NB) & 1)) break;
         fence_after();
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           mma_f16(tSC, desc(sq + krow(k), 16, 1024), desc(sk + krow(k), 16, 1024), kBase, k > 0);
         mma_commit(&bar.sc_done);
-        if (!wait(&bar.s_ready, ph) || (i > 0 && !wait(&bar.o_read, (i - 1) & 1))) break;
+        if (!wwait(&bar.s_ready, ph) || (i > 0 && !wwait(&bar.o_read, (i - 1) & 1))) break;
         fence_after();
 #pragma unroll
         for (int m = 0; m < 2; ++m)
@@ -224,17 +228,17 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
                     m + k > 0);
         mma_commit(&bar.in_done);
       }
-      if (!wait_buf(bar.v_full, i)) break;
+      if (!wwait(&bar.v_full[i % NB], (i / NB) & 1)) break;
       for (int j = 0; j < CT / kPart; ++j) {
         if (!STATE_ONLY && j == 2) {
-          if (!wait(&bar.p_ready, ph)) break;
+          if (!wwait(&bar.p_ready, ph)) break;
           fence_after();
 #pragma unroll
           for (int k = 0; k < 8; ++k)
             mma_tmem_a(tOT, tSC + k * 8, desc(sv + k * 2048, kTile / 2, 1024), kBase | kBmn, k > 0);
           mma_commit(&bar.ot_done);
         }
-        if (!wait(&bar.kp_ready[j & 1], ((i * (CT / kPart) + j) >> 1) & 1)) break;
+        if (!wwait(&bar.kp_ready[j & 1], ((i * (CT / kPart) + j) >> 1) & 1)) break;
         fence_after();
         const uint32_t kp = skp + (j & 1) * 3 * kPartBytes;
 #pragma unroll
@@ -389,12 +393,29 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
         }
         fence_before();
         arrive(&bar.o_read);
-        if (row < n) {
-          bf16* dst = row_ptr<bf16>(a.o, b, begin + (int64_t)i * CT + row, h) + c0;
+        // Four lanes trade 16-byte units, so that a store covers 64 bytes of 8 rows, not 16 of 32 (which took 2900 of
+        // a chunk's 14000 cycles): unit u of the lane's own row -> its unit (lane & 3) of row 4 (lane / 4) + u.
+#pragma unroll
+        for (int bit = 1; bit < 4; bit <<= 1)
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            if (c0 + u * 8 < a.f)
-              *reinterpret_cast<uint4*>(dst + u * 8) = make_uint4(out[4 * u], out[4 * u + 1], out[4 * u + 2], out[4 * u + 3]);
+            if (!(u & bit))
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                uint32_t &lo = out[4 * u + e], &hi = out[4 * (u | bit) + e];
+                const bool up = lane & bit;
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? lo : hi, bit);
+                if (up) lo = got;
+                else hi = got;
+              }
+        {
+          const int col = c0 + (lane & 3) * 8, row4 = row & ~3;
+          bf16* dst = row_ptr<bf16>(a.o, b, begin + (int64_t)i * CT + row4, h) + col;
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (row4 + u < n && col < a.f)
+              *reinterpret_cast<uint4*>(dst + u * a.o.token) =
+                  make_uint4(out[4 * u], out[4 * u + 1], out[4 * u + 2], out[4 * u + 3]);
         }
         if (i + 1 < chunks || a.state_out) advance(i);
         if (i + 1 < chunks) publish();  // the read-out of the old state has ended

@@ -128,17 +128,22 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, bool mn_major) {
   return (uint64_t)((addr & 0x3ffff) >> 4) | lbo << 16 | sbo << 32 | (uint64_t)1 << 46 | swizzle << 61;
 }
 
+// Products and commits are issued by one elected lane of a converged warp: with
+// the whole warp in the loop its descriptors stay in uniform registers, where the
+// instruction wants them.
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "{\n .reg .pred p, e;\n setp.ne.u32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
       : "memory");
 }
 
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+  asm volatile(
+      "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
+      : "memory");
 }
 
 // 16 consecutive accumulator columns of this thread's TMEM lane.
@@ -171,6 +176,11 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, uint32_t po
   }
   *abort_flag = 1;
   return false;
+}
+
+// The same for a converged warp that has to stay so.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t polls, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, wait(bar, parity, polls, abort_flag));
 }
 
 // A warp's chunk of an output (or of dh): 32 rows, one per lane, of CH elements,
@@ -334,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
   char* epi_mem = smem + ST * F::kStage;
   Barriers& bar = *reinterpret_cast<Barriers*>(epi_mem + F::kEpi);
   volatile int* abort_flag = &bar.abort_flag;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) mbar_init(&bar.full[i], 1), mbar_init(&bar.empty[i], 1);
@@ -402,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
     // Nothing may land after the block has left: the last copies of every stage.
     for (uint32_t i = n > ST ? n - ST : 0; i < n; ++i)
       mbar_wait_bounded(&bar.full[i % ST], (i / ST) & 1, kTransferDrainPolls);
-  } else if (warp == 1 && lane == 0) {  // products
+  } else if (warp == 1) {  // products
     int64_t m0;
     int n0, kb0, kb1, split;
     uint32_t n = 0, accs = 0;
@@ -412,11 +422,11 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
       for (int seg = kb0; ok && seg < kb1; seg = kb1 - seg > F::kSeg ? seg + F::kSeg : kb1, ++accs) {
         const int end = kb1 - seg > F::kSeg ? seg + F::kSeg : kb1;
         const uint32_t buf = accs & 1, d = tmem + buf * NT;
-        if (accs >= 2 && !(ok = wait(&bar.acc_empty[buf], (accs / 2 - 1) & 1, p.polls, abort_flag))) break;
+        if (accs >= 2 && !(ok = warp_wait(&bar.acc_empty[buf], (accs / 2 - 1) & 1, p.polls, abort_flag))) break;
         fence_after();
         for (int kb = seg; kb < end; ++kb, ++n) {
           const int s = n % ST;
-          if (!(ok = wait(&bar.full[s], (n / ST) & 1, p.polls, abort_flag))) break;
+          if (!(ok = warp_wait(&bar.full[s], (n / ST) & 1, p.polls, abort_flag))) break;
           fence_after();
           const uint32_t a = smem_u32(smem + s * F::kStage), b = a + NC * kA;
 #pragma unroll

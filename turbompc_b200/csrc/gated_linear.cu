@@ -21,22 +21,49 @@ namespace seq {
 
 inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
-// src [rows][cols] as NC bfloat16 components [NC][rows][pitch].
+// x, w_gate and w_up as bfloat16 components [components][rows][pitch], one launch:
+// rows 0 .. n0 - 1 are x's, the next f w_gate's, the last f w_up's.  Four columns
+// per thread.
 template <typename T>
-__global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ src, bf16* __restrict__ dst, int64_t rows,
-                                                  int cols, int pitch) {
-  const int64_t n = rows * cols;
+struct PackArgs {
+  const T* src[3];
+  bf16* dst[3];
+  int64_t rows[3];
+  int cols, pitch;
+  bool wide;  // rows of whole groups of four at aligned addresses
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) pack_kernel(const PackArgs<T> a) {
+  const int groups = (a.cols + 3) / 4;
+  const int64_t n = (a.rows[0] + a.rows[1] + a.rows[2]) * groups;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / cols;
-    const int64_t o = r * pitch + (i - r * cols);
-    if constexpr (sizeof(T) == 2) {
-      dst[o] = src[i];
+    int64_t r = i / groups;
+    const int c = (int)(i - r * groups) * 4;
+    int w = 0;
+    if (r >= a.rows[0]) r -= a.rows[0], w = 1;
+    if (w == 1 && r >= a.rows[1]) r -= a.rows[1], w = 2;
+    const T* src = a.src[w] + r * a.cols + c;
+    bf16* dst = a.dst[w] + r * a.pitch + c;  // 8-byte aligned: the pitch is a multiple of 8
+    Pack<T, 4> v;
+    if (a.wide) {
+      v = *reinterpret_cast<const Pack<T, 4>*>(src);
     } else {
-      bf16 c[3];
-      gemm::split3(src[i], c);
-      dst[o] = c[0];
-      dst[o + rows * pitch] = c[1];
-      dst[o + 2 * rows * pitch] = c[2];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v.v[e] = c + e < a.cols ? src[e] : from_f<T>(0.f);
+    }
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<Pack<T, 4>*>(dst) = v;
+    } else {
+      Pack<bf16, 4> o[3];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        bf16 s[3];
+        gemm::split3(v.v[e], s);
+        o[0].v[e] = s[0], o[1].v[e] = s[1], o[2].v[e] = s[2];
+      }
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<Pack<bf16, 4>*>(dst + k * a.rows[w] * a.pitch) = o[k];
     }
   }
 }
@@ -130,12 +157,11 @@ template <typename T>
 Operands pack_operands(const Plan& p, int64_t rows, int d, int f, const T* x, const T* wg, const T* wu, char* ws,
                        cudaStream_t st) {
   if (p.direct) return {x, wg, wu};
-  auto pack = [&](const T* src, int64_t off, int64_t n) {
-    const int64_t blocks = std::min<int64_t>((n * d + 255) / 256, 8 * (int64_t)sm_count());
-    pack_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(src, reinterpret_cast<bf16*>(ws + off), n, d, p.dp);
-    return (const void*)(ws + off);
-  };
-  return {pack(x, p.x, rows), pack(wg, p.wg, f), pack(wu, p.wu, f)};
+  auto at = [&](int64_t off) { return reinterpret_cast<bf16*>(ws + off); };
+  const PackArgs<T> a{{x, wg, wu}, {at(p.x), at(p.wg), at(p.wu)}, {rows, f, f}, d, p.dp, d % 4 == 0};
+  const int64_t blocks = std::min<int64_t>(((rows + 2 * (int64_t)f) * ((d + 3) / 4) + 255) / 256, 16 * (int64_t)sm_count());
+  pack_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(a);
+  return {at(p.x), at(p.wg), at(p.wu)};
 }
 
 // The two-projection kernel: forward, or dg | du.

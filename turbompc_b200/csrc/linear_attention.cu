@@ -272,18 +272,30 @@ __global__ void __launch_bounds__(256) scan_kernel(const Args p, float* seg, flo
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
   const float g2 = log2_decay(p.log_decay, h);
   float s = first ? first[bh * elems + i] : 0.f, m = 0.f;
-  for (int k = 0; k < p.nseg; ++k) {
-    const int q = REV ? p.nseg - 1 - k : k;
-    const int64_t at = (bh * p.nseg + q) * elems + i;
-    const int n = min(max(len - q * p.seg_len, 0), p.seg_len);
-    const float w = exp2f(g2 * (float)n), own = seg[at];
-    seg[at] = s;
-    if constexpr (LOG) {
-      const float own_m = segm[at];
-      segm[at] = m;
-      m = fmaf(w, fmaf((float)n, s, m), own_m);
-    }
-    s = fmaf(w, s, own);
+  const int64_t base = bh * p.nseg * elems + i;
+  constexpr int N = 8;  // segments requested before the first is used
+  for (int k0 = 0; k0 < p.nseg; k0 += N) {
+    float own[N], own_m[LOG ? N : 1];
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (k0 + k < p.nseg) {
+        const int64_t at = base + (REV ? p.nseg - 1 - k0 - k : k0 + k) * elems;
+        own[k] = seg[at];
+        if constexpr (LOG) own_m[k] = segm[at];
+      }
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (k0 + k < p.nseg) {
+        const int q = REV ? p.nseg - 1 - k0 - k : k0 + k;
+        const int n = min(max(len - q * p.seg_len, 0), p.seg_len);
+        const float w = exp2f(g2 * (float)n);
+        seg[base + q * elems] = s;
+        if constexpr (LOG) {
+          segm[base + q * elems] = m;
+          m = fmaf(w, fmaf((float)n, s, m), own_m[k]);
+        }
+        s = fmaf(w, s, own[k]);
+      }
   }
 }
 

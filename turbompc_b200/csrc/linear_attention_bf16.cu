@@ -557,13 +557,21 @@ __global__ void __launch_bounds__(256) scan_kernel(const LinAttnArgs a, float* s
   const int len = seq_len(a, b);
   const float g2 = log2_decay(a.log_decay, h);
   float s = first ? first[bh * elems + i] : 0.f;
-  for (int k = 0; k < a.nseg; ++k) {
-    const int m = REV ? a.nseg - 1 - k : k;
-    float* p = seg + (bh * a.nseg + m) * elems + i;
-    const int n = min(max(len - m * a.seg_len, 0), a.seg_len);
-    const float own = *p;
-    *p = s;
-    s = fmaf(exp2f(g2 * (float)n), s, own);
+  float* base = seg + bh * a.nseg * elems + i;
+  constexpr int N = 8;  // segments requested before the first is used
+  for (int k0 = 0; k0 < a.nseg; k0 += N) {
+    float own[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (k0 + k < a.nseg) own[k] = base[(REV ? a.nseg - 1 - k0 - k : k0 + k) * elems];
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (k0 + k < a.nseg) {
+        const int m = REV ? a.nseg - 1 - k0 - k : k0 + k;
+        const int n = min(max(len - m * a.seg_len, 0), a.seg_len);
+        base[m * elems] = s;
+        s = fmaf(exp2f(g2 * (float)n), s, own[k]);
+      }
   }
 }
 

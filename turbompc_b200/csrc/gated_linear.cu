@@ -35,10 +35,10 @@ struct PackArgs {
 
 template <typename T>
 __global__ void __launch_bounds__(256) pack_kernel(const PackArgs<T> a) {
-  const int groups = (a.cols + 3) / 4;
+  const uint32_t groups = (a.cols + 3) / 4;
   const int64_t n = (a.rows[0] + a.rows[1] + a.rows[2]) * groups;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    int64_t r = i / groups;
+    int64_t r = n >> 32 ? i / groups : (uint32_t)i / groups;
     const int c = (int)(i - r * groups) * 4;
     int w = 0;
     if (r >= a.rows[0]) r -= a.rows[0], w = 1;
@@ -97,7 +97,7 @@ struct Plan {
   int64_t x, wg, wu, dgu, part, total;  // byte offsets in the workspace
 };
 
-// Splits of dW's token axis: the fewest that fill the SMs' last wave best, each
+// Splits of dW's token axis: the fewest that fill the last wave best, each
 // at least 8 blocks of 64 tokens.
 inline int dw_splits(int64_t rows, int64_t tiles, int sms) {
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(32, (rows + 511) / 512));
@@ -135,8 +135,9 @@ inline Plan make_plan(int64_t rows, int d, int f, int esize, bool backward) {
   }
   if (backward) {
     const int nt = esize == 4 ? tile_n<float>(d) : tile_n<bf16>(d);
-    const int64_t tiles = (2 * (int64_t)p.fp + gemm::BM - 1) / gemm::BM * ((d + nt - 1) / nt);
-    p.splits = dw_splits(rows, tiles, sm_count());
+    const int cg = nt == 256 ? 2 : 1;  // dW's tiles are pairs' where they are 256 wide
+    const int64_t tiles = (2 * (int64_t)p.fp + cg * gemm::BM - 1) / (cg * gemm::BM) * ((d + nt - 1) / nt);
+    p.splits = dw_splits(rows, tiles, sm_count() / cg);
     p.dgu = take(p.comps * rows * 2 * p.fp * 2);
     p.part = take((int64_t)p.splits * 2 * p.fp * d * 4);
   }
@@ -175,29 +176,36 @@ int dual(const Plan& p, const Operands& o, int64_t rows, int d, int f, int act, 
   q.fp = p.fp;
   q.kblocks = (d + BK - 1) / BK;
   q.splits = 1;
-  q.mtiles = (int)((rows + gemm::BM - 1) / gemm::BM);
   q.out = out;
   q.dh = dh;
   q.wide = wide_rows<T>(f, MODE == gemm::kDact ? (const void*)dh : out);
   const int cols = MODE == gemm::kDact ? p.fp : f;  // dg | du is written to its padded width
   gemm::Maps maps;
-  auto run = [&](auto NT) {
-    constexpr int nt = decltype(NT)::value;
+  auto run = [&](auto NT, auto G) {
+    constexpr int nt = decltype(NT)::value, CG = decltype(G)::value;
     int rc = gemm::make_map(&maps.a, o.x, d, rows, p.comps, p.dp, BK, gemm::BM);
     if (!rc) rc = gemm::make_map(&maps.b0, o.wg, d, f, p.comps, p.dp, BK, nt / 2);
     if (!rc) rc = gemm::make_map(&maps.b1, o.wu, d, f, p.comps, p.dp, BK, nt / 2);
     if (!rc && MODE == gemm::kDact)
-      rc = gemm::make_map(&maps.c, dgu, 2 * p.fp, rows, p.comps, 2 * p.fp, gemm::Config<T, MODE, nt>::kCols, 32);
+      rc = gemm::make_map(&maps.c, dgu, 2 * p.fp, rows, p.comps, 2 * p.fp, gemm::Config<T, MODE, nt, CG>::kCols, 32);
     if (rc) return rc;
+    q.mtiles = (int)((rows + CG * gemm::BM - 1) / (CG * gemm::BM));
     q.ntiles = (cols + nt / 2 - 1) / (nt / 2);
-    return act == TMPC_ACT_SILU ? gemm::launch<T, MODE, nt, TMPC_ACT_SILU>(maps, q, st)
-                                : gemm::launch<T, MODE, nt, TMPC_ACT_GELU>(maps, q, st);
+    return act == TMPC_ACT_SILU ? gemm::launch<T, MODE, nt, TMPC_ACT_SILU, CG>(maps, q, st)
+                                : gemm::launch<T, MODE, nt, TMPC_ACT_GELU, CG>(maps, q, st);
   };
-  // Few tokens: narrow tiles, so that the columns spread over more SMs.
+  using One = std::integral_constant<int, 1>;
+  // Wide tiles where they fill the SMs (of pairs of blocks in the bfloat16 forward
+  // pass: 777 against 819 us for 308224 x 512 x 1365; where the epilogue is longer
+  // than the products they cost more than they give, 991 against 968 us for dg | du
+  // and 27.5 against 22.1 us for d = 64); for few tokens narrow ones, so that the
+  // columns spread over more SMs.
   constexpr int kWide = sizeof(T) == 4 ? 128 : 256;
-  if ((int64_t)q.mtiles * ((cols + kWide / 2 - 1) / (kWide / 2)) >= sm_count())
-    return run(std::integral_constant<int, kWide>{});
-  return run(std::integral_constant<int, 64>{});
+  const int64_t tiles = ((rows + gemm::BM - 1) / gemm::BM) * ((cols + kWide / 2 - 1) / (kWide / 2));
+  if constexpr (sizeof(T) == 2 && MODE == gemm::kAct)
+    if (tiles >= sm_count() && d >= 256) return run(std::integral_constant<int, kWide>{}, std::integral_constant<int, 2>{});
+  if (tiles >= sm_count()) return run(std::integral_constant<int, kWide>{}, One{});
+  return run(std::integral_constant<int, 64>{}, One{});
 }
 
 template <typename T>
@@ -218,8 +226,8 @@ template <typename T, int MODE>
 int single(const gemm::Params& q0, int d, const void* a, int64_t a_inner, int64_t a_outer, int64_t a_pitch,
            const void* b0, const void* b1, int64_t b_outer, int64_t b_pitch, int comps, cudaStream_t st) {
   constexpr int BK = gemm::kBK<T>;
-  auto run = [&](auto NT) {
-    constexpr int nt = decltype(NT)::value;
+  auto run = [&](auto NT, auto G) {
+    constexpr int nt = decltype(NT)::value, CG = decltype(G)::value;
     gemm::Params q = q0;
     gemm::Maps maps;
     int rc = MODE == gemm::kDw ? gemm::make_map(&maps.a, a, a_inner, a_outer, comps, a_pitch, 64, BK)
@@ -227,15 +235,20 @@ int single(const gemm::Params& q0, int d, const void* a, int64_t a_inner, int64_
     if (!rc) rc = gemm::make_map(&maps.b0, b0, d, b_outer, comps, b_pitch, 64, BK);
     if (!rc) rc = gemm::make_map(&maps.b1, b1, d, b_outer, comps, b_pitch, 64, BK);
     if (rc) return rc;
-    q.mtiles = (int)((q.M + gemm::BM - 1) / gemm::BM);
+    q.mtiles = (int)((q.M + CG * gemm::BM - 1) / (CG * gemm::BM));
     q.ntiles = (d + nt - 1) / nt;
-    return gemm::launch<T, MODE, nt, TMPC_ACT_SILU>(maps, q, st);
+    return gemm::launch<T, MODE, nt, TMPC_ACT_SILU, CG>(maps, q, st);
   };
+  using One = std::integral_constant<int, 1>;
   const int nt = tile_n<T>(d);
-  if constexpr (sizeof(T) == 2)
-    if (nt == 256) return run(std::integral_constant<int, 256>{});
-  if (nt == 128) return run(std::integral_constant<int, 128>{});
-  return run(std::integral_constant<int, 64>{});
+  if constexpr (sizeof(T) == 2) {
+    if (nt == 256 && MODE == gemm::kDw) return run(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+    if (nt == 256 && (q0.M + 127) / 128 * ((d + 255) / 256) >= sm_count())
+      return run(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+    if (nt == 256) return run(std::integral_constant<int, 256>{}, One{});
+  }
+  if (nt == 128) return run(std::integral_constant<int, 128>{}, One{});
+  return run(std::integral_constant<int, 64>{}, One{});
 }
 
 template <typename T>

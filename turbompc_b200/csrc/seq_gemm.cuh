@@ -10,9 +10,16 @@
 // float every 32 terms get an accumulator of their own, which the epilogue
 // warps add up in registers.
 //
-// A block computes 128 x NT tiles: warp 0 feeds a ring of stages by TMA, warp 1
+// A block (CG = 1) computes 128 x NT tiles, a pair of blocks (CG = 2) 256 x NT ones:
+// each holds its own 128 rows of A, half of B and 128 rows of the accumulator,
+// and the pair's first block issues the products of both.  With bfloat16 and NT =
+// 256 one block's operands fill the shared memory's bandwidth (A and B written
+// and read once per product: 48 KB per 512 cycles each way); a pair moves two
+// thirds of that.
+//
+// Within a block, warp 0 feeds a ring of stages by TMA, warp 1
 // issues the products (M 128, N NT, K 16 each) into one of two TMEM
-// accumulators, warps 4 .. 11 take a finished accumulator through the epilogue
+// accumulators, warps 4 .. take a finished accumulator through the epilogue
 // while the next one is computed.  Every wait is bounded: a wait that runs out
 // sets the block's abort flag, the copies and products in flight are drained
 // (bounded again), TMEM is freed, and the outputs not computed are stored as NaN.
@@ -31,8 +38,6 @@ constexpr int BM = 128;
 // K elements per stage: 128-byte rows for bfloat16; 64-byte rows of three components for float.
 template <typename T>
 constexpr int kBK = sizeof(T) == 2 ? 64 : 32;
-constexpr int kThreads = 384;
-constexpr int kEpiWarps = 8;
 constexpr int kSmemTotal = 227 * 1024;
 
 enum Mode {
@@ -103,12 +108,35 @@ __device__ __forceinline__ void split3(float x, bf16 (&c)[3]) {
   c[2] = __ushort_as_bfloat16((unsigned short)(__float_as_uint(r2) >> 16));
 }
 
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          smem_u32(dst)),
-      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-      : "memory");
+template <int CG>
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  else  // the barrier may be the other block's
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, "
+        "%4}], [%5];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+
+// The address of a shared variable in block `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer_addr(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int x, int y, int z, const void* src) {
@@ -131,19 +159,37 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, bool mn_major) {
 // Products and commits are issued by one elected lane of a converged warp: with
 // the whole warp in the loop its descriptors stay in uniform registers, where the
 // instruction wants them.
+template <int CG = 1>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
-  asm volatile(
-      "{\n .reg .pred p, e;\n setp.ne.u32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
-      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
-      : "memory");
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n .reg .pred p, e;\n setp.ne.u32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p, e;\n setp.ne.u32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+        " @e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+        : "memory");
 }
 
+// Arrives at bar (CG = 2: of both blocks) when the products issued so far are done.
+template <int CG = 1>
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile(
-      "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
-      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
-      : "memory");
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+        " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+        " @e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}\n" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
 }
 
 // 16 consecutive accumulator columns of this thread's TMEM lane.
@@ -164,6 +210,11 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// The same at a barrier of another block of the cluster.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // Bounded wait that also leaves when another role has given up.
@@ -187,7 +238,8 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32
 // in staging rows of kPitch bytes.  Rows of 2-byte elements may start at any
 // even address; a staging row then holds the row's aligned 4-byte words, i.e.
 // its elements shifted up by one place where the row starts odd.
-constexpr int kPitch = 144;  // 16-byte accesses of 8 rows fall into different banks
+template <typename E, int CH>
+constexpr int kPitch = CH * (int)sizeof(E) + 16;  // 16-byte accesses of 8 rows fall into different banks
 
 template <typename E>
 __device__ __forceinline__ int odd_row(const E* row) {
@@ -197,7 +249,7 @@ __device__ __forceinline__ int odd_row(const E* row) {
 // Staging rows -> global rows, coalesced.  g: the chunk's first element.
 template <typename E, int CH>
 __device__ __forceinline__ void chunk_store(char* stg, int lane, E* g, int64_t pitch, int rows, int cols, bool wide) {
-  constexpr int W = CH * (int)sizeof(E) / 4;  // words of a row
+  constexpr int W = CH * (int)sizeof(E) / 4, RS = 32 / W, P = kPitch<E, CH>;  // words of a row, rows at a time
   __syncwarp();
   if (wide) {
     constexpr int U = W / 4, PER = 16 / sizeof(E);
@@ -205,20 +257,29 @@ __device__ __forceinline__ void chunk_store(char* stg, int lane, E* g, int64_t p
 #pragma unroll
     for (int r = lane / U; r < 32; r += 32 / U)
       if (r < rows && u * PER < cols)
-        *reinterpret_cast<uint4*>(g + r * pitch + u * PER) = *reinterpret_cast<uint4*>(stg + r * kPitch + u * 16);
-  } else if (W == 32 && rows == 32 && cols >= CH) {  // a whole chunk: no bounds
-    const char* s = stg + lane * 4;
-    char* p = reinterpret_cast<char*>(g) + lane * 4;
-#pragma unroll 16
-    for (int r = 0; r < 32; ++r) {
-      const uint32_t x = *reinterpret_cast<const uint32_t*>(s + r * kPitch);
-      const int odd = odd_row(reinterpret_cast<E*>(p));
-      if (sizeof(E) == 4 || lane >= odd) *reinterpret_cast<uint32_t*>(p - 2 * odd) = x;
-      p += pitch * sizeof(E);
+        *reinterpret_cast<uint4*>(g + r * pitch + u * PER) = *reinterpret_cast<uint4*>(stg + r * P + u * 16);
+  } else if (rows == 32 && cols >= CH) {  // a whole chunk: no bounds
+    // Two rows (of each lane's share) at a time: their addresses' parities, which alternate at most, stay the same
+    // from pair to pair.
+    const int w = lane % W;
+    const char* s = stg + lane / W * P + w * 4;
+    char* pa = reinterpret_cast<char*>(g + lane / W * pitch) + w * 4;
+    char* pb = pa + RS * pitch * sizeof(E);
+    const int64_t step = 2 * RS * pitch * sizeof(E);
+    const int oa = odd_row(reinterpret_cast<E*>(pa)), ob = odd_row(reinterpret_cast<E*>(pb));
+    const bool wa = sizeof(E) == 4 || w >= oa, wb = sizeof(E) == 4 || w >= ob;
+    pa -= 2 * oa, pb -= 2 * ob;
+#pragma unroll 8
+    for (int r = 0; r < 32; r += 2 * RS) {
+      const uint32_t xa = *reinterpret_cast<const uint32_t*>(s + r * P);
+      const uint32_t xb = *reinterpret_cast<const uint32_t*>(s + (r + RS) * P);
+      if (wa) *reinterpret_cast<uint32_t*>(pa) = xa;
+      if (wb) *reinterpret_cast<uint32_t*>(pb) = xb;
+      pa += step, pb += step;
     }
     if constexpr (sizeof(E) == 2) {
       E* row = g + lane * pitch;
-      const E* t = reinterpret_cast<const E*>(stg + lane * kPitch);
+      const E* t = reinterpret_cast<const E*>(stg + lane * P);
       if (odd_row(row)) row[0] = t[1], row[CH - 1] = t[CH];
     }
   } else {
@@ -227,17 +288,17 @@ __device__ __forceinline__ void chunk_store(char* stg, int lane, E* g, int64_t p
     for (int r = lane / W; r < 32; r += 32 / W) {
       E* row = g + r * pitch;
       if constexpr (sizeof(E) == 4) {
-        if (r < rows && w < cols) row[w] = *reinterpret_cast<E*>(stg + r * kPitch + w * 4);
+        if (r < rows && w < cols) row[w] = *reinterpret_cast<E*>(stg + r * P + w * 4);
       } else {
         const int odd = odd_row(row);
         if (r < rows && w >= odd && 2 * w + 1 - odd < cols)
-          *reinterpret_cast<uint32_t*>(row + 2 * w - odd) = *reinterpret_cast<uint32_t*>(stg + r * kPitch + w * 4);
+          *reinterpret_cast<uint32_t*>(row + 2 * w - odd) = *reinterpret_cast<uint32_t*>(stg + r * P + w * 4);
       }
     }
     if constexpr (sizeof(E) == 2) {  // the elements that share a word with a neighbour: one lane per row
       E* row = g + lane * pitch;
       const int odd = odd_row(row), n = cols < CH ? cols : CH;
-      const E* s = reinterpret_cast<const E*>(stg + lane * kPitch);
+      const E* s = reinterpret_cast<const E*>(stg + lane * P);
       if (lane < rows && n > 0) {
         if (odd) row[0] = s[1];
         if ((n + odd) & 1) row[n - 1] = s[n - 1 + odd];
@@ -251,7 +312,7 @@ __device__ __forceinline__ void chunk_store(char* stg, int lane, E* g, int64_t p
 // word is returned and put in place by chunk_land.
 template <typename E, int CH>
 __device__ __forceinline__ E chunk_fetch(char* stg, int lane, const E* g, int64_t pitch, int rows, int cols, bool wide) {
-  constexpr int W = CH * (int)sizeof(E) / 4;
+  constexpr int W = CH * (int)sizeof(E) / 4, RS = 32 / W, P = kPitch<E, CH>;
   E tail{};
   if (wide) {
     constexpr int U = W / 4, PER = 16 / sizeof(E);
@@ -259,17 +320,20 @@ __device__ __forceinline__ E chunk_fetch(char* stg, int lane, const E* g, int64_
 #pragma unroll
     for (int r = lane / U; r < 32; r += 32 / U)
       if (r < rows && u * PER < cols)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(stg + r * kPitch + u * 16)),
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(stg + r * P + u * 16)),
                      "l"(g + r * pitch + u * PER)
                      : "memory");
-  } else if (W == 32 && rows == 32 && cols >= CH) {
-    const uint32_t s = smem_u32(stg) + lane * 4;
-    const char* p = reinterpret_cast<const char*>(g) + lane * 4;
-#pragma unroll 16
-    for (int r = 0; r < 32; ++r) {
-      const int odd = odd_row(reinterpret_cast<const E*>(p));
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s + r * kPitch), "l"(p - 2 * odd) : "memory");
-      p += pitch * sizeof(E);
+  } else if (rows == 32 && cols >= CH) {
+    const uint32_t s = smem_u32(stg) + lane / W * P + lane % W * 4;
+    const char* pa = reinterpret_cast<const char*>(g + lane / W * pitch) + lane % W * 4;
+    const char* pb = pa + RS * pitch * sizeof(E);
+    const int64_t step = 2 * RS * pitch * sizeof(E);
+    pa -= 2 * odd_row(reinterpret_cast<const E*>(pa)), pb -= 2 * odd_row(reinterpret_cast<const E*>(pb));
+#pragma unroll 8
+    for (int r = 0; r < 32; r += 2 * RS) {
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s + r * P), "l"(pa) : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s + (r + RS) * P), "l"(pb) : "memory");
+      pa += step, pb += step;
     }
     if constexpr (sizeof(E) == 2) {
       const E* row = g + lane * pitch;
@@ -283,7 +347,7 @@ __device__ __forceinline__ E chunk_fetch(char* stg, int lane, const E* g, int64_
       const int odd = odd_row(row);
       const bool on = r < rows && (sizeof(E) == 4 ? w < cols : 2 * w + 1 - odd < cols);
       if (on)  // an odd row's first word begins with the element before it, which exists
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(stg + r * kPitch + w * 4)),
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(stg + r * P + w * 4)),
                      "l"(reinterpret_cast<const char*>(row) + w * 4 - 2 * odd)
                      : "memory");
     }
@@ -301,25 +365,32 @@ template <typename E, int CH>
 __device__ __forceinline__ void chunk_land(char* stg, int lane, E tail, const E* row, int rows, int cols, bool wide) {
   if constexpr (sizeof(E) == 2) {
     const int odd = odd_row(row), n = cols < CH ? cols : CH;
-    if (!wide && lane < rows && n > 0 && ((n + odd) & 1)) reinterpret_cast<E*>(stg + lane * kPitch)[n - 1 + odd] = tail;
+    if (!wide && lane < rows && n > 0 && ((n + odd) & 1)) reinterpret_cast<E*>(stg + lane * kPitch<E, CH>)[n - 1 + odd] = tail;
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncwarp();
 }
 
-template <typename T, int MODE, int NT>
+template <typename T, int MODE, int NT, int CG = 1>
 struct Config {
   static constexpr bool kFloat = sizeof(T) == 4;
   static constexpr int BK = kBK<T>, NC = kFloat ? 3 : 1;
-  static constexpr int kA = BM * BK * 2, kB = NT * BK * 2;  // one component
+  static constexpr int kA = BM * BK * 2, kB = NT / CG * BK * 2;  // one component, this block's part
   static constexpr int kStage = NC * (kA + kB);
   static constexpr bool kDual = MODE == kAct || MODE == kDact;
-  static constexpr int kCols = (kDual ? NT / 2 : NT) / 2;   // columns (of each projection) of an epilogue warp
+  // Epilogue warps: 16 with the activation, else 8.  In the bfloat16 forward pass two sets of 8 take the tiles in
+  // turn (a tile's way from TMEM to memory takes longer than its products); else all share a tile's columns.
+  static constexpr int EW = kDual && NT > 64 ? 16 : 8;
+  static constexpr int kSets = MODE == kAct && !kFloat && EW == 16 ? 2 : 1;
+  static constexpr int kThreads = (4 + EW) * 32;
+  static constexpr int kCols = (kDual ? NT / 2 : NT) / (EW / kSets / 4);  // columns (of each projection) of a warp
   static constexpr bool kOutFloat = kFloat || MODE == kDw;
   static constexpr int CH = kCols < (kOutFloat ? 32 : 64) ? kCols : (kOutFloat ? 32 : 64);
-  static constexpr int kStoreBytes = MODE == kDact ? 4096 : 0;            // TMA store of dg, du
-  static constexpr int kPad = 32 * kPitch;                                // staging of out or dh
-  static constexpr int kEpi = kEpiWarps * (kStoreBytes + kPad);
+  using E = typename std::conditional<kOutFloat, float, bf16>::type;
+  static constexpr int kStoreBytes = MODE == kDact ? 32 * kCols * 2 * (kFloat ? 2 : 1) : 0;  // TMA store of dg, du
+  static constexpr int kStagePitch = kPitch<E, CH>;
+  static constexpr int kPad = 32 * kStagePitch;                            // staging of out or dh
+  static constexpr int kEpi = EW * (kStoreBytes + kPad);
   static constexpr int kFit = (kSmemTotal - 2048 - kEpi) / kStage;
   static constexpr int ST = kFit > 8 ? 8 : kFit;
   static constexpr int kSeg = kFloat ? 1 : 1 << 30;         // blocks of K per accumulator
@@ -332,13 +403,16 @@ struct Barriers {
   int abort_flag;
 };
 
-template <typename T, int MODE, int NT, int ACT>
-__global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Maps maps, const Params p) {
-  using F = Config<T, MODE, NT>;
+template <typename T, int MODE, int NT, int ACT, int CG>
+__global__ void __launch_bounds__(Config<T, MODE, NT, CG>::kThreads, 1)
+    kernel(const __grid_constant__ Maps maps, const Params p) {
+  using F = Config<T, MODE, NT, CG>;
   constexpr int ST = F::ST, BK = F::BK, NC = F::NC, kA = F::kA, kB = F::kB, CH = F::CH;
   constexpr bool kAmn = MODE == kDw, kBmn = MODE == kDx || MODE == kDw, kDual = F::kDual, kFloat = F::kFloat;
   constexpr uint32_t kIdesc = 1u << 4 | 1u << 7 | 1u << 10 | (kAmn ? 1u << 15 : 0u) | (kBmn ? 1u << 16 : 0u) |
-                              (uint32_t)(NT / 8) << 17 | (uint32_t)(BM / 16) << 24;
+                              (uint32_t)(NT / 8) << 17 | (uint32_t)(CG * BM / 16) << 24;
+  const uint32_t rank = CG == 1 ? 0 : cluster_rank();
+  const int64_t first = blockIdx.x / CG, step = gridDim.x / CG;  // tiles of this block or pair
   extern __shared__ char raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   char* epi_mem = smem + ST * F::kStage;
@@ -348,18 +422,26 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) mbar_init(&bar.full[i], 1), mbar_init(&bar.empty[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&bar.acc_full[i], 1), mbar_init(&bar.acc_empty[i], kEpiWarps);
+    for (int i = 0; i < 2; ++i) mbar_init(&bar.acc_full[i], 1), mbar_init(&bar.acc_empty[i], CG * F::EW / F::kSets);
     mbar_init(&bar.done, 1);
     bar.abort_flag = 0;
   }
   if (warp == 2) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar.tmem)),
-                 "n"(2 * NT)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (CG == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar.tmem)),
+                   "n"(2 * NT)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar.tmem)),
+                   "n"(2 * NT)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
   }
   fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_sync();  // both blocks' barriers are initialised
   fence_after();
   const uint32_t tmem = bar.tmem;
 
@@ -370,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
       split = (int)(t / per);
       t %= per;
     }
-    m0 = t / p.ntiles * BM;
+    m0 = t / p.ntiles * (CG * BM);
     n0 = (int)(t % p.ntiles) * (kDual ? NT / 2 : NT);
     kb0 = (int)((int64_t)p.kblocks * split / p.splits);
     kb1 = (int)((int64_t)p.kblocks * (split + 1) / p.splits);
@@ -381,43 +463,49 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
     int n0, kb0, kb1, split;
     uint32_t n = 0;  // stages issued
     bool ok = true;
-    for (int64_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x) {
+    for (int64_t t = first; ok && t < p.tiles; t += step) {
       tile_of(t, m0, n0, kb0, kb1, split);
       for (int kb = kb0; kb < kb1; ++kb, ++n) {
         const int s = n % ST;
         if (n >= ST && !(ok = wait(&bar.empty[s], (n / ST - 1) & 1, p.polls, abort_flag))) break;
-        uint64_t* full = &bar.full[s];
-        mbar_expect_tx(full, F::kStage);
+        // both blocks' copies count towards the first block's barrier
+        const uint32_t full = CG == 1 ? smem_u32(&bar.full[s]) : peer_addr(&bar.full[s], 0);
+        if (rank == 0) mbar_expect_tx(&bar.full[s], CG * F::kStage);
+        const int m = (int)m0 + (int)rank * BM;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           char *a = smem + s * F::kStage + c * kA, *b = smem + s * F::kStage + NC * kA + c * kB;
           if (kAmn) {
-            tma_load_3d(a, &maps.a, (int)m0, kb * BK, c, full);
-            tma_load_3d(a + BK * 128, &maps.a, (int)m0 + 64, kb * BK, c, full);
+            tma_load_3d<CG>(a, &maps.a, m, kb * BK, c, full);
+            tma_load_3d<CG>(a + BK * 128, &maps.a, m + 64, kb * BK, c, full);
           } else {
-            tma_load_3d(a, &maps.a, kb * BK, (int)m0, c, full);
+            tma_load_3d<CG>(a, &maps.a, kb * BK, m, c, full);
           }
           if (kDual) {
-            tma_load_3d(b, &maps.b0, kb * BK, n0, c, full);
-            tma_load_3d(b + kB / 2, &maps.b1, kb * BK, n0, c, full);
+            if (CG == 1) {
+              tma_load_3d<CG>(b, &maps.b0, kb * BK, n0, c, full);
+              tma_load_3d<CG>(b + kB / 2, &maps.b1, kb * BK, n0, c, full);
+            } else {  // half of B each: one projection's rows
+              tma_load_3d<CG>(b, rank == 0 ? &maps.b0 : &maps.b1, kb * BK, n0, c, full);
+            }
           } else {
             const bool up = MODE == kDx && kb >= p.fp / BK;
-            const int k = (up ? kb - p.fp / BK : kb) * BK;
-            for (int j = 0; j < NT / 64; ++j)
-              tma_load_3d(b + j * BK * 128, up ? &maps.b1 : &maps.b0, n0 + j * 64, k, c, full);
+            const int k = (up ? kb - p.fp / BK : kb) * BK, n1 = n0 + (int)rank * (NT / CG);
+            for (int j = 0; j < NT / CG / 64; ++j)
+              tma_load_3d<CG>(b + j * BK * 128, up ? &maps.b1 : &maps.b0, n1 + j * 64, k, c, full);
           }
         }
       }
     }
     // Nothing may land after the block has left: the last copies of every stage.
-    for (uint32_t i = n > ST ? n - ST : 0; i < n; ++i)
+    for (uint32_t i = n > ST ? n - ST : 0; rank == 0 && i < n; ++i)
       mbar_wait_bounded(&bar.full[i % ST], (i / ST) & 1, kTransferDrainPolls);
-  } else if (warp == 1) {  // products
+  } else if (warp == 1 && rank == 0) {  // products
     int64_t m0;
     int n0, kb0, kb1, split;
     uint32_t n = 0, accs = 0;
     bool ok = true;
-    for (int64_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x) {
+    for (int64_t t = first; ok && t < p.tiles; t += step) {
       tile_of(t, m0, n0, kb0, kb1, split);
       for (int seg = kb0; ok && seg < kb1; seg = kb1 - seg > F::kSeg ? seg + F::kSeg : kb1, ++accs) {
         const int end = kb1 - seg > F::kSeg ? seg + F::kSeg : kb1;
@@ -436,35 +524,44 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
             const uint64_t da = smem_desc<BK>(a + ca * kA, kAmn), db = smem_desc<BK>(b + cb * kB, kBmn);
 #pragma unroll
             for (int k = 0; k < BK / 16; ++k)  // 16 K elements: 32 bytes of a K-major row, 16 rows of an MN-major box
-              mma_f16(d, da + k * ((kAmn ? 2048 : 32) >> 4), db + k * ((kBmn ? 2048 : 32) >> 4), kIdesc,
-                      kb > seg || term > (kFloat ? 0 : 5) || k > 0);
+              mma_f16<CG>(d, da + k * ((kAmn ? 2048 : 32) >> 4), db + k * ((kBmn ? 2048 : 32) >> 4), kIdesc,
+                          kb > seg || term > (kFloat ? 0 : 5) || k > 0);
           }
-          mma_commit(&bar.empty[s]);
+          mma_commit<CG>(&bar.empty[s]);
         }
-        if (ok) mma_commit(&bar.acc_full[buf]);
+        if (ok) mma_commit<CG>(&bar.acc_full[buf]);
       }
     }
     if (!ok) {  // TMEM may be freed only after the products in flight
-      mma_commit(&bar.done);
+      mma_commit<CG>(&bar.done);
       mbar_wait_bounded(&bar.done, 0, kTransferDrainPolls);
     }
-  } else if (warp >= 4) {  // epilogue: lanes 32 (warp % 4) .. + 31, half of the columns each
+  } else if (warp >= 4) {  // epilogue: lanes 32 (warp % 4) .. + 31, a group of columns each
     constexpr int kCols = F::kCols;
-    using E = typename std::conditional<F::kOutFloat, float, bf16>::type;
+    using E = typename F::E;
     constexpr int RC = kFloat ? kCols : 16;  // accumulator columns held in registers
-    const int quad = warp & 3, half = (warp - 4) >> 2;
+    constexpr int kSet = F::EW / F::kSets;  // warps of a set
+    const int quad = warp & 3, group = (warp - 4) % kSet >> 2, set = (warp - 4) / kSet;
     char* tst = epi_mem + (warp - 4) * F::kStoreBytes;
-    char* stg = epi_mem + kEpiWarps * F::kStoreBytes + (warp - 4) * F::kPad;
+    char* stg = epi_mem + F::EW * F::kStoreBytes + (warp - 4) * F::kPad;
     int64_t m0;
     int n0, kb0, kb1, split;
     uint32_t accs = 0;
     bool ok = true;
     const float nan = __int_as_float(0x7fffffff);
-    for (int64_t t = blockIdx.x; t < p.tiles; t += gridDim.x) {
+    auto release = [&](uint64_t* w) {
+      if (CG == 1) mbar_arrive(w);
+      else mbar_arrive_remote(peer_addr(w, 0));
+    };
+    for (int64_t t = first; t < p.tiles; t += step) {
+      if (F::kSets == 2 && (int)(accs & 1) != set) {  // one accumulator per tile: the other set's
+        ++accs;
+        continue;
+      }
       tile_of(t, m0, n0, kb0, kb1, split);
-      const int64_t row0 = m0 + quad * 32;
+      const int64_t row0 = m0 + rank * BM + quad * 32;
       const int rows = (int)(p.M - row0 < 32 ? p.M - row0 : 32);
-      const int colw = n0 + half * kCols;
+      const int colw = n0 + group * kCols;
       T tail{};
       const T* dh = nullptr;
       if constexpr (MODE == kDact) {  // on its way while the products run
@@ -485,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
         if (ok) ok = wait(&bar.acc_full[buf], (accs / 2) & 1, p.polls, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         fence_after();
-        acc = tmem + ((uint32_t)(quad * 32) << 16) + buf * NT + half * kCols;
+        acc = tmem + ((uint32_t)(quad * 32) << 16) + buf * NT + group * kCols;
         if constexpr (kFloat) {
           if (ok) {
 #pragma unroll
@@ -509,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
           }
           fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bar.acc_empty[buf]);
+          if (lane == 0) release(&bar.acc_empty[buf]);
         }
       }
       if constexpr (MODE == kDact) chunk_land<T, CH>(stg, lane, tail, dh + (int64_t)lane * p.N, rows, p.N - colw, p.wide);
@@ -551,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
             }
           }
           if constexpr (MODE != kDact) {
-            char* s = stg + lane * kPitch + c * sizeof(E);
+            char* s = stg + lane * F::kStagePitch + c * sizeof(E);
             if constexpr (F::kOutFloat) {
 #pragma unroll
               for (int i = 0; i < 16; i += 4)
@@ -570,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
             }
           } else {  // dg, du in place of g, u
             float y[16];
-            const char* s = stg + lane * kPitch + c * sizeof(T);
+            const char* s = stg + lane * F::kStagePitch + c * sizeof(T);
             if constexpr (kFloat) {
 #pragma unroll
               for (int i = 0; i < 16; i += 4) {
@@ -609,13 +706,13 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
           }
         }
         if constexpr (!F::kOutFloat && MODE != kDact)  // an odd row's last element opens one more word
-          *reinterpret_cast<uint32_t*>(stg + lane * kPitch + CH * 2) = carry >> 16;
+          *reinterpret_cast<uint32_t*>(stg + lane * F::kStagePitch + CH * 2) = carry >> 16;
         if constexpr (MODE != kDact) chunk_store<E, CH>(stg, lane, out, p.N, rows, p.N - colw - c0, p.wide);
       }
       if constexpr (!kFloat) {
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.acc_empty[(accs - 1) & 1]);
+        if (lane == 0) release(&bar.acc_empty[(accs - 1) & 1]);
       }
       if constexpr (MODE == kDact) {
         // Through the swizzled staging box to dg | du: 16-byte units of a row of
@@ -668,9 +765,13 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
   __syncwarp();
   fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_sync();  // neither block leaves, or frees TMEM, before the other is done with it
   fence_after();
   if (warp == 2) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(2 * NT) : "memory");
+    if constexpr (CG == 1)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(2 * NT) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(2 * NT) : "memory");
   }
 }
 
@@ -712,15 +813,26 @@ inline int make_map(CUtensorMap* m, const void* base, int64_t inner, int64_t out
   return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
 }
 
-template <typename T, int MODE, int NT, int ACT>
+template <typename T, int MODE, int NT, int ACT, int CG = 1>
 int launch(const Maps& maps, Params p, cudaStream_t st) {
   p.tiles = (int64_t)p.mtiles * p.ntiles * p.splits;
   p.polls = transfer_poll_limit().load();
-  const int rc = allow_smem<kernel<T, MODE, NT, ACT>>(kSmemTotal);
+  const int rc = allow_smem<kernel<T, MODE, NT, ACT, CG>>(kSmemTotal);
   if (rc) return rc;
-  const int64_t sms = sm_count();
-  kernel<T, MODE, NT, ACT><<<(unsigned)(p.tiles < sms ? p.tiles : sms), kThreads, kSmemTotal, st>>>(maps, p);
-  return (int)cudaPeekAtLastError();
+  const int64_t slots = sm_count() / CG;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3((unsigned)(CG * (p.tiles < slots ? p.tiles : slots)));
+  c.blockDim = dim3(Config<T, MODE, NT, CG>::kThreads);
+  c.dynamicSmemBytes = kSmemTotal;
+  c.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  c.attrs = attr;
+  c.numAttrs = CG > 1 ? 1 : 0;
+  return (int)cudaLaunchKernelEx(&c, kernel<T, MODE, NT, ACT, CG>, maps, p);
 }
 
 }  // namespace gemm

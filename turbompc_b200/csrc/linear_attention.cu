@@ -12,10 +12,11 @@
 // Bound by the float units: 2 operations per state element and token.  A thread
 // keeps 8 x 4 elements of S; a token costs it 5 shared-memory loads and 64
 // multiply-adds.  The decay is taken out of the inner loop: within 16 tokens
-// the state is held as d^-u S, with a and b scaled by d^u and d^-u as they are
-// staged; where d^-16 could overflow (d < 2^-6) the state is rescaled at every
+// the state is held as d^-u S, c is scaled by d^-u and the finished read-out by
+// d^u; where d^-16 could overflow (d < 2^-6) the state is rescaled at every
 // token instead.  The read-outs of four tokens are summed over the lanes that
-// share a column group together, each lane keeping its share.
+// share a column group together, each lane keeping its share.  The next 16
+// tokens are copied to shared memory meanwhile (cp.async).
 #include <type_traits>
 
 #include "seq_attention.cuh"
@@ -52,10 +53,17 @@ struct Shape {
   static constexpr int RG = D / 8;                      // lanes that share a column group
 };
 
+// A tile's rows of a, b, c (and x), two of each, and the factors of the tokens.
+template <int D, bool LOG>
+struct Smem {
+  float rows[2][LOG ? 4 : 3][kTile][D];
+  float fc[kTile], fo[kTile], red[16];
+};
+
 template <int D, bool REV, bool LOG, bool OUT>
-__global__ void __launch_bounds__(Shape<D>::BLOCK) pass_kernel(const Args p) {
+__global__ void __launch_bounds__(Shape<D>::BLOCK, D == 128 ? 1 : LOG ? 3 : 4) pass_kernel(const Args p) {
   using Z = Shape<D>;
-  __shared__ __align__(16) float smem[Z::UNITS][LOG ? 4 : 3][kTile][D];
+  extern __shared__ __align__(16) char raw[];
   const int sub = threadIdx.x / Z::NT, tid = threadIdx.x % Z::NT, lane = threadIdx.x & 31;
   const int64_t unit = (int64_t)blockIdx.x * Z::UNITS + sub;
   if (unit >= p.units) return;  // whole warps; a block of several states has no block-wide barrier
@@ -63,7 +71,7 @@ __global__ void __launch_bounds__(Shape<D>::BLOCK) pass_kernel(const Args p) {
     if constexpr (Z::UNITS > 1) __syncwarp();
     else __syncthreads();
   };
-  float(*sa)[D] = smem[sub][0], (*sb)[D] = smem[sub][1], (*sc)[D] = smem[sub][2], (*sx)[D] = smem[sub][LOG ? 3 : 0];
+  Smem<D, LOG>& sm = reinterpret_cast<Smem<D, LOG>*>(raw)[sub];
   const int heads = p.H / p.rep;
   const int hu = (int)(unit % heads), seg = (int)(unit / heads % p.nseg);
   const int b = (int)(unit / heads / p.nseg);
@@ -95,81 +103,81 @@ __global__ void __launch_bounds__(Shape<D>::BLOCK) pass_kernel(const Args p) {
       }
     int pending = REV ? 0 : 1;  // powers of d due on S before the next token; afterwards the tokens since a rescaling
 
-    // a tile's rows in registers, one tile ahead
-    constexpr int NV = kTile * D / 4 / Z::NT, NTEN = LOG ? 4 : 3;
-    float4 next[NTEN][NV];
+    sync();  // the last head's factors and tiles have been read
+    if (tid < kTile) {
+      const float pw = rn == 1 ? 1.f : exp2f(g2 * (float)tid);
+      sm.fc[tid] = p.b_scale / pw;
+      sm.fo[tid] = p.a_scale * pw;
+    }
     auto fetch = [&](int u0) {
 #pragma unroll
-      for (int w = 0; w < NTEN; ++w) {
+      for (int w = 0; w < (LOG ? 4 : 3); ++w) {
         const TmpcSeqView& v = w == 0 ? p.a : w == 1 ? p.b : w == 2 ? p.c : p.x;
         const int head = w == 0 ? (p.a_key ? g : h) : w == 1 ? (p.b_key ? g : h) : w == 2 ? (p.c_key ? g : h) : h;
         const int d = w < 2 ? p.e : p.f;
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-          const int idx = tid + n * Z::NT, u = u0 + idx / (D / 4), i = idx % (D / 4) * 4;
-          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (u < len && i < d) {
-            const float* src = row_ptr<float>(v, b, begin + (REV ? len - 1 - u : u), head) + i;
-            if (p.vec) {
-              x = *reinterpret_cast<const float4*>(src);
-            } else {
-              x.x = src[0];
-              if (i + 1 < d) x.y = src[1];
-              if (i + 2 < d) x.z = src[2];
-              if (i + 3 < d) x.w = src[3];
-            }
-          }
-          next[w][n] = x;
+        float* to = &sm.rows[(u0 / kTile) & 1][w][0][0];
+        const float* base = row_ptr<float>(v, b, begin, head);
+        const int W = p.vec ? 4 : 1;  // floats per copy
+        for (int idx = tid * W; idx < kTile * D; idx += Z::NT * W) {
+          const int u = u0 + idx / D, i = idx % D;
+          const bool on = u < len && i < d;
+          const float* src = on ? base + (REV ? len - 1 - u : u) * v.token + i : base;
+          const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to + idx);
+          if (p.vec)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+          else
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
         }
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     };
     if (len > 0) fetch(0);
     for (int u0 = 0; u0 < len; u0 += kTile) {
-      sync();  // the last tile has been read
-#pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        const int idx = tid + n * Z::NT, u = idx / (D / 4), i = idx % (D / 4) * 4;
-        const float pw = rn == 1 ? 1.f : exp2f(g2 * (float)u);
-        const float fa = pw * p.a_scale, fb = p.b_scale / pw;
-        const float4 x = next[0][n], y = next[1][n];
-        *reinterpret_cast<float4*>(&sa[u][i]) = make_float4(x.x * fa, x.y * fa, x.z * fa, x.w * fa);
-        *reinterpret_cast<float4*>(&sb[u][i]) = make_float4(y.x * fb, y.y * fb, y.z * fb, y.w * fb);
-        *reinterpret_cast<float4*>(&sc[u][i]) = next[2][n];
-        if constexpr (LOG) *reinterpret_cast<float4*>(&sx[u][i]) = next[3][n];
-      }
-      sync();
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      sync();  // this tile has landed, the one before has been read
       if (u0 + kTile < len) fetch(u0 + kTile);
+      const int buf = (u0 / kTile) & 1;
+      const float(*sa)[D] = sm.rows[buf][0], (*sb)[D] = sm.rows[buf][1], (*sc)[D] = sm.rows[buf][2];
+      const float(*sx)[D] = sm.rows[buf][LOG ? 3 : 0];
       const int m = min(kTile, len - u0);
+      // S <- d^pending S (and M <- d^pending (M + S)): what is due before a token is added
+      auto rescale = [&] {
+        const float w = exp2f(g2 * (float)pending);
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if constexpr (LOG) M[r][c] = (M[r][c] + S[r][c]) * w;
+            S[r][c] *= w;
+          }
+        pending = 0;
+      };
+      if (rn != 1) rescale();
 #pragma unroll 1
       for (int v0 = 0; v0 < m; v0 += 4) {
         float o[4][4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int u = v0 + q;  // rows past m are zero: they leave the state alone
-          if (u < m && (rn == 1 || u == 0)) {
-            const float w = exp2f(g2 * (float)pending);
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                if constexpr (LOG) M[r][c] = (M[r][c] + S[r][c]) * w;
-                S[r][c] *= w;
-              }
-            pending = 0;
-          } else if (LOG && u < m) {
+          if (rn == 1) {
+            if (u < m) {
+              rescale();
+              pending = 1;
+            }
+          } else if (LOG && u > 0 && u < m) {
 #pragma unroll
             for (int r = 0; r < 8; ++r)
 #pragma unroll
               for (int c = 0; c < 4; ++c) M[LOG ? r : 0][c] += S[r][c];
           }
-          if (u < m) ++pending;
           float av[8], bv[8];
           *reinterpret_cast<float4*>(av) = *reinterpret_cast<const float4*>(&sa[u][rg * 4]);
           *reinterpret_cast<float4*>(av + 4) = *reinterpret_cast<const float4*>(&sa[u][D / 2 + rg * 4]);
           *reinterpret_cast<float4*>(bv) = *reinterpret_cast<const float4*>(&sb[u][rg * 4]);
           *reinterpret_cast<float4*>(bv + 4) = *reinterpret_cast<const float4*>(&sb[u][D / 2 + rg * 4]);
           const float4 cv = *reinterpret_cast<const float4*>(&sc[u][j0]);
-          const float cc[4] = {cv.x, cv.y, cv.z, cv.w};
+          const float fc = sm.fc[u];
+          const float cc[4] = {cv.x * fc, cv.y * fc, cv.z * fc, cv.w * fc};
           float xm[4] = {};
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -184,7 +192,7 @@ __global__ void __launch_bounds__(Shape<D>::BLOCK) pass_kernel(const Args p) {
           }
           if constexpr (LOG && OUT) {
             const float4 xv = *reinterpret_cast<const float4*>(&sx[u][j0]);
-            dlog += xm[0] * xv.x + xm[1] * xv.y + xm[2] * xv.z + xm[3] * xv.w;
+            dlog = fmaf(sm.fo[u], xm[0] * xv.x + xm[1] * xv.y + xm[2] * xv.z + xm[3] * xv.w, dlog);
           }
         }
         if constexpr (OUT) {
@@ -205,6 +213,9 @@ __global__ void __launch_bounds__(Shape<D>::BLOCK) pass_kernel(const Args p) {
           }
           constexpr int KEEP = 16 / Z::RG;  // values of this lane: token first / 4, columns j0 + first % 4 ..
           const int u = u0 + v0 + first / 4, j = j0 + first % 4;
+          const float fo = sm.fo[v0 + first / 4];
+#pragma unroll
+          for (int i = 0; i < KEEP; ++i) x[i] *= fo;
           if (u < len && j < p.f) {
             float* dst = row_ptr<float>(p.o, b, begin + (REV ? len - 1 - u : u), REV ? g : h) + j;
             if (KEEP == 4 && p.vec) {
@@ -222,6 +233,7 @@ __global__ void __launch_bounds__(Shape<D>::BLOCK) pass_kernel(const Args p) {
           }
         }
       }
+      if (rn != 1) pending = m;
     }
     // the state after the last token (forward), or the adjoint before the first (backward)
     const float w = exp2f(g2 * (float)(REV ? pending : pending - 1));
@@ -246,10 +258,10 @@ __global__ void __launch_bounds__(Shape<D>::BLOCK) pass_kernel(const Args p) {
       dlog = warp_sum(dlog);
       if constexpr (Z::NW > 1) {
         sync();
-        if (lane == 0) sa[0][tid / 32] = dlog;
+        if (lane == 0) sm.red[tid / 32] = dlog;
         sync();
         dlog = 0.f;
-        for (int i = 0; i < Z::NW; ++i) dlog += sa[0][i];
+        for (int i = 0; i < Z::NW; ++i) dlog += sm.red[i];
       }
       if (tid == 0) p.dlog[bh * p.nseg + seg] = dlog;
     }
@@ -314,13 +326,17 @@ __global__ void __launch_bounds__(128) dlog_kernel(const float* part, float* out
 
 template <bool REV, bool LOG, bool OUT>
 int run(Args p, const TmpcLinAttnDims* d, cudaStream_t st) {
+  int rc = 0;
   by_size(d, [&](auto dd) {
     constexpr int D = decltype(dd)::value;
     using Z = Shape<D>;
+    constexpr int smem = Z::UNITS * (int)sizeof(Smem<D, LOG>);
     p.units = (int64_t)d->B * (p.H / p.rep) * p.nseg;
-    pass_kernel<D, REV, LOG, OUT><<<(unsigned)((p.units + Z::UNITS - 1) / Z::UNITS), Z::BLOCK, 0, st>>>(p);
+    rc = allow_smem<pass_kernel<D, REV, LOG, OUT>>(smem);
+    if (!rc)
+      pass_kernel<D, REV, LOG, OUT><<<(unsigned)((p.units + Z::UNITS - 1) / Z::UNITS), Z::BLOCK, smem, st>>>(p);
   });
-  return (int)cudaPeekAtLastError();
+  return rc ? rc : (int)cudaPeekAtLastError();
 }
 
 // One pass; a long sequence in segments: each one's own state first, then the
@@ -343,7 +359,7 @@ int pass(Args p, const TmpcLinAttnDims* d, float* seg, float* segm, const float*
 // States that fit the device at once, by the registers.
 inline int64_t resident(const TmpcLinAttnDims* d) {
   const int m = std::max(d->dk, d->dv);
-  return (int64_t)sm_count() * (m <= 32 ? 8 : m <= 64 ? 2 : 1);
+  return (int64_t)sm_count() * (m <= 32 ? 16 : m <= 64 ? 4 : 1);
 }
 
 inline Args base_args(const LinAttnArgs& a, const TmpcLinAttnDims* d, int64_t heads) {

@@ -5,12 +5,13 @@
 //             (dt is the gradient of x and of r)
 //
 // Bound by HBM: forward reads x, r and writes y, t; backward reads dy, ds, t
-// and writes dt.  A row belongs to TPR threads which keep it in registers
-// between the sum of squares and the scaling, so every element is read once.
+// and writes dt.  A row belongs to TPR threads (8, a warp, or a block of 128 or
+// 512) which keep it in registers between the sum of squares and the scaling, so
+// every element is read once; the rows' values stay packed until they are used.
 // dw: a fixed grid walks the rows with a stride, each thread summing its own
-// columns in registers; one partial row per block goes to the workspace and a
-// second kernel adds the blocks in order, so the result does not depend on
-// the order of execution.
+// columns in registers, the next row on its way meanwhile; one partial row per
+// block goes to the workspace and a second kernel adds the blocks in order, so
+// the result does not depend on the order of execution.
 #include <algorithm>
 
 #include "seq_common.cuh"
@@ -18,13 +19,58 @@
 namespace tmpc {
 namespace seq {
 
-constexpr int kNormThreads = 256;
+constexpr int kNormThreads = 256;  // of a block whose rows have a warp or less
 constexpr int kNormMaxD = 16384;
 
-// Sum over the TPR threads of a row (TPR = 32: a warp; else the whole block).
+// V elements in 32-bit registers (V == 1 in bfloat16: half of one).
+template <typename T, int V>
+struct Packed {
+  static constexpr int W = V * (int)sizeof(T) >= 4 ? V * (int)sizeof(T) / 4 : 1;
+  uint32_t w[W];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (W == 4) {
+      const uint4 x = *reinterpret_cast<const uint4*>(p);
+      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else if constexpr (W == 2) {
+      const uint2 x = *reinterpret_cast<const uint2*>(p);
+      w[0] = x.x, w[1] = x.y;
+    } else if constexpr (V * sizeof(T) == 4) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (W == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else if constexpr (W == 2) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else if constexpr (V * sizeof(T) == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
+    else *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
+  }
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+    else return __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+  }
+  __device__ __forceinline__ void set(const float (&v)[V]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) w[e] = __float_as_uint(v[e]);
+    } else if constexpr (V == 1) {
+      w[0] = __bfloat16_as_ushort(__float2bfloat16_rn(v[0]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(v[e], v[e + 1]);
+        w[e / 2] = *reinterpret_cast<const uint32_t*>(&x);
+      }
+    }
+  }
+};
+
+// Sum over the TPR threads of a row.
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* red) {
-  v = warp_sum(v);
+#pragma unroll
+  for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if constexpr (TPR > 32) {
     const int w = threadIdx.x >> 5;
     __syncthreads();
@@ -37,121 +83,141 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
   return v;
 }
 
+template <int TPR>
+struct Rows {
+  static constexpr int kBlock = TPR <= 32 ? kNormThreads : TPR;
+  static constexpr int kRows = kBlock / TPR;  // rows of a block at a time
+};
+
 template <typename T, int V, int NV, int TPR>
-__global__ void __launch_bounds__(TPR == 32 ? kNormThreads : TPR)
+__global__ void __launch_bounds__(Rows<TPR>::kBlock)
     norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ r, const T* __restrict__ w, T* __restrict__ y,
                     T* __restrict__ t, float* __restrict__ inv, int64_t rows, int d, int64_t xs, int64_t rs,
                     float eps) {
-  using P = Pack<T, V>;
+  using P = Packed<T, V>;
   __shared__ float red[32];
-  constexpr int RPB = TPR == 32 ? kNormThreads / 32 : 1;
-  const int lane = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
-  const int64_t row = (int64_t)blockIdx.x * RPB + (TPR == 32 ? (threadIdx.x >> 5) : 0);
-  if (row >= rows) return;  // whole rows leave together
-  const int nv = d / V;
-  float s[NV][V];
+  const int lane = threadIdx.x % TPR;
+  const int64_t row = (int64_t)blockIdx.x * Rows<TPR>::kRows + threadIdx.x / TPR;
+  const bool on = row < rows;  // the rows of a warp sum together, those past the end add nothing
+  const int nv = on ? d / V : 0;
   P px[NV], pr[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = lane + j * TPR;
     if (c < nv) {
-      px[j] = reinterpret_cast<const P*>(x + row * xs)[c];
-      if (r) pr[j] = reinterpret_cast<const P*>(r + row * rs)[c];
+      px[j].load(x + row * xs + c * V);
+      if (r) pr[j].load(r + row * rs + c * V);
     }
   }
+  float s[NV][V];
   float sq = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = lane + j * TPR;
-#pragma unroll
-    for (int e = 0; e < V; ++e) s[j][e] = 0.f;
     if (c < nv) {
-      P o;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        s[j][e] = to_f(px[j].v[e]) + (r ? to_f(pr[j].v[e]) : 0.f);
+        s[j][e] = px[j].get(e) + (r ? pr[j].get(e) : 0.f);
         sq = fmaf(s[j][e], s[j][e], sq);
-        o.v[e] = from_f<T>(s[j][e]);
       }
-      if (t) reinterpret_cast<P*>(t + row * d)[c] = o;
+      if (t) {
+        px[j].set(s[j]);
+        px[j].store(t + row * d + c * V);
+      }
     }
   }
   const float iv = rsqrtf(row_sum<TPR>(sq, red) / (float)d + eps);
-  if (inv && lane == 0) inv[row] = iv;
+  if (inv && on && lane == 0) inv[row] = iv;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = lane + j * TPR;
     if (c < nv) {
-      const P pw = reinterpret_cast<const P*>(w)[c];
-      P o;
+      P pw;
+      pw.load(w + c * V);
 #pragma unroll
-      for (int e = 0; e < V; ++e) o.v[e] = from_f<T>(s[j][e] * iv * to_f(pw.v[e]));
-      reinterpret_cast<P*>(y + row * d)[c] = o;
+      for (int e = 0; e < V; ++e) s[j][e] *= iv * pw.get(e);
+      pw.set(s[j]);
+      pw.store(y + row * d + c * V);
     }
   }
 }
 
 template <typename T, int V, int NV, int TPR>
-__global__ void __launch_bounds__(TPR == 32 ? kNormThreads : TPR)
+__global__ void __launch_bounds__(Rows<TPR>::kBlock)
     norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ ds, const T* __restrict__ t,
                     const T* __restrict__ w, const float* __restrict__ inv, T* __restrict__ dt,
                     float* __restrict__ dw_part, int64_t rows, int d) {
-  using P = Pack<T, V>;
+  using P = Packed<T, V>;
   __shared__ float red[32];
-  constexpr int RPB = TPR == 32 ? kNormThreads / 32 : 1;
-  const int lane = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
-  const int sub = TPR == 32 ? (threadIdx.x >> 5) : 0;
+  constexpr int RPB = Rows<TPR>::kRows;
+  const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   const int nv = d / V;
   const float invd = 1.f / (float)d;
   float acc[NV][V];
-  P pw[NV];
+  P pw[NV], nt[NV], nd[NV], ns[NV];  // the weights; the next row
+  float ni = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int c = lane + j * TPR;
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[j][e] = 0.f;
-    if (c < nv) pw[j] = reinterpret_cast<const P*>(w)[c];
+#pragma unroll
+    for (int e = 0; e < P::W; ++e) pw[j].w[e] = nt[j].w[e] = nd[j].w[e] = ns[j].w[e] = 0;
+    if (lane + j * TPR < nv) pw[j].load(w + (lane + j * TPR) * V);
   }
-  for (int64_t row = (int64_t)blockIdx.x * RPB + sub; row < rows; row += (int64_t)gridDim.x * RPB) {
-    P pt[NV], pd[NV], ps[NV];
+  auto fetch = [&](int64_t row) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = lane + j * TPR;
       if (c < nv) {
-        pt[j] = reinterpret_cast<const P*>(t + row * d)[c];
-        pd[j] = reinterpret_cast<const P*>(dy + row * d)[c];
-        if (ds) ps[j] = reinterpret_cast<const P*>(ds + row * d)[c];
+        nt[j].load(t + row * d + c * V);
+        nd[j].load(dy + row * d + c * V);
+        if (ds) ns[j].load(ds + row * d + c * V);
       }
     }
-    const float iv = inv[row];
+    ni = inv[row];
+  };
+  const int64_t stride = (int64_t)gridDim.x * RPB;
+  const int64_t base = (int64_t)blockIdx.x * RPB;
+  if (base + sub < rows) fetch(base + sub);
+  for (int64_t b = base; b < rows; b += stride) {  // whole blocks stay together: a warp's rows sum together
+    const int64_t row = b + sub;
+    P pt[NV], pd[NV], ps[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) pt[j] = nt[j], pd[j] = nd[j], ps[j] = ns[j];
+    const float iv = ni;
+    const bool on = row < rows;
+    if (row + stride < rows) fetch(row + stride);
     float dot = 0.f;
+    if (on) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (lane + j * TPR < nv) {
+      for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float a = to_f(pd[j].v[e]), b = to_f(pt[j].v[e]);
-          dot = fmaf(a * to_f(pw[j].v[e]), b, dot);
-          acc[j][e] = fmaf(a * iv, b, acc[j][e]);
+          const float a = pd[j].get(e), c = pt[j].get(e);
+          dot = fmaf(a * pw[j].get(e), c, dot);
+          acc[j][e] = fmaf(a * iv, c, acc[j][e]);
         }
-      }
+    }
     const float m = row_sum<TPR>(dot, red) * invd * iv * iv * iv;
+    if (on) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (lane + j * TPR < nv) {
-        P o;
+      for (int j = 0; j < NV; ++j)
+        if (lane + j * TPR < nv) {
+          float g[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          float g = iv * to_f(pd[j].v[e]) * to_f(pw[j].v[e]) - m * to_f(pt[j].v[e]);
-          if (ds) g += to_f(ps[j].v[e]);
-          o.v[e] = from_f<T>(g);
+          for (int e = 0; e < V; ++e) {
+            g[e] = iv * pd[j].get(e) * pw[j].get(e) - m * pt[j].get(e);
+            if (ds) g[e] += ps[j].get(e);
+          }
+          P o;
+          o.set(g);
+          o.store(dt + row * d + (lane + j * TPR) * V);
         }
-        reinterpret_cast<P*>(dt + row * d)[lane + j * TPR] = o;
-      }
+    }
   }
-  // The block's rows in order: TPR = 32 adds the warps one after another.
+  // The block's rows in order, one group of TPR threads after another.
   extern __shared__ float sdw[];
-  if constexpr (TPR == 32) {
+  if constexpr (TPR <= 32) {
     for (int s = 0; s < RPB; ++s) {
       if (sub == s) {
 #pragma unroll
@@ -166,7 +232,7 @@ __global__ void __launch_bounds__(TPR == 32 ? kNormThreads : TPR)
       }
       __syncthreads();
     }
-    for (int c = threadIdx.x; c < d; c += kNormThreads) dw_part[(int64_t)blockIdx.x * d + c] = sdw[c];
+    for (int c = threadIdx.x; c < d; c += Rows<TPR>::kBlock) dw_part[(int64_t)blockIdx.x * d + c] = sdw[c];
   } else {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -193,11 +259,14 @@ __global__ void __launch_bounds__(1024) norm_dw_kernel(const float* __restrict__
   if (threadIdx.x == 0 && co < d) dw[co] = from_f<T>(v);
 }
 
-// Blocks of the backward pass: eight warps each, four blocks per SM.
+// Threads per row: up to 16 elements each, 32 from 8193 columns on.
+inline int norm_tpr(int d) { return d <= 128 ? 8 : d <= 512 ? 32 : d <= 2048 ? 128 : 512; }
+
+// Blocks of the backward pass: about as many as are resident at once.
 inline int norm_bwd_blocks(int64_t rows, int d) {
-  const int rpb = d <= 1024 ? kNormThreads / 32 : 1;
+  const int tpr = norm_tpr(d), rpb = tpr <= 32 ? kNormThreads / tpr : 1;
   const int64_t need = (rows + rpb - 1) / rpb;
-  return (int)std::min<int64_t>(need, 4 * (int64_t)sm_count());
+  return (int)std::min<int64_t>(need, (tpr == 128 ? 6 : 2) * (int64_t)sm_count());
 }
 
 // Widest access that divides the row and suits every pointer.
@@ -211,21 +280,22 @@ int vec_elems(int d, int64_t xs, int64_t rs, std::initializer_list<const void*> 
   return 1;
 }
 
-// Calls f<V, NV, TPR>: up to 32 elements per thread, a warp per row to 1024
-// columns, a block of 128 to 4096, of 512 to 16384.
+// Calls f<V, NV, TPR>.
 template <typename T, int V, typename F>
 void norm_shape(int d, F&& f) {
-  const int nv = d / V;
   auto pick = [&](auto tpr) {
     constexpr int TPR = decltype(tpr)::value;
-    const int per = (nv + TPR - 1) / TPR;
-    if (per * V <= 8 && V <= 8) f(std::integral_constant<int, V>{}, std::integral_constant<int, 8 / V>{}, tpr);
-    else if (per * V <= 16) f(std::integral_constant<int, V>{}, std::integral_constant<int, 16 / V>{}, tpr);
+    const int per = (d / V + TPR - 1) / TPR * V;  // elements per thread
+    if (per <= 8) f(std::integral_constant<int, V>{}, std::integral_constant<int, 8 / V>{}, tpr);
+    else if (per <= 16) f(std::integral_constant<int, V>{}, std::integral_constant<int, 16 / V>{}, tpr);
     else f(std::integral_constant<int, V>{}, std::integral_constant<int, 32 / V>{}, tpr);
   };
-  if (d <= 1024) pick(std::integral_constant<int, 32>{});
-  else if (d <= 4096) pick(std::integral_constant<int, 128>{});
-  else pick(std::integral_constant<int, 512>{});
+  switch (norm_tpr(d)) {
+    case 8: return pick(std::integral_constant<int, 8>{});
+    case 32: return pick(std::integral_constant<int, 32>{});
+    case 128: return pick(std::integral_constant<int, 128>{});
+    default: return pick(std::integral_constant<int, 512>{});
+  }
 }
 
 template <typename T, typename F>
@@ -246,8 +316,8 @@ int norm_fwd(int64_t rows, int d, const T* x, int64_t xs, const T* r, int64_t rs
   if (!x || !w || !y || (r && !t)) return TMPC_ERR_NULL_ARG;
   const int v = vec_elems<T>(d, xs, r ? rs : 0, {x, r, w, y, t});
   norm_dispatch<T>(v, d, [&](auto V, auto NV, auto TPR) {
-    constexpr int rpb = TPR == 32 ? kNormThreads / 32 : 1;
-    norm_fwd_kernel<T, V, NV, TPR><<<(unsigned)((rows + rpb - 1) / rpb), TPR == 32 ? kNormThreads : TPR, 0, st>>>(
+    constexpr int rpb = Rows<TPR>::kRows;
+    norm_fwd_kernel<T, V, NV, TPR><<<(unsigned)((rows + rpb - 1) / rpb), Rows<TPR>::kBlock, 0, st>>>(
         x, r, w, y, t, inv, rows, d, xs, rs, (float)eps);
   });
   return (int)cudaPeekAtLastError();
@@ -271,7 +341,7 @@ int norm_bwd(int64_t rows, int d, const T* dy, const T* ds, const T* t, const T*
   const int v = vec_elems<T>(d, 0, 0, {dy, ds, t, w, dt});
   float* part = static_cast<float*>(ws);
   norm_dispatch<T>(v, d, [&](auto V, auto NV, auto TPR) {
-    norm_bwd_kernel<T, V, NV, TPR><<<nblk, TPR == 32 ? kNormThreads : TPR, TPR == 32 ? d * sizeof(float) : 0, st>>>(
+    norm_bwd_kernel<T, V, NV, TPR><<<nblk, Rows<TPR>::kBlock, TPR <= 32 ? d * sizeof(float) : 0, st>>>(
         dy, ds, t, w, inv, dt, part, rows, d);
   });
   norm_dw_kernel<T><<<(d + 31) / 32, dim3(32, 32), 0, st>>>(part, dw, nblk, d);

@@ -556,3 +556,109 @@ def test_operators_in_a_cuda_graph():
     S.copy_(keep)
     for a, b in zip(out, step()):
         assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------------------
+# Sizes that select other kernels than the lists above
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("rows,d,f", [(20000, 264, 301), (12345, 512, 130), (19001, 256, 256)])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gated_linear_pairs_of_blocks(rows, d, f, act):
+    """Wide bfloat16 products over many tokens: two blocks share a tile; rows that
+    end inside a pair's tile, odd row pitches, a reduction axis of one block and a half."""
+    test_gated_linear(rows, d, f, act, torch.bfloat16)
+
+
+@pytest.mark.parametrize("shape", [(3, 300, 2, 1, 128, 128), (2, 700, 4, 2, 72, 128), (2, 257, 2, 2, 128, 8),
+                                   (1, 5000, 3, 3, 104, 96)], ids=str)
+def test_wide_heads_ignore_what_lies_past_the_lengths(shape):
+    """Heads of more than 64 elements, whole and in segments: NaN and infinities past
+    the lengths reach nothing, gradients included."""
+    q, k, v, g, S, L = attention_inputs(*shape, torch.bfloat16, 30, lengths="ragged")
+    o, st = sequence.linear_attention(q, k, v, g, initial_state=S, lengths=L, return_state=True)
+    ro, rs = ref_attention(q, k, v, g, S, L)
+    assert err(o, ro) < TOL[torch.bfloat16] and err(st, rs) < F32_TOL
+    dirty = [t.clone() for t in (q, k, v)]
+    for t in dirty:
+        for b in range(shape[0]):
+            t[b, L[b]:] = float("nan") if b % 2 else float("inf")
+    o2, st2 = sequence.linear_attention(*dirty, g, initial_state=S, lengths=L, return_state=True)
+    assert torch.equal(o, o2) and torch.equal(st, st2)
+    leaves, dleaves = ([t.clone().requires_grad_(True) for t in x] for x in ((q, k, v), dirty))
+    do = torch.randn(o.shape, generator=gen(31), device="cuda").bfloat16()
+    for a, b in zip(torch.autograd.grad(sequence.linear_attention(*leaves, g, lengths=L), leaves, do),
+                    torch.autograd.grad(sequence.linear_attention(*dleaves, g, lengths=L), dleaves, do)):
+        assert torch.equal(a, b)
+
+
+def test_wide_heads_strided_broadcast_and_unaligned():
+    """Views that the asynchronous copies can and cannot read."""
+    B, T, H, D = 2, 200, 2, 128
+    g = attention_inputs(B, T, H, H, D, D, torch.bfloat16, 0)[3]
+    big = torch.randn(B, T, 3, H, D, generator=gen(32), device="cuda").bfloat16()
+    odd = torch.randn(3, B * T * H * D + 1, generator=gen(33), device="cuda").bfloat16()
+    for q, k, v in (tuple(big[:, :, i] for i in range(3)), tuple(odd[i, 1:].view(B, T, H, D) for i in range(3)),
+                    tuple(big[:1, :, i].expand(B, T, H, D) for i in range(3)),
+                    tuple(big[:, :1, i].expand(B, T, H, D) for i in range(3)),
+                    tuple(big[..., :72][:, :, i] for i in range(3))):
+        assert err(sequence.linear_attention(q, k, v, g), ref_attention(q, k, v, g)[0]) < TOL[torch.bfloat16]
+
+
+def test_without_dlog_the_gradients_are_those_with_it():
+    """log_decay without a gradient selects kernels with fewer terms: the results agree to bfloat16."""
+    for D in (32, 64, 128):
+        q, k, v, g, _, L = attention_inputs(3, 150, 4, 2, D, D, torch.bfloat16, 34, state=False, lengths="ragged")
+        do = torch.randn(q.shape, generator=gen(35), device="cuda").bfloat16()
+        leaves = [t.requires_grad_(True) for t in (q, k, v)]
+        refs = [t.detach().double().requires_grad_(True) for t in leaves]
+        want = torch.autograd.grad(ref_attention(*refs, g, None, L)[0], refs, do.double())
+        for a, b in zip(torch.autograd.grad(sequence.linear_attention(*leaves, g, lengths=L), leaves, do), want):
+            assert err(a, b) < TOL[torch.bfloat16]
+
+
+def test_waits_that_run_out_leave_nan_and_a_usable_context():
+    """With a poll limit of 0 every wait of the tensor-core kernels gives up at once (their
+    copies do complete and are drained): the outputs are NaN, and the next call is right."""
+    from turbompc_b200 import _ffi
+    lib = _ffi.load()
+    x = torch.randn(300, 128, generator=gen(36), device="cuda").bfloat16().requires_grad_(True)
+    w = torch.randn(200, 128, generator=gen(37), device="cuda").bfloat16() / 11
+    X = torch.randn(20000, 264, generator=gen(38), device="cuda").bfloat16()
+    W = torch.randn(304, 264, generator=gen(39), device="cuda").bfloat16() / 16
+    q, k, v, g, S, _ = attention_inputs(2, 300, 2, 1, 128, 128, torch.bfloat16, 40)
+    before = lib.tmpc_set_transfer_poll_limit(0)
+    try:
+        h = sequence.gated_linear(x, w, w)
+        dx, = torch.autograd.grad(h, x, torch.ones_like(h))
+        H = sequence.gated_linear(X, W, W)
+        o, st = sequence.linear_attention(q, k, v, g, initial_state=S, return_state=True)
+        torch.cuda.synchronize()
+    finally:
+        lib.tmpc_set_transfer_poll_limit(before)
+    assert torch.isnan(h).all() and torch.isnan(dx).all() and torch.isnan(H).all()
+    assert torch.isnan(o).all() and torch.isnan(st).all()
+    assert err(sequence.gated_linear(x, w, w).detach(), ref_gated(x.detach(), w, w, "silu")) < TOL[torch.bfloat16]
+    assert err(sequence.gated_linear(X, W, W), ref_gated(X, W, W, "silu")) < TOL[torch.bfloat16]
+    o, st = sequence.linear_attention(q, k, v, g, initial_state=S, return_state=True)
+    ro, rs = ref_attention(q, k, v, g, S)
+    assert err(o, ro) < TOL[torch.bfloat16] and err(st, rs) < F32_TOL
+
+
+def test_gated_linear_from_a_thread_that_made_no_cuda_call():
+    """The maps of the asynchronous copies are made by a driver call, which needs the
+    device's context on the calling thread (a backward pass has a thread of its own)."""
+    import threading
+    x = torch.randn(300, 128, generator=gen(41), device="cuda").bfloat16()
+    w = torch.randn(200, 128, generator=gen(42), device="cuda").bfloat16() / 11
+    want = sequence.gated_linear(x, w, w)
+    torch.empty(300, 200, device="cuda", dtype=torch.bfloat16)  # leaves a block for the thread's output
+    got = []
+
+    def work():
+        with torch.no_grad():
+            got.append(sequence.gated_linear(x, w, w))
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    assert len(got) == 1 and torch.equal(got[0], want)

@@ -447,8 +447,6 @@ __global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Ma
 // A [batch][token][head][d] view as a map of boxes of 64 x 128 tokens.  Fails
 // (false) where TMA cannot read it: a stride of zero on an axis longer than one.
 inline bool view_map(CUtensorMap* m, const TmpcSeqView& v, int d, int heads, int T, int B) {
-  const gemm::EncodeFn fn = gemm::encode_fn();
-  if (!fn) return false;
   const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)T, (cuuint64_t)B};
   const int64_t st[3] = {v.head, v.token, v.batch};
   cuuint64_t strides[3];
@@ -458,10 +456,8 @@ inline bool view_map(CUtensorMap* m, const TmpcSeqView& v, int d, int heads, int
     if (s <= 0 || s >= (int64_t)1 << 40) return false;
     strides[i] = (cuuint64_t)s;
   }
-  const cuuint32_t box[4] = {64, 1, (cuuint32_t)CT, 1}, es[4] = {1, 1, 1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, v.ptr, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)CT, 1};
+  return gemm::encode(m, 4, v.ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <bool STATE_ONLY>

@@ -794,23 +794,38 @@ inline EncodeFn encode_fn() {
   return fn;
 }
 
+// cuTensorMapEncodeTiled.  It is a driver call and needs the device's context on
+// the calling thread; a thread that has made no runtime call yet that sets it up (a
+// backward pass runs on a thread of its own) gets it here.
+inline bool encode(CUtensorMap* m, int rank, void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+                   const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+  const EncodeFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint32_t es[4] = {1, 1, 1, 1};
+  auto call = [&] {
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, base, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = call();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = call();
+  }
+  return r == CUDA_SUCCESS;
+}
+
 // A bfloat16 array [components][outer][inner], rows of `pitch` elements (a
 // multiple of 8, 16-byte aligned base), moved in boxes of box_inner (64, 32 or
 // 16) x box_outer, swizzled over the box's row.
 inline int make_map(CUtensorMap* m, const void* base, int64_t inner, int64_t outer, int comps, int64_t pitch,
                     int box_inner, int box_outer) {
-  const EncodeFn fn = encode_fn();
-  if (!fn) return (int)cudaErrorNotSupported;
   const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)comps};
   const cuuint64_t strides[2] = {(cuuint64_t)pitch * 2, (cuuint64_t)pitch * 2 * (cuuint64_t)outer};
-  const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer, 1}, es[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer, 1};
   const CUtensorMapSwizzle sw = box_inner == 64   ? CU_TENSOR_MAP_SWIZZLE_128B
                                 : box_inner == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
                                                   : CU_TENSOR_MAP_SWIZZLE_32B;
-  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, es,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
+  return encode(m, 3, const_cast<void*>(base), dims, strides, box, sw) ? 0 : (int)cudaErrorInvalidValue;
 }
 
 template <typename T, int MODE, int NT, int ACT, int CG = 1>

@@ -250,11 +250,16 @@ struct State {
       for (int j = 0; j < Z::SC / 8; j += 2) {
         uint32_t r[4];
         ldsm_t(r, frag_bk<F>(b, col0 + j * 8, k * 16));
+        // The matrix instructions' sums are cut, not rounded: the terms meet in an accumulator of their own, smallest
+        // first, and reach the state by a rounded addition.
+        float t0[4] = {}, t1[4] = {};
 #pragma unroll
-        for (int m = 0; m < N; ++m) {
-          mma(s[j], x[m], r[0], r[1]);
-          mma(s[j + 1], x[m], r[2], r[3]);
+        for (int m = N - 1; m >= 0; --m) {
+          mma(t0, x[m], r[0], r[1]);
+          mma(t1, x[m], r[2], r[3]);
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[j][e] += t0[e], s[j + 1][e] += t1[e];
       }
     }
   }
@@ -414,11 +419,11 @@ __global__ void __launch_bounds__(Shape<E, F>::NT, Shape<E, F>::kBlocks) fwd_ker
         for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
       if (state_on) {
 #pragma unroll
-        for (int k = 0; k < E / 16; ++k)
+        for (int m = NS - 1; m >= 0; --m)  // smallest terms first: the sums are cut to the accumulator's size
 #pragma unroll
-          for (int j = 0; j < Z::OC / 8; j += 2)
+          for (int k = 0; k < E / 16; ++k)
 #pragma unroll
-            for (int m = 0; m < NS; ++m) {
+            for (int j = 0; j < Z::OC / 8; j += 2) {
               uint32_t r[4];
               ldsm_t(r, frag_bk<F>(st + m * Z::STATE, col0 + j * 8, k * 16));
               mma(o[j], q[k], r[0], r[1]);
@@ -653,8 +658,8 @@ __global__ void __launch_bounds__(Shape<D, D>::NT, Shape<D, D>::kBlocksDkv) dkv_
               mma(dv[j], ka, f[0], f[1]);
               mma(dv[j + 1], ka, f[2], f[3]);
 #pragma unroll
-              for (int m = 0; m < NS; ++m) {
-                ldsm(f, frag_bn<D>(st + m * Z::STATE, col0 + j * 8, k * 16));  // dk_s = R v_s
+              for (int m = NS - 1; m >= 0; --m) {  // dk_s = R v_s, smallest terms first
+                ldsm(f, frag_bn<D>(st + m * Z::STATE, col0 + j * 8, k * 16));
                 mma(dk[j], va, f[0], f[1]);
                 mma(dk[j + 1], va, f[2], f[3]);
               }

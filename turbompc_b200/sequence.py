@@ -199,7 +199,9 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     at and past a sequence's length give zero outputs and zero gradients and
     leave the state alone.  Returns o (B, T, H, dv), or (o, state) with the
     float32 state after the last token, which ``linear_attention_step`` and a
-    later call's ``initial_state`` continue from.
+    later call's ``initial_state`` continue from.  Products are taken over
+    chunks of tokens in bfloat16, so a NaN or infinity in a valid token may
+    also reach the earlier outputs of its chunk.
 
     Differentiable with respect to q, k, v, log_decay and initial_state.
     """

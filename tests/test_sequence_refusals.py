@@ -124,3 +124,31 @@ def test_wrappers_refuse_shapes_and_devices():
         sequence.gated_linear(q, z(16), z(16))
     with pytest.raises(TypeError):
         sequence.gated_linear(q, z(8, 16, dtype=torch.bfloat16), z(8, 16))
+
+
+def test_calling_module_refuses_what_it_cannot_take():
+    """None before anything is launched; the wrappers turn it into an error."""
+    calls = _ffi.load_sequence()
+    q, g, w = torch.zeros(2, 3, 4, 16), torch.zeros(4), torch.zeros(8, 16)
+    assert calls.linear_attention(q, q, q, g, None, None, None, True) is None
+    assert calls.linear_attention_step(q[:, 0], q[:, 0], q[:, 0], g, None, None, None) is None
+    assert calls.add_rms_norm("x", None, g, 1e-6, False) is None
+    assert calls.gated_linear(q, w, None, 0) is None
+    with pytest.raises(RuntimeError):
+        calls.linear_attention(q)
+    with pytest.raises(TypeError):
+        calls.bind(3)
+    with pytest.raises(TypeError):
+        calls.bind([0])
+
+
+@pytest.mark.gpu
+def test_calling_module_raises_the_entry_points_errors():
+    x, w = torch.zeros(2, 16, device="cuda"), torch.zeros(8, 16, device="cuda")
+    with pytest.raises(_ffi.TmpcError, match="tmpc_gated_linear_f32") as e:
+        _ffi.load_sequence().gated_linear(x, w, w, 7)  # no such activation
+    assert e.value.code == -3
+    with pytest.raises(TypeError):
+        sequence.add_rms_norm(x, x, w[0], eps="small")
+    with pytest.raises(TypeError):
+        sequence.linear_attention(*[x.view(1, 2, 1, 16)] * 3, torch.zeros(1, device="cuda"), scale="small")

@@ -7,6 +7,8 @@ the library is missing or a call fails, an exception is raised.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.machinery
+import importlib.util
 import os
 import threading
 
@@ -132,6 +134,7 @@ for _s in ("f32", "bf16"):
                                                  [C.c_int32] + [_P] * 5 + [C.c_size_t, _P])
 
 _lib = None
+_sequence = None
 _lock = threading.Lock()
 
 
@@ -160,6 +163,24 @@ def load(build_if_missing: bool = True):
             fn.argtypes = args
         _lib = lib
         return lib
+
+
+def load_sequence():
+    """The module that makes the sequence operators' calls, bound to the
+    library's entry points (both built first if needed)."""
+    global _sequence
+    lib = load()
+    with _lock:
+        if _sequence is None:
+            path = _build.SEQ_LIB
+            if not os.path.exists(path):
+                _build.build_sequence()
+            loader = importlib.machinery.ExtensionFileLoader("tmpc_sequence", path)
+            module = importlib.util.module_from_spec(importlib.util.spec_from_loader("tmpc_sequence", loader))
+            loader.exec_module(module)
+            module.bind([C.cast(getattr(lib, name), C.c_void_p).value for name in module.names()])
+            _sequence = module
+        return _sequence
 
 
 def exported_symbols():

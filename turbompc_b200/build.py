@@ -3,7 +3,9 @@
 Plain ``nvcc`` (no torch JIT cache): every ``csrc/*.cu`` file is compiled to an
 object in ``turbompc_b200/_build/`` (in parallel) and linked into one shared
 library exporting the C ABI declared in ``include/tmpc_b200.h``.  The library
-is rebuilt when a source or header is newer than it.
+is rebuilt when a source or header is newer than it.  The module through which
+PyTorch calls the sequence operators (``csrc/ffi/sequence_torch.cc``) is built
+beside it by g++, against torch's headers.
 
     python -m turbompc_b200.build [--force] [--verbose]
 """
@@ -16,6 +18,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -93,6 +96,35 @@ def build(force: bool = False, verbose: bool = False, extra=()) -> str:
     return LIB
 
 
+SEQ_SRC = os.path.join(CSRC, "ffi", "sequence_torch.cc")
+SEQ_LIB = os.path.join(LIBDIR, "tmpc_sequence" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_sequence(force: bool = False) -> str:
+    """Compile the sequence operators' calling module (csrc/ffi/sequence_torch.cc)
+    against this interpreter's and torch's headers, if it is missing or older
+    than its source; returns its path."""
+    deps = [SEQ_SRC, os.path.join(INCLUDE, "tmpc_b200.h")]
+    if not force and os.path.exists(SEQ_LIB) and os.path.getmtime(SEQ_LIB) >= max(map(os.path.getmtime, deps)):
+        return SEQ_LIB
+    import torch
+
+    at = os.path.dirname(torch.__file__)
+    os.makedirs(LIBDIR, exist_ok=True)
+    tmp = f"{SEQ_LIB}.{os.getpid()}.tmp"
+    cuda_inc = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-I" + os.path.join(at, "include"),
+           "-I" + os.path.join(at, "include", "torch", "csrc", "api", "include"),
+           "-I" + sysconfig.get_paths()["include"], "-I" + cuda_inc, "-I" + INCLUDE,
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", SEQ_SRC, "-o", tmp,
+           "-L" + os.path.join(at, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"build of {SEQ_SRC} failed:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, SEQ_LIB)
+    return SEQ_LIB
+
+
 FFI_SRC = os.path.join(CSRC, "ffi", "admm_b200_ffi.cc")
 FFI_LIB = os.path.join(LIBDIR, "libtmpc_b200_ffi.so")
 
@@ -123,5 +155,6 @@ if __name__ == "__main__":
                     help="also build the XLA FFI handlers against these jaxlib headers")
     a = ap.parse_args()
     print(build(force=a.force, verbose=a.verbose))
+    print(build_sequence(force=a.force))
     if a.ffi:
         print(build_ffi(a.ffi))

@@ -1,0 +1,436 @@
+// The sequence operators' calls from PyTorch: a CPython module over the C ABI.
+//
+// A step of a few environments runs for 3 us on the GPU; building the same call
+// from Python (checks, outputs, addresses, the call itself) took 14.  Here it
+// takes what allocating the outputs and the launch cost.
+//
+// Functions take tensors, check them, allocate the outputs (and a workspace of
+// the caching allocator's, which is safe to drop after the launch) and make one C
+// call on the device's current stream, without Python's lock.  Arguments that an
+// operator refuses make it return None before anything is launched: the Python
+// side then finds out which one and raises.  The C entry points come in by address
+// (bind), so that there is one library in the process, whichever was loaded.
+#include <ATen/core/Tensor.h>
+#include <ATen/core/grad_mode.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <climits>
+#include <cmath>
+#include <cstring>
+#include <optional>
+#include <string>
+
+#include "tmpc_b200.h"
+
+namespace {
+
+using at::Tensor;
+using Opt = std::optional<Tensor>;
+constexpr int kMaxHead = 128;
+
+// Per dtype: float, bfloat16.
+struct Entries {
+  decltype(&tmpc_linear_attention_f32) attention[2];
+  decltype(&tmpc_linear_attention_backward_f32) attention_backward[2];
+  decltype(&tmpc_linear_attention_step_f32) step[2];
+  decltype(&tmpc_add_rms_norm_f32) norm[2];
+  decltype(&tmpc_add_rms_norm_backward_f32) norm_backward[2];
+  decltype(&tmpc_gated_linear_f32) gated[2];
+  decltype(&tmpc_gated_linear_backward_f32) gated_backward[2];
+  decltype(&tmpc_linear_attention_workspace_bytes) attention_ws;
+  decltype(&tmpc_linear_attention_backward_workspace_bytes) attention_backward_ws;
+  decltype(&tmpc_add_rms_norm_workspace_bytes) norm_ws;
+  decltype(&tmpc_gated_linear_workspace_bytes) gated_ws;
+  decltype(&tmpc_gated_linear_backward_workspace_bytes) gated_backward_ws;
+} fn;
+const char* const kPlain[] = {"tmpc_linear_attention_workspace_bytes", "tmpc_linear_attention_backward_workspace_bytes",
+                              "tmpc_add_rms_norm_workspace_bytes", "tmpc_gated_linear_workspace_bytes",
+                              "tmpc_gated_linear_backward_workspace_bytes"};
+const char* const kTyped[] = {"tmpc_linear_attention", "tmpc_linear_attention_backward", "tmpc_linear_attention_step",
+                              "tmpc_add_rms_norm",     "tmpc_add_rms_norm_backward",     "tmpc_gated_linear",
+                              "tmpc_gated_linear_backward"};
+enum { kAttention, kAttentionBackward, kStep, kNorm, kNormBackward, kGated, kGatedBackward };
+bool bound = false;
+
+PyObject* refused() { Py_RETURN_NONE; }
+
+PyObject* wrap(const Tensor& t) { return THPVariable_Wrap(t); }
+PyObject* wrap(const Opt& t) {
+  if (t) return THPVariable_Wrap(*t);
+  Py_RETURN_NONE;
+}
+template <typename... Ts>
+PyObject* tuple_of(const Ts&... ts) {
+  PyObject* out = PyTuple_New(sizeof...(Ts));
+  if (!out) return nullptr;
+  Py_ssize_t i = 0;
+  bool ok = true;
+  (([&] {
+     PyObject* o = wrap(ts);
+     ok = ok && o;
+     PyTuple_SET_ITEM(out, i++, o);
+   }()),
+   ...);
+  if (ok) return out;
+  Py_DECREF(out);
+  return nullptr;
+}
+
+const Tensor* tensor(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
+// None or a tensor; false: neither.
+bool optional(PyObject* o, const Tensor*& t) {
+  t = o == Py_None ? nullptr : tensor(o);
+  return t || o == Py_None;
+}
+template <typename P = void>
+P* ptr(const Tensor* t) {
+  return t ? static_cast<P*>(t->data_ptr()) : nullptr;
+}
+template <typename P = void>
+P* ptr(const Opt& t) {
+  return t ? static_cast<P*>(t->data_ptr()) : nullptr;
+}
+// 0 float, 1 bfloat16, -1 neither
+int type_of(const Tensor& t) {
+  return t.scalar_type() == at::kFloat ? 0 : t.scalar_type() == at::kBFloat16 ? 1 : -1;
+}
+bool like(const Tensor* t, at::ScalarType type, const Tensor& on) {
+  return t && t->is_cuda() && t->scalar_type() == type && t->device() == on.device();
+}
+bool needs_grad(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t && t->requires_grad()) return true;
+  return false;
+}
+// The kernels take any stride but the last axis's.
+Tensor rows(const Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+// Contiguous, and at an address that TMA can read.
+Tensor aligned(const Tensor& t) {
+  Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
+}
+Tensor empty(at::IntArrayRef shape, const Tensor& like) { return at::empty(shape, like.options().requires_grad(false)); }
+Tensor empty_float(at::IntArrayRef shape, const Tensor& like) {
+  return at::empty(shape, like.options().dtype(at::kFloat).requires_grad(false));
+}
+Opt workspace(size_t bytes, const Tensor& like) {
+  if (!bytes) return std::nullopt;
+  return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte).requires_grad(false));
+}
+TmpcSeqView view(const Tensor& t) {  // (B, T, heads, dim), or (B, heads, dim): one token
+  const auto s = t.strides();
+  return s.size() == 3 ? TmpcSeqView{t.data_ptr(), s[0], 0, s[1]} : TmpcSeqView{t.data_ptr(), s[0], s[1], s[2]};
+}
+
+// One C call on the current stream of t's device; false with a Python exception set.
+template <typename F>
+bool call(const Tensor& t, int entry, F&& launch) {
+  const c10::cuda::CUDAGuard guard(t.device());
+  tmpc_stream_t stream = c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
+  int32_t code;
+  Py_BEGIN_ALLOW_THREADS;
+  code = launch(stream);
+  Py_END_ALLOW_THREADS;
+  if (!code) return true;
+  PyObject* ffi = PyImport_ImportModule("turbompc_b200._ffi");
+  PyObject* type = ffi ? PyObject_GetAttrString(ffi, "TmpcError") : nullptr;
+  if (type) {
+    PyObject* e = PyObject_CallFunction(type, "si", (std::string(kTyped[entry]) + (type_of(t) ? "_bf16" : "_f32")).c_str(), code);
+    if (e) PyErr_SetObject(type, e);
+    Py_XDECREF(e);
+  }
+  Py_XDECREF(type);
+  Py_XDECREF(ffi);
+  return false;
+}
+
+// None: 1 / sqrt(dk)
+bool scale_of(PyObject* o, int dk, double& s) {
+  s = o == Py_None ? 1. / std::sqrt((double)dk) : PyFloat_AsDouble(o);
+  return o == Py_None || !(s == -1. && PyErr_Occurred());
+}
+
+// The dimensions of q, k, v (with a token axis or without) and log_decay, if they fit.
+bool attention_dims(const Tensor* q, const Tensor* k, const Tensor* v, const Tensor* decay, int axes,
+                    TmpcLinAttnDims& d) {
+  if (!q || !k || !v || !decay || type_of(*q) < 0 || !q->is_cuda() || !like(k, q->scalar_type(), *q) ||
+      !like(v, q->scalar_type(), *q) || !like(decay, at::kFloat, *q) || q->dim() != axes || k->dim() != axes ||
+      v->dim() != axes || decay->dim() != 1)
+    return false;
+  const auto sq = q->sizes(), sk = k->sizes(), sv = v->sizes();
+  for (int i = 0; i + 2 < axes; ++i)
+    if (sk[i] != sq[i] || sv[i] != sq[i] || sq[i] > INT_MAX) return false;
+  const int64_t H = sq[axes - 2], G = sk[axes - 2], dk = sq[axes - 1], dv = sv[axes - 1];
+  if (sv[axes - 2] != G || sk[axes - 1] != dk || G < 1 || H < 1 || H > INT_MAX || H % G || decay->size(0) != H || dk < 1 ||
+      dk > kMaxHead || dv < 1 || dv > kMaxHead)
+    return false;
+  d = {(int32_t)sq[0], axes == 4 ? (int32_t)sq[1] : 1, (int32_t)H, (int32_t)G, (int32_t)dk, (int32_t)dv};
+  return true;
+}
+bool is_state(const Tensor* t, const TmpcLinAttnDims& d, const Tensor& q) {
+  return like(t, at::kFloat, q) && t->sizes() == at::IntArrayRef({d.B, d.H, d.dk, d.dv});
+}
+
+#define ARGS(n)                                                              \
+  HANDLE_TH_ERRORS                                                           \
+  if (!bound || count != (n)) {                                              \
+    PyErr_SetString(PyExc_RuntimeError, "entry points not bound, or a wrong number of arguments"); \
+    return nullptr;                                                          \
+  }
+
+// linear_attention(q, k, v, log_decay, initial, lengths, scale, want_state) -> (o, state or None)
+PyObject* linear_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  ARGS(8)
+  const Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]), *decay = tensor(a[3]), *initial, *lengths;
+  TmpcLinAttnDims d;
+  if (!attention_dims(q, k, v, decay, 4, d) || !optional(a[4], initial) || !optional(a[5], lengths) ||
+      (initial && !is_state(initial, d, *q)) ||
+      (lengths && !(like(lengths, at::kInt, *q) && lengths->sizes() == at::IntArrayRef({d.B}))))
+    return refused();
+  double scale;
+  if (!scale_of(a[6], d.dk, scale)) return nullptr;
+  const Tensor q1 = rows(*q), k1 = rows(*k), v1 = rows(*v), decay1 = decay->contiguous();
+  const Opt initial1 = initial ? Opt(initial->contiguous()) : Opt(), lengths1 = lengths ? Opt(lengths->contiguous()) : Opt();
+  const Tensor o = empty({d.B, d.T, d.H, d.dv}, *q);
+  const Opt state = a[7] == Py_True ? Opt(empty_float({d.B, d.H, d.dk, d.dv}, *q)) : Opt();
+  const size_t need = fn.attention_ws(&d);
+  const Opt ws = workspace(need, *q);
+  const TmpcSeqView qv = view(q1), kv = view(k1), vv = view(v1), ov = view(o);
+  if (!call(*q, kAttention, [&](tmpc_stream_t st) {
+        return fn.attention[type_of(*q)](&d, &qv, &kv, &vv, &ov, ptr<float>(&decay1), ptr<int32_t>(lengths1),
+                                         ptr<float>(initial1), ptr<float>(state), scale, ptr(ws), need, st);
+      }))
+    return nullptr;
+  return tuple_of(o, state);
+  END_HANDLE_TH_ERRORS
+}
+
+// linear_attention_backward(q, k, v, log_decay, initial, lengths, scale, do or None, dstate or None, want dlog_decay,
+//                           want dinitial) -> (dq, dk, dv, dlog_decay or None, dinitial or None)
+// The first seven as linear_attention took them.
+PyObject* linear_attention_backward(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  ARGS(11)
+  const Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]), *decay = tensor(a[3]), *initial, *lengths, *dout,
+               *dstate;
+  TmpcLinAttnDims d;
+  if (!attention_dims(q, k, v, decay, 4, d) || !optional(a[4], initial) || !optional(a[5], lengths) ||
+      !optional(a[7], dout) || !optional(a[8], dstate))
+    return refused();
+  double scale;
+  if (!scale_of(a[6], d.dk, scale)) return nullptr;
+  const Tensor q1 = rows(*q), k1 = rows(*k), v1 = rows(*v), decay1 = decay->contiguous();
+  const Tensor do1 = dout ? rows(*dout) : at::zeros({d.B, d.T, d.H, d.dv}, q->options().requires_grad(false));
+  const Opt initial1 = initial ? Opt(initial->contiguous()) : Opt(), lengths1 = lengths ? Opt(lengths->contiguous()) : Opt(),
+            dstate1 = dstate ? Opt(dstate->contiguous()) : Opt();
+  const Tensor dq = empty(q->sizes(), *q), dk = empty(k->sizes(), *q), dv = empty(v->sizes(), *q);
+  const Opt dlog = a[9] == Py_True ? Opt(empty_float({d.H}, *q)) : Opt();
+  const Opt dinit = a[10] == Py_True ? Opt(empty_float({d.B, d.H, d.dk, d.dv}, *q)) : Opt();
+  const size_t need = fn.attention_backward_ws(&d);
+  const Opt ws = workspace(need, *q);
+  const TmpcSeqView qv = view(q1), kv = view(k1), vv = view(v1), dov = view(do1), dqv = view(dq), dkv = view(dk),
+                    dvv = view(dv);
+  if (!call(*q, kAttentionBackward, [&](tmpc_stream_t st) {
+        return fn.attention_backward[type_of(*q)](&d, &qv, &kv, &vv, &dov, &dqv, &dkv, &dvv, ptr<float>(&decay1),
+                                                  ptr<int32_t>(lengths1), ptr<float>(initial1), ptr<float>(dstate1),
+                                                  ptr<float>(dlog), ptr<float>(dinit), scale, ptr(ws), need, st);
+      }))
+    return nullptr;
+  return tuple_of(dq, dk, dv, dlog, dinit);
+  END_HANDLE_TH_ERRORS
+}
+
+// linear_attention_step(q, k, v, log_decay, state, state_out or None, scale) -> o
+PyObject* linear_attention_step(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  ARGS(7)
+  const Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]), *decay = tensor(a[3]), *state = tensor(a[4]), *out;
+  TmpcLinAttnDims d;
+  if (!attention_dims(q, k, v, decay, 3, d) || !optional(a[5], out)) return refused();
+  if (!out) out = state;
+  if (!is_state(state, d, *q) || !is_state(out, d, *q) || !state->is_contiguous() || !out->is_contiguous() ||
+      needs_grad({q, k, v, decay, state, out}))
+    return refused();
+  double scale;
+  if (!scale_of(a[6], d.dk, scale)) return nullptr;
+  const Tensor q1 = rows(*q), k1 = rows(*k), v1 = rows(*v), decay1 = decay->contiguous();
+  const Tensor o = empty({d.B, d.H, d.dv}, *q);
+  const TmpcSeqView qv = view(q1), kv = view(k1), vv = view(v1), ov = view(o);
+  if (!call(*q, kStep, [&](tmpc_stream_t st) {
+        return fn.step[type_of(*q)](&d, &qv, &kv, &vv, &ov, ptr<float>(&decay1), ptr<float>(state), ptr<float>(out), scale,
+                                    st);
+      }))
+    return nullptr;
+  return wrap(o);
+  END_HANDLE_TH_ERRORS
+}
+
+// Rows of the last axis at one stride: t, or a copy.
+Tensor as_rows(const Tensor& t, int64_t d) {
+  if (t.is_contiguous() || t.dim() == 2) return rows(t);
+  return rows(t.reshape({t.numel() / d, d}));
+}
+int64_t row_stride(const Tensor& t, int64_t d) { return t.dim() == 2 ? t.stride(0) : d; }
+
+// add_rms_norm(x, residual or None, weight, eps, want_inv) -> (y, t or None, inv or None)
+PyObject* add_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  ARGS(5)
+  const Tensor *x = tensor(a[0]), *residual, *weight = tensor(a[2]);
+  if (!x || type_of(*x) < 0 || !x->is_cuda() || !optional(a[1], residual) || !like(weight, x->scalar_type(), *x) ||
+      x->dim() < 1 || weight->dim() != 1)
+    return refused();
+  const int64_t d = x->size(-1);
+  if (d < 1 || d > 16384 || weight->size(0) != d ||
+      (residual && !(like(residual, x->scalar_type(), *x) && residual->sizes() == x->sizes())))
+    return refused();
+  const double eps = PyFloat_AsDouble(a[3]);
+  if (eps == -1. && PyErr_Occurred()) return nullptr;
+  const int64_t n = x->numel() / d;
+  const Tensor x1 = as_rows(*x, d), w1 = weight->contiguous();
+  const Opt r1 = residual ? Opt(as_rows(*residual, d)) : Opt();
+  const Tensor y = empty(x->sizes(), *x);
+  const Opt sum = residual ? Opt(empty(x->sizes(), *x)) : Opt();
+  const Opt inv = a[4] == Py_True ? Opt(empty_float({n}, *x)) : Opt();
+  if (!call(*x, kNorm, [&](tmpc_stream_t st) {
+        return fn.norm[type_of(*x)](n, (int32_t)d, ptr(&x1), row_stride(x1, d), ptr(r1), r1 ? row_stride(*r1, d) : 0,
+                                    ptr(&w1), eps, ptr(&y), ptr(sum), ptr<float>(inv), st);
+      }))
+    return nullptr;
+  return tuple_of(y, sum, inv);
+  END_HANDLE_TH_ERRORS
+}
+
+// add_rms_norm_backward(t, weight, inv, dy or None, dt or None) -> (dx, dweight), t contiguous, as saved
+PyObject* add_rms_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  ARGS(5)
+  const Tensor *t = tensor(a[0]), *weight = tensor(a[1]), *inv = tensor(a[2]), *dy, *dt;
+  if (!t || type_of(*t) < 0 || !weight || !inv || !t->is_contiguous() || !optional(a[3], dy) || !optional(a[4], dt))
+    return refused();
+  const int64_t d = t->size(-1), n = inv->numel();
+  const Tensor w1 = weight->contiguous();
+  const Tensor dy1 = dy ? dy->contiguous() : at::zeros(t->sizes(), t->options().requires_grad(false));
+  const Opt dt1 = dt ? Opt(dt->contiguous()) : Opt();
+  const Tensor dx = empty(t->sizes(), *t), dw = empty({d}, *t);
+  const size_t need = fn.norm_ws(n, (int32_t)d);
+  const Opt ws = workspace(need, *t);
+  if (!call(*t, kNormBackward, [&](tmpc_stream_t st) {
+        return fn.norm_backward[type_of(*t)](n, (int32_t)d, ptr(&dy1), ptr(dt1), ptr(t), ptr(&w1), ptr<float>(inv),
+                                             ptr(&dx), ptr(&dw), ptr(ws), need, st);
+      }))
+    return nullptr;
+  return tuple_of(dx, dw);
+  END_HANDLE_TH_ERRORS
+}
+
+// x (..., d), w_gate and w_up (f, d), if they fit
+bool gated_dims(const Tensor* x, const Tensor* wg, const Tensor* wu, int64_t& n, int64_t& d, int64_t& f) {
+  if (!x || type_of(*x) < 0 || !x->is_cuda() || !like(wg, x->scalar_type(), *x) || !like(wu, x->scalar_type(), *x) ||
+      x->dim() < 1 || wg->dim() != 2 || wg->sizes() != wu->sizes())
+    return false;
+  d = x->size(-1), f = wg->size(0);
+  if (d < 1 || f < 1 || wg->size(1) != d || d > INT_MAX || f > INT_MAX) return false;
+  n = x->numel() / d;
+  return true;
+}
+
+// gated_linear(x, w_gate, w_up, activation) -> h
+PyObject* gated_linear(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  ARGS(4)
+  const Tensor *x = tensor(a[0]), *wg = tensor(a[1]), *wu = tensor(a[2]);
+  int64_t n, d, f;
+  if (!gated_dims(x, wg, wu, n, d, f)) return refused();
+  const long act = PyLong_AsLong(a[3]);
+  if (act == -1 && PyErr_Occurred()) return nullptr;
+  const Tensor x1 = aligned(*x), g1 = aligned(*wg), u1 = aligned(*wu);
+  auto shape = x->sizes().vec();
+  shape.back() = f;
+  const Tensor h = empty(shape, *x);
+  const size_t need = fn.gated_ws(n, (int32_t)d, (int32_t)f, (int32_t)x->element_size());
+  const Opt ws = workspace(need, *x);
+  if (!call(*x, kGated, [&](tmpc_stream_t st) {
+        return fn.gated[type_of(*x)](n, (int32_t)d, (int32_t)f, ptr(&x1), ptr(&g1), ptr(&u1), (int32_t)act, ptr(&h),
+                                     ptr(ws), need, st);
+      }))
+    return nullptr;
+  return wrap(h);
+  END_HANDLE_TH_ERRORS
+}
+
+// gated_linear_backward(x, w_gate, w_up, activation, dh, want dx, want dw) -> (dx, dw_gate, dw_up), or None in their place
+PyObject* gated_linear_backward(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  ARGS(7)
+  const Tensor *x = tensor(a[0]), *wg = tensor(a[1]), *wu = tensor(a[2]), *dh = tensor(a[4]);
+  int64_t n, d, f;
+  if (!gated_dims(x, wg, wu, n, d, f) || !dh) return refused();
+  const long act = PyLong_AsLong(a[3]);
+  if (act == -1 && PyErr_Occurred()) return nullptr;
+  const Tensor x1 = aligned(*x), g1 = aligned(*wg), u1 = aligned(*wu), dh1 = dh->contiguous();
+  const bool want_w = a[6] == Py_True;
+  const Opt dx = a[5] == Py_True ? Opt(empty(x->sizes(), *x)) : Opt();
+  const Opt dg = want_w ? Opt(empty(wg->sizes(), *x)) : Opt(), du = want_w ? Opt(empty(wg->sizes(), *x)) : Opt();
+  const size_t need = fn.gated_backward_ws(n, (int32_t)d, (int32_t)f, (int32_t)x->element_size());
+  const Opt ws = workspace(need, *x);
+  if (!call(*x, kGatedBackward, [&](tmpc_stream_t st) {
+        return fn.gated_backward[type_of(*x)](n, (int32_t)d, (int32_t)f, ptr(&x1), ptr(&g1), ptr(&u1), (int32_t)act,
+                                              ptr(&dh1), ptr(dx), ptr(dg), ptr(du), ptr(ws), need, st);
+      }))
+    return nullptr;
+  return tuple_of(dx, dg, du);
+  END_HANDLE_TH_ERRORS
+}
+
+// names() -> the entry points that bind expects; bind(addresses, in that order)
+PyObject* names(PyObject*, PyObject*) {
+  PyObject* out = PyList_New(0);
+  auto add = [&](const std::string& s) {
+    PyObject* o = PyUnicode_FromString(s.c_str());
+    const bool ok = o && PyList_Append(out, o) == 0;
+    Py_XDECREF(o);
+    return ok;
+  };
+  bool ok = out;
+  for (const char* n : kTyped)
+    for (const char* s : {"_f32", "_bf16"}) ok = ok && add(std::string(n) + s);
+  for (const char* n : kPlain) ok = ok && add(n);
+  if (ok) return out;
+  Py_XDECREF(out);
+  return nullptr;
+}
+PyObject* bind(PyObject*, PyObject* list) {
+  constexpr Py_ssize_t n = 2 * std::size(kTyped) + std::size(kPlain);
+  static_assert(sizeof(Entries) == n * sizeof(void*), "the entry points, in the order of their names");
+  if (!PyList_Check(list) || PyList_GET_SIZE(list) != n) {
+    PyErr_SetString(PyExc_TypeError, "bind takes the list of the entry points' addresses");
+    return nullptr;
+  }
+  void* at[n];
+  for (Py_ssize_t i = 0; i < n; ++i)
+    if (!(at[i] = PyLong_AsVoidPtr(PyList_GET_ITEM(list, i)))) {
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "an entry point's address is null");
+      return nullptr;
+    }
+  std::memcpy(&fn, at, sizeof fn);
+  bound = true;
+  Py_RETURN_NONE;
+}
+
+#define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
+PyMethodDef methods[] = {FAST(linear_attention),
+                         FAST(linear_attention_backward),
+                         FAST(linear_attention_step),
+                         FAST(add_rms_norm),
+                         FAST(add_rms_norm_backward),
+                         FAST(gated_linear),
+                         FAST(gated_linear_backward),
+                         {"names", names, METH_NOARGS, nullptr},
+                         {"bind", bind, METH_O, nullptr},
+                         {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "tmpc_sequence", nullptr, -1, methods};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit_tmpc_sequence() { return PyModule_Create(&module); }

@@ -146,6 +146,13 @@ def test_linear_attention_backward(shape, dtype, lengths):
         assert err(got[4], want[4]) < F32_TOL
 
 
+@pytest.mark.parametrize("shape", [(1250, 5, 2, 1, 16, 24), (610, 3, 1, 1, 64, 40), (155, 4, 2, 1, 128, 20)], ids=str)
+@pytest.mark.parametrize("lengths", [None, "ragged"])
+def test_linear_attention_backward_of_many_states(shape, lengths):
+    """More float states than the device holds at once: the gradient's passes one after the other."""
+    test_linear_attention_backward(shape, torch.float32, lengths)
+
+
 def test_linear_attention_backward_of_the_state_alone():
     q, k, v, g, S, _ = attention_inputs(2, 33, 2, 1, 32, 32, torch.float32, 4)
     leaves = [t.requires_grad_(True) for t in (q, k, v, g, S)]

@@ -61,11 +61,10 @@ struct Smem {
 };
 
 template <int D, bool REV, bool LOG, bool OUT>
-__global__ void __launch_bounds__(Shape<D>::BLOCK, D == 128 ? 1 : LOG ? 3 : 4) pass_kernel(const Args p) {
+__device__ __forceinline__ void pass_block(const Args& p, int64_t block, char* raw) {
   using Z = Shape<D>;
-  extern __shared__ __align__(16) char raw[];
   const int sub = threadIdx.x / Z::NT, tid = threadIdx.x % Z::NT, lane = threadIdx.x & 31;
-  const int64_t unit = (int64_t)blockIdx.x * Z::UNITS + sub;
+  const int64_t unit = block * Z::UNITS + sub;
   if (unit >= p.units) return;  // whole warps; a block of several states has no block-wide barrier
   auto sync = [&] {
     if constexpr (Z::UNITS > 1) __syncwarp();
@@ -273,6 +272,30 @@ __global__ void __launch_bounds__(Shape<D>::BLOCK, D == 128 ? 1 : LOG ? 3 : 4) p
   }
 }
 
+template <int D, bool LOG>
+constexpr int kBlocks = D == 128 ? 1 : LOG ? 3 : 4;  // per SM
+
+template <int D, bool REV, bool LOG, bool OUT>
+__global__ void __launch_bounds__(Shape<D>::BLOCK, kBlocks<D, LOG>) pass_kernel(const Args p) {
+  extern __shared__ __align__(16) char raw[];
+  pass_block<D, REV, LOG, OUT>(p, blockIdx.x, raw);
+}
+
+// The three passes of the gradient side by side.
+struct BackwardArgs {
+  Args q, v, k;
+  int q_blocks, kv_blocks;
+};
+template <int D, bool LOG>
+__global__ void __launch_bounds__(Shape<D>::BLOCK, kBlocks<D, LOG>)
+    backward_kernel(const __grid_constant__ BackwardArgs p) {
+  extern __shared__ __align__(16) char raw[];
+  const int i = (int)blockIdx.x - p.q_blocks;
+  if (i < 0) pass_block<D, false, LOG, true>(p.q, blockIdx.x, raw);
+  else if (i < p.kv_blocks) pass_block<D, true, false, true>(p.v, i, raw);
+  else pass_block<D, true, false, true>(p.k, i - p.kv_blocks, raw);
+}
+
 // In place: what each segment leaves alone -> the state (and M) before each
 // segment, or (REV) the adjoint after each.
 template <bool REV, bool LOG>
@@ -356,6 +379,22 @@ int pass(Args p, const TmpcLinAttnDims* d, float* seg, float* segm, const float*
   return run<REV, LOG, true>(p, d, st);
 }
 
+// dq, dv and dk of whole sequences in one launch.
+template <bool LOG>
+int backward(BackwardArgs p, const TmpcLinAttnDims* d, cudaStream_t st) {
+  int rc = 0;
+  by_size(d, [&](auto dd) {
+    constexpr int D = decltype(dd)::value, U = Shape<D>::UNITS;
+    constexpr int smem = U * (int)sizeof(Smem<D, LOG>);
+    p.q.units = (int64_t)d->B * d->H, p.v.units = p.k.units = (int64_t)d->B * d->G;
+    p.q_blocks = (int)((p.q.units + U - 1) / U), p.kv_blocks = (int)((p.v.units + U - 1) / U);
+    rc = allow_smem<backward_kernel<D, LOG>>(smem);
+    if (!rc)
+      backward_kernel<D, LOG><<<(unsigned)p.q_blocks + 2u * (unsigned)p.kv_blocks, Shape<D>::BLOCK, smem, st>>>(p);
+  });
+  return rc ? rc : (int)cudaPeekAtLastError();
+}
+
 // States that fit the device at once, by the registers.
 inline int64_t resident(const TmpcLinAttnDims* d) {
   const int m = std::max(d->dk, d->dv);
@@ -420,9 +459,6 @@ int LinAttn<float>::backward(LinAttnArgs a, const TmpcLinAttnDims* d, float* dlo
   q.e = d->dv, q.f = d->dk, q.si = 1, q.sj = d->dv;
   q.a_scale = a.scale;
   q.dstate_out = a.dstate_out, q.dlog = part;
-  int rc = dlog_decay ? rec::pass<false, true>(q, d, seg, segm, a.state_in, st)
-                      : rec::pass<false, false>(q, d, seg, nullptr, a.state_in, st);
-  if (rc) return rc;
   p.rep = d->H / d->G;
   p.a_key = true;
   p.b_scale = a.scale;
@@ -430,11 +466,24 @@ int LinAttn<float>::backward(LinAttnArgs a, const TmpcLinAttnDims* d, float* dlo
   v.a = a.k, v.b = a.q, v.c = a.o, v.o = a.gv;
   v.e = d->dk, v.f = d->dv, v.si = d->dv, v.sj = 1;
   v.state_out = a.dstate_in;
-  rc = rec::pass<true, false>(v, d, seg, nullptr, a.dstate_out, st);
-  if (rc) return rc;
   p.a = a.v, p.b = a.o, p.c = a.q, p.o = a.gk;  // dk
   p.e = d->dv, p.f = d->dk, p.si = 1, p.sj = d->dv;
-  rc = rec::pass<true, false>(p, d, seg, nullptr, a.dstate_out, st);
+  int rc = 0;
+  // Few states leave the SMs' schedulers idle between a token's dependent steps:
+  // the three passes then go side by side (51 tokens, 4 heads of 32 x 24: 24 us
+  // against 48 for 64 sequences, 52 against 61 for 256). Where one pass fills the
+  // device, one after the other, as each runs with more registers or more blocks
+  // (617 us against 652 for 4096 sequences; heads of 64, 256 sequences: 172 against 184).
+  if (p.nseg == 1 && (int64_t)d->B * d->H <= rec::resident(d)) {
+    q.state_in = a.state_in, v.state_in = p.state_in = a.dstate_out;
+    const rec::BackwardArgs all{q, v, p};
+    rc = dlog_decay ? rec::backward<true>(all, d, st) : rec::backward<false>(all, d, st);
+  } else {  // with segments, they share the workspace of the segments' states
+    rc = dlog_decay ? rec::pass<false, true>(q, d, seg, segm, a.state_in, st)
+                    : rec::pass<false, false>(q, d, seg, nullptr, a.state_in, st);
+    if (!rc) rc = rec::pass<true, false>(v, d, seg, nullptr, a.dstate_out, st);
+    if (!rc) rc = rec::pass<true, false>(p, d, seg, nullptr, a.dstate_out, st);
+  }
   if (rc) return rc;
   if (dlog_decay) rec::dlog_kernel<<<d->H, 128, 0, st>>>(part, dlog_decay, d->B, d->H, p.nseg);
   return (int)cudaPeekAtLastError();

@@ -13,6 +13,8 @@ Errors are norm-wise, |got - want| / |want|.  Tolerances:
 * the norm in float32: a few roundings and a sum of at most 2^14 squares: 2^-20;
 * dlog_decay: a sum of signed terms over every token, so its error is taken
   against the root sum of squares of the sequences' shares: 2^-12."""
+import math
+
 import pytest
 import torch
 
@@ -669,3 +671,30 @@ def test_gated_linear_from_a_thread_that_made_no_cuda_call():
     t.start()
     t.join()
     assert len(got) == 1 and torch.equal(got[0], want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gated_linear_activation_in_its_tails(act, dtype):
+    """One projection is g itself, the other 1: act(g) and act'(g) element by element, where act is tiny too.
+    bfloat16: the result's rounding (2^-9) once, and less than that of the functions' errors; float: erfc's
+    relative error per rounding of its argument, 2^-24 g^2 (81 at g = -9), twice, and some roundings."""
+    g = torch.linspace(-9, 9, 3 * 128 + 5, device="cuda").to(dtype)
+    x = torch.zeros(len(g), 16, device="cuda", dtype=dtype)
+    x[:, 0], x[:, 1] = g, 1
+    w = torch.zeros(2, 1, 16, device="cuda", dtype=dtype)
+    w[0, 0, 0] = w[1, 0, 1] = 1
+    x.requires_grad_(True)
+    h = sequence.gated_linear(x, w[0], w[1], activation=act)
+    dx, = torch.autograd.grad(h, x, torch.ones_like(h))
+    r = g.double()
+    if act == "silu":
+        s = torch.sigmoid(r)
+        a, parts = r * s, (s, r * s * (1 - s))
+    else:
+        c = 0.5 * torch.special.erfc(-r * 0.5 ** 0.5)
+        a, parts = r * c, (c, r * torch.exp(-r * r / 2) * (2 * math.pi) ** -0.5)
+    tol = 2.0 ** -8 if dtype == torch.bfloat16 else 200 * 2.0 ** -24
+    assert float(((h.double()[:, 0] - a).abs() / a.abs().clamp(min=1e-30)).max()) < tol
+    size = parts[0].abs() + parts[1].abs()
+    assert float(((dx.double()[:, 0] - sum(parts)).abs() / size).max()) < tol

@@ -195,15 +195,15 @@ int dual(const Plan& p, const Operands& o, int64_t rows, int d, int f, int act, 
                                 : gemm::launch<T, MODE, nt, TMPC_ACT_GELU, CG>(maps, q, st);
   };
   using One = std::integral_constant<int, 1>;
-  // Wide tiles where they fill the SMs (of pairs of blocks in the bfloat16 forward
-  // pass: 777 against 819 us for 308224 x 512 x 1365; where the epilogue is longer
-  // than the products they cost more than they give, 991 against 968 us for dg | du
-  // and 27.5 against 22.1 us for d = 64); for few tokens narrow ones, so that the
-  // columns spread over more SMs.
+  // Wide tiles where they fill the SMs; for few tokens narrow ones, so that the
+  // columns spread over more SMs. Pairs of blocks in the bfloat16 forward pass: 698
+  // against 792 us for 308224 x 512 x 1365; with few products per tile its epilogue
+  // is all that counts and they give nothing (16384 rows, d = 256: 33.4 against
+  // 32.4 us), nor for dg | du, whose epilogue is longer (958 against 953 us).
   constexpr int kWide = sizeof(T) == 4 ? 128 : 256;
   const int64_t tiles = ((rows + gemm::BM - 1) / gemm::BM) * ((cols + kWide / 2 - 1) / (kWide / 2));
   if constexpr (sizeof(T) == 2 && MODE == gemm::kAct)
-    if (tiles >= sm_count() && d >= 256) return run(std::integral_constant<int, kWide>{}, std::integral_constant<int, 2>{});
+    if (tiles >= sm_count() && d > 256) return run(std::integral_constant<int, kWide>{}, std::integral_constant<int, 2>{});
   if (tiles >= sm_count()) return run(std::integral_constant<int, kWide>{}, One{});
   return run(std::integral_constant<int, 64>{}, One{});
 }

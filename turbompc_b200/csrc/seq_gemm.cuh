@@ -87,9 +87,27 @@ __device__ __forceinline__ void activation(float g, float& a, float& da) {
     a = g * s;
     da = s * (1.f + g * (1.f - s));
   } else {
-    const float c = 0.5f * erfcf(-0.70710678118654752f * g);
+    float c, e;
+    if constexpr (FAST) {
+      // With x = |g| / sqrt 2: erfc(x) / 2 = exp(-x^2) t Q(t), t = 1 / (1 + 0.65 x), where t Q(t) stands for the scaled
+      // function exp(x^2) erfc(x) / 2, smooth in t on (0, 1]; Q of degree 5, fitted for the least relative error
+      // (8e-06 up to x = 9.5, where exp(-x^2) ends). The exponential is the one the derivative needs.
+      e = fast_exp(-0.5f * g * g);
+      const float t = fast_rcp(fmaf(fabsf(g), 0.459619408f, 1.f));
+      float h = 0.0721257154f;
+      h = fmaf(h, t, -0.236653316f);
+      h = fmaf(h, t, 0.178636946f);
+      h = fmaf(h, t, 0.115726972f);
+      h = fmaf(h, t, 0.186977675f);
+      h = fmaf(h, t, 0.183190219f);
+      h *= t * e;
+      c = g < 0.f ? h : 1.f - h;
+    } else {
+      e = expf(-0.5f * g * g);
+      c = 0.5f * erfcf(-0.70710678118654752f * g);
+    }
     a = g * c;
-    da = c + g * 0.39894228040143268f * (FAST ? fast_exp(-0.5f * g * g) : expf(-0.5f * g * g));
+    da = c + g * 0.39894228040143268f * e;
   }
 }
 
@@ -638,6 +656,13 @@ __global__ void __launch_bounds__(Config<T, MODE, NT, CG>::kThreads, 1)
                 if constexpr (kDual) ww[i] = nan;
               }
             }
+            // The accumulator has been read; released before the stores, for which a release to the pair's other
+            // block would wait (698 against 771 us for 308224 x 512 x 1365 forward). dg | du stores by TMA: later there.
+            if (MODE != kDact && c0 + c + 16 == kCols) {
+              fence_before();
+              __syncwarp();
+              if (lane == 0) release(&bar.acc_empty[(accs - 1) & 1]);
+            }
           }
           if constexpr (kDual && MODE == kAct) {
 #pragma unroll
@@ -709,7 +734,7 @@ __global__ void __launch_bounds__(Config<T, MODE, NT, CG>::kThreads, 1)
           *reinterpret_cast<uint32_t*>(stg + lane * F::kStagePitch + CH * 2) = carry >> 16;
         if constexpr (MODE != kDact) chunk_store<E, CH>(stg, lane, out, p.N, rows, p.N - colw - c0, p.wide);
       }
-      if constexpr (!kFloat) {
+      if constexpr (MODE == kDact && !kFloat) {
         fence_before();
         __syncwarp();
         if (lane == 0) release(&bar.acc_empty[(accs - 1) & 1]);

@@ -22,7 +22,7 @@ namespace seq {
 inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
 // x, w_gate and w_up as bfloat16 components [components][rows][pitch], one launch:
-// rows 0 .. n0 - 1 are x's, the next f w_gate's, the last f w_up's.  Four columns
+// rows 0 .. n0 - 1 are x's, the next f w_gate's, the last f w_up's.  Eight columns
 // per thread.
 template <typename T>
 struct PackArgs {
@@ -35,35 +35,37 @@ struct PackArgs {
 
 template <typename T>
 __global__ void __launch_bounds__(256) pack_kernel(const PackArgs<T> a) {
-  const uint32_t groups = (a.cols + 3) / 4;
+  const uint32_t groups = (a.cols + 7) / 8;
   const int64_t n = (a.rows[0] + a.rows[1] + a.rows[2]) * groups;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     int64_t r = n >> 32 ? i / groups : (uint32_t)i / groups;
-    const int c = (int)(i - r * groups) * 4;
+    const int c = (int)(i - r * groups) * 8;
     int w = 0;
     if (r >= a.rows[0]) r -= a.rows[0], w = 1;
     if (w == 1 && r >= a.rows[1]) r -= a.rows[1], w = 2;
     const T* src = a.src[w] + r * a.cols + c;
-    bf16* dst = a.dst[w] + r * a.pitch + c;  // 8-byte aligned: the pitch is a multiple of 8
-    Pack<T, 4> v;
-    if (a.wide) {
-      v = *reinterpret_cast<const Pack<T, 4>*>(src);
+    bf16* dst = a.dst[w] + r * a.pitch + c;  // 16-byte aligned: the pitch is a multiple of 8
+    alignas(16) Pack<T, 4> v[2];
+    if (a.wide) {  // the columns are a multiple of 4
+      v[0] = *reinterpret_cast<const Pack<T, 4>*>(src);
+      if (c + 4 < a.cols) v[1] = *reinterpret_cast<const Pack<T, 4>*>(src + 4);
+      else v[1] = Pack<T, 4>{};
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v.v[e] = c + e < a.cols ? src[e] : from_f<T>(0.f);
+      for (int e = 0; e < 8; ++e) v[e / 4].v[e % 4] = c + e < a.cols ? src[e] : from_f<T>(0.f);
     }
     if constexpr (sizeof(T) == 2) {
-      *reinterpret_cast<Pack<T, 4>*>(dst) = v;
+      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
     } else {
-      Pack<bf16, 4> o[3];
+      Pack<bf16, 8> o[3];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < 8; ++e) {
         bf16 s[3];
-        gemm::split3(v.v[e], s);
+        gemm::split3(v[e / 4].v[e % 4], s);
         o[0].v[e] = s[0], o[1].v[e] = s[1], o[2].v[e] = s[2];
       }
 #pragma unroll
-      for (int k = 0; k < 3; ++k) *reinterpret_cast<Pack<bf16, 4>*>(dst + k * a.rows[w] * a.pitch) = o[k];
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<Pack<bf16, 8>*>(dst + k * a.rows[w] * a.pitch) = o[k];
     }
   }
 }
@@ -160,7 +162,7 @@ Operands pack_operands(const Plan& p, int64_t rows, int d, int f, const T* x, co
   if (p.direct) return {x, wg, wu};
   auto at = [&](int64_t off) { return reinterpret_cast<bf16*>(ws + off); };
   const PackArgs<T> a{{x, wg, wu}, {at(p.x), at(p.wg), at(p.wu)}, {rows, f, f}, d, p.dp, d % 4 == 0};
-  const int64_t blocks = std::min<int64_t>(((rows + 2 * (int64_t)f) * ((d + 3) / 4) + 255) / 256, 16 * (int64_t)sm_count());
+  const int64_t blocks = std::min<int64_t>(((rows + 2 * (int64_t)f) * ((d + 7) / 8) + 255) / 256, 16 * (int64_t)sm_count());
   pack_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(a);
   return {at(p.x), at(p.wg), at(p.wu)};
 }

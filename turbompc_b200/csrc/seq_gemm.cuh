@@ -77,35 +77,55 @@ __device__ __forceinline__ float fast_rcp(float x) {
   return y;
 }
 
-// act(g) and act'(g).  FAST: with the functions above, whose errors vanish in
-// bfloat16 results.
+// 1 / x for finite x >= 1, to the last place or two (0 past 2^126): the hardware's and one Newton step.
+__device__ __forceinline__ float newton_rcp(float x) {
+  const float r = fast_rcp(x);
+  return fmaf(r, fmaf(-x, r, 1.f), r);
+}
+
+// act(g) and act'(g).  FAST: with the hardware's functions alone, whose errors
+// vanish in bfloat16 results.
+//
+// GELU, with x = |g| / sqrt 2: erfc(x) / 2 = exp(-x^2) t Q(t), t = 1 / (1 + p x).
+// t Q(t) stands for exp(x^2) erfc(x) / 2, which is smooth in t on (0, 1]; Q is
+// fitted for the least relative error up to x = 9.5, where exp(-x^2) ends: degree
+// 5 with p = 0.65 (8e-6) for bfloat16, degree 8 with p = 0.3 (1e-7) for float.  The
+// exponential is the one that the derivative needs.  Against erfc: 775 against 1155
+// us forward in bfloat16 (308224 x 512 x 1365), 33 against 37 in float (15616 x 128 x 341).
 template <int ACT, bool FAST>
 __device__ __forceinline__ void activation(float g, float& a, float& da) {
   if constexpr (ACT == TMPC_ACT_SILU) {
-    // exp(-g) is infinite for g < -88 and s = 0 then, as it is in the limit
-    const float s = FAST ? fast_rcp(1.f + fast_exp(-g)) : 1.f / (1.f + expf(-g));
+    // exp(-g) overflows for g < -88 and s = 0 then, as it is in the limit; the Newton step wants it finite
+    const float s = FAST ? fast_rcp(1.f + fast_exp(-g)) : newton_rcp(1.f + fminf(expf(-g), 3e38f));
     a = g * s;
     da = s * (1.f + g * (1.f - s));
   } else {
-    float c, e;
+    float e, h;
     if constexpr (FAST) {
-      // With x = |g| / sqrt 2: erfc(x) / 2 = exp(-x^2) t Q(t), t = 1 / (1 + 0.65 x), where t Q(t) stands for the scaled
-      // function exp(x^2) erfc(x) / 2, smooth in t on (0, 1]; Q of degree 5, fitted for the least relative error
-      // (8e-06 up to x = 9.5, where exp(-x^2) ends). The exponential is the one the derivative needs.
       e = fast_exp(-0.5f * g * g);
       const float t = fast_rcp(fmaf(fabsf(g), 0.459619408f, 1.f));
-      float h = 0.0721257154f;
+      h = 0.0721257154f;
       h = fmaf(h, t, -0.236653316f);
       h = fmaf(h, t, 0.178636946f);
       h = fmaf(h, t, 0.115726972f);
       h = fmaf(h, t, 0.186977675f);
       h = fmaf(h, t, 0.183190219f);
       h *= t * e;
-      c = g < 0.f ? h : 1.f - h;
     } else {
       e = expf(-0.5f * g * g);
-      c = 0.5f * erfcf(-0.70710678118654752f * g);
+      const float t = newton_rcp(fmaf(fminf(fabsf(g), 1e18f), 0.212132034f, 1.f));
+      h = -0.0602559337f;
+      h = fmaf(h, t, 0.221752821f);
+      h = fmaf(h, t, -0.214577258f);
+      h = fmaf(h, t, 0.228558212f);
+      h = fmaf(h, t, -0.0176283418f);
+      h = fmaf(h, t, 0.095508394f);
+      h = fmaf(h, t, 0.0770480731f);
+      h = fmaf(h, t, 0.0849793318f);
+      h = fmaf(h, t, 0.0846147539f);
+      h *= t * e;
     }
+    const float c = g < 0.f ? h : 1.f - h;
     a = g * c;
     da = c + g * 0.39894228040143268f * e;
   }

@@ -4,11 +4,14 @@
 // Operands are bfloat16 arrays [component][outer][inner] read by TMA in
 // swizzled boxes.  bfloat16 tensors have one component.  A float tensor is held
 // as three, x = c0 + c1 + c2 exactly (8 mantissa bits each, by truncation), and
-// a float product is the sum of the six component products above 2^-24, the
-// smallest first.  The tensor cores' accumulation does not round to nearest:
-// over one accumulator a float product of 128 terms came out 4.4e-6 off.  So for
-// float every 32 terms get an accumulator of their own, which the epilogue
-// warps add up in registers.
+// a float product is the sum of the six component products above 2^-24.  The
+// tensor cores' accumulation does not round to nearest: with everything in one
+// accumulator a float product of 128 terms came out 4.4e-6 off.  So for float the
+// five small products have an accumulator of their own, where the error is 2^-8 of
+// that, and the large one gets a new accumulator every 128 terms, which the
+// epilogue warps add up in registers: 3.3e-7 off, as a float matrix product is.
+// Every 32 terms it would be 2.3e-7, but 165 instead of 148 us in the kernels
+// for 15616 x 128 x 341 forward and backward.
 //
 // A block (CG = 1) computes 128 x NT tiles, a pair of blocks (CG = 2) 256 x NT ones:
 // each holds its own 128 rows of A, half of B and 128 rows of the accumulator,
@@ -431,7 +434,8 @@ struct Config {
   static constexpr int kEpi = EW * (kStoreBytes + kPad);
   static constexpr int kFit = (kSmemTotal - 2048 - kEpi) / kStage;
   static constexpr int ST = kFit > 8 ? 8 : kFit;
-  static constexpr int kSeg = kFloat ? 1 : 1 << 30;         // blocks of K per accumulator
+  static constexpr int kSeg = kFloat ? 4 : 1 << 30;         // blocks of K per accumulator
+  static constexpr int kTmem = (kFloat ? 4 : 2) * NT;       // columns: two accumulators; float: two more, the small products'
   static_assert(ST >= 2, "");
 };
 
@@ -467,12 +471,12 @@ __global__ void __launch_bounds__(Config<T, MODE, NT, CG>::kThreads, 1)
   if (warp == 2) {
     if constexpr (CG == 1) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar.tmem)),
-                   "n"(2 * NT)
+                   "n"(F::kTmem)
                    : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     } else {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar.tmem)),
-                   "n"(2 * NT)
+                   "n"(F::kTmem)
                    : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
@@ -541,10 +545,11 @@ __global__ void __launch_bounds__(Config<T, MODE, NT, CG>::kThreads, 1)
   } else if (warp == 1 && rank == 0) {  // products
     int64_t m0;
     int n0, kb0, kb1, split;
-    uint32_t n = 0, accs = 0;
+    uint32_t n = 0, accs = 0, turn = 0;
     bool ok = true;
-    for (int64_t t = first; ok && t < p.tiles; t += step) {
+    for (int64_t t = first; ok && t < p.tiles; t += step, turn ^= 1) {
       tile_of(t, m0, n0, kb0, kb1, split);
+      const uint32_t small = tmem + (2 + turn) * NT;
       for (int seg = kb0; ok && seg < kb1; seg = kb1 - seg > F::kSeg ? seg + F::kSeg : kb1, ++accs) {
         const int end = kb1 - seg > F::kSeg ? seg + F::kSeg : kb1;
         const uint32_t buf = accs & 1, d = tmem + buf * NT;
@@ -562,8 +567,9 @@ __global__ void __launch_bounds__(Config<T, MODE, NT, CG>::kThreads, 1)
             const uint64_t da = smem_desc<BK>(a + ca * kA, kAmn), db = smem_desc<BK>(b + cb * kB, kBmn);
 #pragma unroll
             for (int k = 0; k < BK / 16; ++k)  // 16 K elements: 32 bytes of a K-major row, 16 rows of an MN-major box
-              mma_f16<CG>(d, da + k * ((kAmn ? 2048 : 32) >> 4), db + k * ((kBmn ? 2048 : 32) >> 4), kIdesc,
-                          kb > seg || term > (kFloat ? 0 : 5) || k > 0);
+              mma_f16<CG>(kFloat && term < 5 ? small : d, da + k * ((kAmn ? 2048 : 32) >> 4),
+                          db + k * ((kBmn ? 2048 : 32) >> 4), kIdesc,
+                          k > 0 || (kFloat && term < 5 ? term > 0 || kb > kb0 : kb > seg));
           }
           mma_commit<CG>(&bar.empty[s]);
         }
@@ -586,12 +592,15 @@ __global__ void __launch_bounds__(Config<T, MODE, NT, CG>::kThreads, 1)
     int n0, kb0, kb1, split;
     uint32_t accs = 0;
     bool ok = true;
+    // Float: the small products' accumulator, the other one from tile to tile.  It is free again when the tile's last
+    // accumulator is, which the products of the tile after the next have waited for.
+    uint32_t turn = 0;
     const float nan = __int_as_float(0x7fffffff);
     auto release = [&](uint64_t* w) {
       if (CG == 1) mbar_arrive(w);
       else mbar_arrive_remote(peer_addr(w, 0));
     };
-    for (int64_t t = first; t < p.tiles; t += step) {
+    for (int64_t t = first; t < p.tiles; t += step, turn ^= 1) {
       if (F::kSets == 2 && (int)(accs & 1) != set) {  // one accumulator per tile: the other set's
         ++accs;
         continue;
@@ -633,6 +642,21 @@ __global__ void __launch_bounds__(Config<T, MODE, NT, CG>::kThreads, 1)
               for (int i = 0; i < 16; ++i) {
                 v[c + i] += x[i];
                 if constexpr (kDual) w[c + i] += y[i];
+              }
+            }
+            if (kb1 - seg <= F::kSeg) {  // the tile's last: the small products
+              const uint32_t small = tmem + ((uint32_t)(quad * 32) << 16) + (2 + turn) * NT + group * kCols;
+#pragma unroll
+              for (int c = 0; c < kCols; c += 16) {
+                float x[16], y[16];
+                tmem_ld16(small + c, x);
+                if constexpr (kDual) tmem_ld16(small + NT / 2 + c, y);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  v[c + i] += x[i];
+                  if constexpr (kDual) w[c + i] += y[i];
+                }
               }
             }
           } else {
@@ -764,17 +788,23 @@ __global__ void __launch_bounds__(Config<T, MODE, NT, CG>::kThreads, 1)
         // kCols elements, permuted as the map's swizzle does.
         constexpr int kRow = kCols * 2, U = kRow / 16;
         const int sw = kRow == 128 ? lane & 7 : kRow == 64 ? (lane >> 1) & 3 : (lane >> 2) & 1;
+        // Float: two boxes in turn, six stores a tile; a box is filled while the one before it is read.
+        int half = 0;
         auto box_store = [&](const uint32_t* words, int col, int comp) {
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          char* box = tst + (kFloat ? half ^= 32 * kRow : 0);
+          if (lane == 0) {
+            if constexpr (kFloat) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          }
           __syncwarp();
 #pragma unroll
           for (int u = 0; u < U; ++u)
-            *reinterpret_cast<uint4*>(tst + lane * kRow + ((u ^ sw) * 16)) =
+            *reinterpret_cast<uint4*>(box + lane * kRow + ((u ^ sw) * 16)) =
                 make_uint4(words[4 * u], words[4 * u + 1], words[4 * u + 2], words[4 * u + 3]);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0 && rows > 0 && colw < p.fp) {
-            tma_store_3d(&maps.c, col, (int)row0, comp, tst);
+            tma_store_3d(&maps.c, col, (int)row0, comp, box);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
         };
@@ -814,9 +844,9 @@ __global__ void __launch_bounds__(Config<T, MODE, NT, CG>::kThreads, 1)
   fence_after();
   if (warp == 2) {
     if constexpr (CG == 1)
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(2 * NT) : "memory");
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(F::kTmem) : "memory");
     else
-      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(2 * NT) : "memory");
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(F::kTmem) : "memory");
   }
 }
 

@@ -169,6 +169,8 @@ def load_sequence():
     """The module that makes the sequence operators' calls, bound to the
     library's entry points (both built first if needed)."""
     global _sequence
+    import torch  # noqa: F401  (the libraries that the module is linked to)
+
     lib = load()
     with _lock:
         if _sequence is None:

@@ -37,6 +37,8 @@ struct PackArgs {
 
 template <typename T>
 __global__ void __launch_bounds__(256) pack_kernel(const PackArgs<T> a) {
+  // The products' kernel may set itself up meanwhile; it waits for this one before it reads.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t groups = (a.cols + 7) / 8;
   const int64_t n = (a.rows[0] + a.rows[1] + a.rows[2]) * groups;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
@@ -195,8 +197,8 @@ int dual(const Plan& p, const Operands& o, int64_t rows, int d, int f, int act, 
     if (rc) return rc;
     q.mtiles = (int)((rows + CG * gemm::BM - 1) / (CG * gemm::BM));
     q.ntiles = (cols + nt / 2 - 1) / (nt / 2);
-    return act == TMPC_ACT_SILU ? gemm::launch<T, MODE, nt, TMPC_ACT_SILU, CG>(maps, q, st)
-                                : gemm::launch<T, MODE, nt, TMPC_ACT_GELU, CG>(maps, q, st);
+    return act == TMPC_ACT_SILU ? gemm::launch<T, MODE, nt, TMPC_ACT_SILU, CG>(maps, q, st, !p.direct)
+                                : gemm::launch<T, MODE, nt, TMPC_ACT_GELU, CG>(maps, q, st, !p.direct);
   };
   using One = std::integral_constant<int, 1>;
   // Wide tiles where they fill the SMs; for few tokens narrow ones, so that the
